@@ -191,9 +191,8 @@ def _rows(gen, shape, dtype):
 def _encode(x):
     """4-bit codes, two a byte (the even channel in the low half), and (scale, zero) in fp16, a row of x."""
     x = x.float()
-    low, high = x.amin(-1), x.amax(-1)
-    zero = low.clamp(-FP16_MAX, FP16_MAX).half()
-    scale = ((high - low) * (1.0 / 15.0)).clamp(max=FP16_MAX).half()
+    low, high = (y.clamp(-FP16_MAX, FP16_MAX) for y in (x.amin(-1), x.amax(-1)))
+    zero, scale = low.half(), ((high - low) * (1.0 / 15.0)).half()
     step, start = scale.float()[..., None], zero.float()[..., None]
     code = torch.round((x - start) / step)
     code = torch.where(step > 0, code, torch.zeros_like(code)).clamp(0, 15).to(torch.uint8)
