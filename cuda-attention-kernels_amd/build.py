@@ -21,7 +21,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB_OUT = os.path.join(HERE, "fused_attn", "libfused_attn_hip.so")
-SOURCES = ["fa_prefill.hip", "fa_prefill_f32.hip", "fa_splitk.hip", "fa_generic.hip", "fa_quant.hip", "fa_abi.cpp"]
+SOURCES = ["fa_prefill.hip", "fa_prefill_f32.hip", "fa_splitk.hip", "fa_generic.hip", "fa_quant.hip", "fa_int4.hip",
+           "fa_cache.hip", "fa_evict.hip", "fa_abi.cpp"]
 # the matrix-core ceiling probe bench.py times beside the prefill workload: a library of its own
 PROBE_SOURCES = ["fa_ceiling.hip"]
 PROBE_OUT = os.path.join(HERE, "fused_attn", "libfa_probe.so")
@@ -45,7 +46,7 @@ COMMON = [
 # (D=256, B=16 Hq=64 Hkv=8: FP8 decode over 16384 keys 271 -> 234 us; fp32 prefill, 2 x 4 heads, 2048 x 2048:
 # 630 -> 601).  The 16-bit prefill keeps the default: it measured 5-7% slower at D=256 with it.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-EXTRA = {"fa_splitk.hip": VGPR_FORM, "fa_prefill_f32.hip": VGPR_FORM}
+EXTRA = {"fa_splitk.hip": VGPR_FORM, "fa_prefill_f32.hip": VGPR_FORM, "fa_cache.hip": VGPR_FORM}
 
 
 def _run(cmd: list[str]) -> None:

@@ -99,6 +99,97 @@ fa_status validate(const fa_fwd_params* p, bool varlen, bool fp8_ok, bool generi
   return FA_OK;
 }
 
+// Rows of a 4-bit cache; *empty: nothing to do.
+fa_status validate_int4(const fa_int4_params* p, bool* empty) {
+  if (p->batch < 0 || p->heads < 0 || p->seqlen < 0) return fail(FA_ERR_INVALID_ARGUMENT, "sizes must be non-negative");
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(FA_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+  if (p->dtype != FA_DTYPE_F32 && p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16)
+    return fail(FA_ERR_UNSUPPORTED, "x must be float32, float16 or bfloat16");
+  *empty = p->batch == 0 || p->heads == 0 || p->seqlen == 0;
+  if (*empty) return FA_OK;
+  if (p->x == nullptr || p->codes == nullptr || p->scale == nullptr)
+    return fail(FA_ERR_INVALID_ARGUMENT, "x, codes and scale must be non-NULL");
+  if (p->x_stride_b < 0 || p->x_stride_h < 0 || p->x_stride_n < 0 || p->codes_stride_b < 0 || p->codes_stride_h < 0 ||
+      p->codes_stride_n < 0 || p->scale_stride_b < 0 || p->scale_stride_h < 0 || p->scale_stride_n < 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "negative stride");
+  const int64_t vec = 16 / (int64_t)dtype_bytes(p->dtype);
+  if (!aligned(p->x, 16) || p->x_stride_b % vec || p->x_stride_h % vec || p->x_stride_n % vec)
+    return fail(FA_ERR_INVALID_ARGUMENT, "x must be 16-byte aligned with strides of whole 16 bytes");
+  if (!aligned(p->codes, 4) || p->codes_stride_b % 4 || p->codes_stride_h % 4 || p->codes_stride_n % 4 ||
+      !aligned(p->scale, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "codes must be 4-byte aligned with strides of whole words, scale 4-byte aligned");
+  return FA_OK;
+}
+
+fa_status int4_rows(const fa_int4_params* p, bool read, void* stream) {
+  g_last_error.clear();
+  if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  bool empty = false;
+  fa_status st = validate_int4(p, &empty);
+  if (st != FA_OK || empty) return st;
+  const char* err = nullptr;
+  st = fa::run_int4_rows(*p, read, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+fa_status validate_cache(const fa_cache_params* p, int32_t split_len) {
+  if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->batch < 0 || p->heads_q <= 0 || p->heads_kv <= 0 || p->seqlen_q < 0 || p->seqlen_k < 0 || p->head_dim <= 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "sizes must be non-negative (heads and head_dim positive)");
+  if (p->seqlen_k > (1 << 30)) return fail(FA_ERR_UNSUPPORTED, "seqlen_k must be at most 2^30");
+  if (p->heads_q % p->heads_kv != 0) return fail(FA_ERR_INVALID_ARGUMENT, "H_q must be a multiple of H_kv");
+  if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16)
+    return fail(FA_ERR_UNSUPPORTED, "q/o dtype must be float16 or bfloat16");
+  const bool i4 = p->kv_dtype == FA_DTYPE_INT4, paged = p->block_table != nullptr;
+  if (!i4 && p->kv_dtype != p->dtype) return fail(FA_ERR_INVALID_ARGUMENT, "k/v must be 4-bit codes or have q's dtype");
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(FA_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+  if (!(p->scale - p->scale == 0.f)) return fail(FA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (split_len <= 0 || split_len % 64 != 0 || split_len > (1 << 30))
+    return fail(FA_ERR_INVALID_ARGUMENT, "split_len must be a positive multiple of 64, at most 2^30");
+  if (!i4 && (p->scores_out == nullptr || paged))
+    return fail(FA_ERR_UNSUPPORTED, "a 16-bit cache is served here for its scores only, dense");
+  if (paged && p->scores_out != nullptr) return fail(FA_ERR_UNSUPPORTED, "scores need a dense cache");
+  if (p->batch == 0 || p->seqlen_q == 0) return FA_OK;
+  if (p->q == nullptr || p->o == nullptr || (p->seqlen_k > 0 && (p->k == nullptr || p->v == nullptr)))
+    return fail(FA_ERR_INVALID_ARGUMENT, "q, k, v and o must be non-NULL");
+  if (i4 && p->seqlen_k > 0 && (p->k_scale == nullptr || p->v_scale == nullptr))
+    return fail(FA_ERR_INVALID_ARGUMENT, "a 4-bit cache needs k_scale and v_scale");
+  if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->o, 8) || !aligned(p->k_scale, 4) ||
+      !aligned(p->v_scale, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "q/k/v must be 16-byte, o 8-byte and the scales 4-byte aligned");
+  if (p->q_stride_b % 8 || p->q_stride_h % 8 || p->q_stride_n % 8)
+    return fail(FA_ERR_INVALID_ARGUMENT, "q strides must be multiples of 16 bytes");
+  const int64_t kvb = i4 ? 1 : 2, vec = 16 / kvb;
+  if (p->k_stride_b % vec || p->k_stride_h % vec || p->k_stride_n % vec || p->v_stride_b % vec || p->v_stride_h % vec ||
+      p->v_stride_n % vec)
+    return fail(FA_ERR_INVALID_ARGUMENT, "k/v strides must be multiples of 16 bytes");
+  if (p->o_stride_b % 4 || p->o_stride_h % 4 || p->o_stride_n % 4)
+    return fail(FA_ERR_INVALID_ARGUMENT, "o strides must be multiples of 8 bytes");
+  // tiles of 32 rows are addressed with 32-bit byte offsets
+  if (p->k_stride_n < 0 || p->v_stride_n < 0 || p->k_stride_n * kvb >= (1 << 24) || p->v_stride_n * kvb >= (1 << 24))
+    return fail(FA_ERR_UNSUPPORTED, "k/v token stride must be below 16 MiB");
+  if (p->lse != nullptr && (p->lse_stride_b < 0 || p->lse_stride_h < 0))
+    return fail(FA_ERR_INVALID_ARGUMENT, "negative LSE stride");
+  if (!aligned(p->scores_in, 4) || !aligned(p->scores_out, 4) || !aligned(p->seqlens_k, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "scores and seqlens_k must be 4-byte aligned");
+  if (paged) {
+    if (p->seqlens_k == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "block_table and seqlens_k must be non-NULL");
+    if (p->page_size <= 0 || p->page_size % 16 != 0 || p->page_size > FA_MAX_PAGE_SIZE)
+      return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 16, at most 2^24 keys");
+    if (p->num_pages <= 0 || p->block_table_cols < 0) return fail(FA_ERR_INVALID_ARGUMENT, "the pool needs a page");
+    if (p->batch > 1 && p->block_table_stride < p->block_table_cols)
+      return fail(FA_ERR_INVALID_ARGUMENT, "block_table rows overlap (stride below cols)");
+    if ((int64_t)p->block_table_cols * p->page_size < p->seqlen_k)
+      return fail(FA_ERR_INVALID_ARGUMENT, "block_table has fewer pages per sequence than seqlen_k needs");
+    if (p->k_stride_b < 0 || p->v_stride_b < 0) return fail(FA_ERR_INVALID_ARGUMENT, "negative page stride");
+    if (!aligned(p->block_table, 4)) return fail(FA_ERR_INVALID_ARGUMENT, "block_table must be 4-byte aligned");
+  }
+  return FA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -316,5 +407,100 @@ fa_status fa_quantize_kv_fp8(const fa_quant_params* p, void* stream) {
 }
 
 int32_t fa_abi_version(void) { return FA_ABI_VERSION; }
+
+fa_status fa_quantize_kv_int4(const fa_int4_params* p, void* stream) { return int4_rows(p, false, stream); }
+fa_status fa_dequantize_kv_int4(const fa_int4_params* p, void* stream) { return int4_rows(p, true, stream); }
+
+fa_status fa_append_kv_int4(const fa_int4_append_params* p, void* stream) {
+  g_last_error.clear();
+  if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  bool empty = false;
+  for (const fa_int4_params* t : {&p->k, &p->v}) {
+    const fa_status st = validate_int4(t, &empty);
+    if (st != FA_OK) return st;
+  }
+  if (p->k.batch != p->v.batch || p->k.heads != p->v.heads || p->k.seqlen != p->v.seqlen ||
+      p->k.head_dim != p->v.head_dim || p->k.dtype != p->v.dtype)
+    return fail(FA_ERR_INVALID_ARGUMENT, "k and v must have the same sizes and dtype");
+  if (p->block_table != nullptr) {
+    if (p->page_size <= 0 || p->page_size > FA_MAX_PAGE_SIZE)
+      return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be positive and at most 2^24 keys");
+    if (p->num_pages < 0 || p->block_table_cols < 0) return fail(FA_ERR_INVALID_ARGUMENT, "negative page count");
+    if (p->k.batch > 1 && p->block_table_stride < p->block_table_cols)
+      return fail(FA_ERR_INVALID_ARGUMENT, "block_table rows overlap (stride below cols)");
+    if (!aligned(p->block_table, 4)) return fail(FA_ERR_INVALID_ARGUMENT, "block_table must be 4-byte aligned");
+  } else if (p->capacity < 0) {
+    return fail(FA_ERR_INVALID_ARGUMENT, "negative capacity");
+  }
+  if (empty) return FA_OK;
+  if (p->seqlens_k == nullptr || !aligned(p->seqlens_k, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "seqlens_k must be non-NULL and 4-byte aligned");
+  const char* err = nullptr;
+  const fa_status st = fa::run_append_int4(*p, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+size_t fa_attention_cache_workspace_bytes(const fa_cache_params* p, int32_t split_len) {
+  g_last_error.clear();
+  if (validate_cache(p, split_len) != FA_OK) return 0;
+  if (p->batch == 0 || p->seqlen_q == 0) return 0;
+  return fa::cache_workspace_bytes(*p, split_len);
+}
+
+fa_status fa_attention_cache(const fa_cache_params* p, int32_t split_len, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  g_last_error.clear();
+  fa_status st = validate_cache(p, split_len);
+  if (st != FA_OK) return st;
+  // (without queries scores_out still takes scores_in: the caller's copy, as there is nothing to add)
+  if (p->batch == 0 || p->seqlen_q == 0) return FA_OK;
+  const size_t need = fa::cache_workspace_bytes(*p, split_len);
+  if (workspace == nullptr || workspace_bytes < need) {
+    char buf[160];
+    snprintf(buf, sizeof(buf), "cache attention workspace too small: need %zu bytes, got %zu", need,
+             workspace == nullptr ? (size_t)0 : workspace_bytes);
+    return fail(FA_ERR_WORKSPACE, buf);
+  }
+  if (!aligned(workspace, 16)) return fail(FA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  const char* err = nullptr;
+  st = fa::run_cache(*p, split_len, workspace, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+fa_status fa_evict_kv(const fa_evict_params* p, void* stream) {
+  g_last_error.clear();
+  if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->batch < 0 || p->heads < 0 || p->seqlen < 0 || p->seqlen > (1 << 30))
+    return fail(FA_ERR_INVALID_ARGUMENT, "sizes must be non-negative, seqlen at most 2^30");
+  if (p->recent < 0 || p->recent > p->keep || p->keep > p->seqlen)
+    return fail(FA_ERR_INVALID_ARGUMENT, "need 0 <= recent <= keep <= seqlen");
+  if (p->num_tensors < 0 || p->num_tensors > FA_MAX_EVICT_TENSORS)
+    return fail(FA_ERR_INVALID_ARGUMENT, "num_tensors must be 0 to 8");
+  if (p->batch == 0 || p->heads == 0) return FA_OK;
+  if (p->seqlens_out == nullptr || !aligned(p->seqlens_out, 4) || !aligned(p->seqlens_k, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "seqlens_out must be non-NULL, lengths 4-byte aligned");
+  if (p->seqlen > 0 && p->scores == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "scores must be non-NULL");
+  if (p->keep > 0 && (p->index == nullptr || p->scores_out == nullptr))
+    return fail(FA_ERR_INVALID_ARGUMENT, "index and scores_out must be non-NULL");
+  if (!aligned(p->scores, 4) || !aligned(p->scores_out, 4) || !aligned(p->index, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "scores, scores_out and index must be 4-byte aligned");
+  if (p->scores_stride_b < 0 || p->scores_stride_h < 0) return fail(FA_ERR_INVALID_ARGUMENT, "negative stride");
+  for (int i = 0; i < p->num_tensors; ++i) {
+    const fa_evict_tensor& t = p->tensors[i];
+    if (t.row_bytes <= 0) return fail(FA_ERR_INVALID_ARGUMENT, "row_bytes must be positive");
+    if (p->keep > 0 && (t.src == nullptr || t.dst == nullptr))
+      return fail(FA_ERR_INVALID_ARGUMENT, "src and dst must be non-NULL");
+    if (t.src_stride_b < 0 || t.src_stride_h < 0 || t.src_stride_n < 0 || t.dst_stride_b < 0 || t.dst_stride_h < 0 ||
+        t.dst_stride_n < 0)
+      return fail(FA_ERR_INVALID_ARGUMENT, "negative stride");
+    if (p->keep > 1 && t.dst_stride_n < t.row_bytes) return fail(FA_ERR_INVALID_ARGUMENT, "dst rows overlap");
+  }
+  const char* err = nullptr;
+  const fa_status st = fa::run_evict(*p, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
 
 }  // extern "C"

@@ -81,6 +81,72 @@ struct CombineArgs {
   int32_t nk, split_len;
 };
 
+// 4-bit rows (fa_int4.hip): floats x, codes (bytes) and (scale, zero) pairs (4-byte words), strides in elements.
+struct Int4Args {
+  const void* x;
+  uint8_t* codes;
+  uint32_t* pairs;
+  int64_t sxb, sxh, sxn, scb, sch, scn, ssb, ssh, ssn;
+  int64_t rows;  // batch * h * n
+  int32_t h, n;
+};
+
+struct AppendArgs {
+  Int4Args k, v;  // scb and ssb: between sequences, or between pages
+  const int32_t* seqlens_k;
+  const int32_t* block_table;  // NULL for a dense cache
+  int64_t sbt, capacity;
+  int32_t page_size, num_pages;
+};
+
+// Attention over a 4-bit cache and scored attention (fa_cache.hip).  Strides in elements of what is pointed to (codes:
+// bytes; pairs: 4-byte words); paged: the batch strides of k, v and their pairs are page strides.
+struct CacheArgs {
+  const void *q, *k, *v, *k_scale, *v_scale;
+  float* part;  // normalised fp32 partials [B, Hq, Nq, S, D]
+  float* ml;    // their (max, sum)
+  float* raw;   // scored: log2-domain scores [B, Hkv, G * Nq, raw_stride]
+  int64_t sqb, sqh, sqn, skb, skh, skn, svb, svh, svn;
+  int64_t sksb, sksh, sksn, svsb, svsh, svsn;
+  int64_t raw_stride, sbt;
+  const int32_t* seqlens_k;
+  const int32_t* block_table;
+  int32_t batch, hq, hkv, group, nq, nk;
+  int32_t n_rowblk, n_split, split_len, n_items, total;
+  int32_t causal, page_size, num_pages, page_magic_shift;
+  uint32_t page_magic;
+  float qk_scale;
+};
+
+struct FinishArgs {
+  const float* raw;
+  const float* lse;
+  const float* in;
+  float* out;
+  int64_t raw_stride, slb, slh, sib, sih, sob, soh;
+  const int32_t* seqlens_k;
+  int32_t hkv, group, nq, nk, causal, chunks;
+};
+
+// Eviction (fa_evict.hip): strides of the tensors in bytes.
+struct EvictTensor {
+  const void* src;
+  void* dst;
+  int64_t sb, sh, sn, db, dh, dn;
+  int32_t unit, units;  // bytes a thread copies, and how many make a row
+  int32_t shift;        // log2(units), -1 if units is no power of two
+};
+struct EvictArgs {
+  const float* scores;
+  int64_t ssb, ssh;
+  const int32_t* seqlens_k;
+  int32_t* index;
+  float* scores_out;
+  int32_t* seqlens_out;
+  int32_t h, nk, keep, recent, chunks;
+  EvictTensor tensors[FA_MAX_EVICT_TENSORS];
+};
+
 // Number of rows (q-heads x queries) one split-K workgroup covers, and the
 // workgroup shape chosen for a given row count G*Nq.
 int splitk_waves_for_rows(int rows);
@@ -114,6 +180,14 @@ fa_status run_quantize_fp8(const fa_quant_params& p, hipStream_t stream, const c
 constexpr size_t kSplitkScratchBytes = size_t{64} << 20;
 // This device's address of that array (looked up once per device), for fa_attention_splitk_noalloc.
 fa_status splitk_scratch(void** ptr, const char** err);
+// The merge of split-K partials (fa_splitk.hip) for head dim d and bf16 or fp16 output.
+fa_status run_combine(const CombineArgs& c, int d, bool bf16, int64_t rows, hipStream_t stream, const char** err);
+// read: floats from codes; else codes from floats
+fa_status run_int4_rows(const fa_int4_params& p, bool read, hipStream_t stream, const char** err);
+fa_status run_append_int4(const fa_int4_append_params& p, hipStream_t stream, const char** err);
+size_t cache_workspace_bytes(const fa_cache_params& p, int32_t split_len);
+fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace, hipStream_t stream, const char** err);
+fa_status run_evict(const fa_evict_params& p, hipStream_t stream, const char** err);
 // kv: paged K/V (nullptr for a dense cache)
 fa_status run_splitk(const fa_fwd_params& p, int32_t split_len, void* workspace, hipStream_t stream,
                      const char** err, const fa_paged_kv* kv = nullptr);

@@ -897,6 +897,18 @@ static hipError_t launch_combine(const CombineArgs& c, int64_t rows, hipStream_t
   return hipGetLastError();
 }
 
+fa_status run_combine(const CombineArgs& c, int d, bool bf, int64_t rows, hipStream_t stream, const char** err) {
+  hipError_t e;
+  if (d == 128) {
+    e = bf ? launch_combine<128, BF16>(c, rows, stream) : launch_combine<128, F16>(c, rows, stream);
+  } else if (d == 256) {
+    e = bf ? launch_combine<256, BF16>(c, rows, stream) : launch_combine<256, F16>(c, rows, stream);
+  } else {
+    e = bf ? launch_combine<64, BF16>(c, rows, stream) : launch_combine<64, F16>(c, rows, stream);
+  }
+  return hip_status(e, err);
+}
+
 TileArgs common_args(const fa_fwd_params& p) {
   TileArgs a{};
   a.q = p.q;
@@ -1094,14 +1106,7 @@ fa_status run_splitk(const fa_fwd_params& p, int32_t split_len, void* workspace,
   c.lse = p.lse;
   c.slb = p.lse_stride_b;
   c.slh = p.lse_stride_h;
-  if (p.head_dim == 128) {
-    e = bf ? launch_combine<128, BF16>(c, out_rows, stream) : launch_combine<128, F16>(c, out_rows, stream);
-  } else if (p.head_dim == 256) {
-    e = bf ? launch_combine<256, BF16>(c, out_rows, stream) : launch_combine<256, F16>(c, out_rows, stream);
-  } else {
-    e = bf ? launch_combine<64, BF16>(c, out_rows, stream) : launch_combine<64, F16>(c, out_rows, stream);
-  }
-  return hip_status(e, err);
+  return run_combine(c, p.head_dim, bf, out_rows, stream, err);
 }
 
 }  // namespace fa

@@ -27,7 +27,7 @@ LIB_NAME = "libfused_attn_hip.so"
 ABI_VERSION = 6
 
 # fa_dtype codes
-F16, BF16, F32, FP8_E4M3 = 0, 1, 2, 3
+F16, BF16, F32, FP8_E4M3, INT4 = 0, 1, 2, 3, 4
 _DTYPE_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
 _FP8 = getattr(torch, "float8_e4m3fn", None)
 if _FP8 is not None:
@@ -122,6 +122,120 @@ class PagedKV(ctypes.Structure):
     ]
 
 
+def _int64s(*names: str) -> list:
+    return [(n, ctypes.c_int64) for n in names]
+
+
+class Int4Params(ctypes.Structure):
+    """Mirror of ``fa_int4_params`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        *_int64s("x_stride_b", "x_stride_h", "x_stride_n"),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("seqlen", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("codes", ctypes.c_void_p),
+        *_int64s("codes_stride_b", "codes_stride_h", "codes_stride_n"),
+        ("scale", ctypes.c_void_p),
+        *_int64s("scale_stride_b", "scale_stride_h", "scale_stride_n"),
+    ]
+
+
+class Int4AppendParams(ctypes.Structure):
+    """Mirror of ``fa_int4_append_params`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("k", Int4Params),
+        ("v", Int4Params),
+        ("seqlens_k", ctypes.c_void_p),
+        ("capacity", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class CacheParams(ctypes.Structure):
+    """Mirror of ``fa_cache_params`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        *_int64s("q_stride_b", "q_stride_h", "q_stride_n", "k_stride_b", "k_stride_h", "k_stride_n", "v_stride_b",
+                 "v_stride_h", "v_stride_n", "o_stride_b", "o_stride_h", "o_stride_n"),
+        ("batch", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("seqlen_q", ctypes.c_int32),
+        ("seqlen_k", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        *_int64s("k_scale_stride_b", "k_scale_stride_h", "k_scale_stride_n", "v_scale_stride_b", "v_scale_stride_h",
+                 "v_scale_stride_n"),
+        ("seqlens_k", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("lse", ctypes.c_void_p),
+        *_int64s("lse_stride_b", "lse_stride_h"),
+        ("scores_in", ctypes.c_void_p),
+        *_int64s("scores_in_stride_b", "scores_in_stride_h"),
+        ("scores_out", ctypes.c_void_p),
+        *_int64s("scores_out_stride_b", "scores_out_stride_h"),
+    ]
+
+
+MAX_EVICT_TENSORS = 8  # FA_MAX_EVICT_TENSORS
+
+
+class EvictTensor(ctypes.Structure):
+    """Mirror of ``fa_evict_tensor`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        *_int64s("src_stride_b", "src_stride_h", "src_stride_n", "dst_stride_b", "dst_stride_h", "dst_stride_n",
+                 "row_bytes"),
+    ]
+
+
+class EvictParams(ctypes.Structure):
+    """Mirror of ``fa_evict_params`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("scores", ctypes.c_void_p),
+        *_int64s("scores_stride_b", "scores_stride_h"),
+        ("seqlens_k", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("seqlen", ctypes.c_int32),
+        ("keep", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("num_tensors", ctypes.c_int32),
+        ("index", ctypes.c_void_p),
+        ("scores_out", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p),
+        ("tensors", EvictTensor * MAX_EVICT_TENSORS),
+    ]
+
+
 _lib = None
 _lib_error: Optional[str] = None
 _lock = threading.Lock()
@@ -134,6 +248,18 @@ def library_path() -> str:
 
 def _has_fwd_workspace(lib: ctypes.CDLL) -> bool:
     return isinstance(getattr(lib, "fa_attention_fwd_ws", None), lib._FuncPtr)
+
+
+def _has_int4(lib: ctypes.CDLL) -> bool:
+    return isinstance(getattr(lib, "fa_attention_cache", None), lib._FuncPtr)
+
+
+def _cache_library() -> ctypes.CDLL:
+    """The library, if it has the 4-bit cache's functions and eviction (added within this ABI version)."""
+    lib = load_library()
+    if not _has_int4(lib):
+        raise RuntimeError(f"fused_attn HIP backend: {library_path()} is older than the 4-bit cache: build it again")
+    return lib
 
 
 def _bind(lib: ctypes.CDLL) -> None:
@@ -163,6 +289,18 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.fa_attention_paged_decode.restype = ctypes.c_int
     lib.fa_quantize_kv_fp8.argtypes = [ctypes.POINTER(QuantParams), ctypes.c_void_p]
     lib.fa_quantize_kv_fp8.restype = ctypes.c_int
+    if _has_int4(lib):
+        for f in (lib.fa_quantize_kv_int4, lib.fa_dequantize_kv_int4):
+            f.argtypes, f.restype = [ctypes.POINTER(Int4Params), ctypes.c_void_p], ctypes.c_int
+        lib.fa_append_kv_int4.argtypes = [ctypes.POINTER(Int4AppendParams), ctypes.c_void_p]
+        lib.fa_append_kv_int4.restype = ctypes.c_int
+        lib.fa_attention_cache_workspace_bytes.argtypes = [ctypes.POINTER(CacheParams), ctypes.c_int32]
+        lib.fa_attention_cache_workspace_bytes.restype = ctypes.c_size_t
+        lib.fa_attention_cache.argtypes = [ctypes.POINTER(CacheParams), ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t,
+                                           ctypes.c_void_p]
+        lib.fa_attention_cache.restype = ctypes.c_int
+        lib.fa_evict_kv.argtypes = [ctypes.POINTER(EvictParams), ctypes.c_void_p]
+        lib.fa_evict_kv.restype = ctypes.c_int
     lib.fa_device_supported.argtypes = [ctypes.c_int32]
     lib.fa_device_supported.restype = ctypes.c_int32
     lib.fa_last_error.argtypes = []
@@ -743,3 +881,317 @@ def quantize_kv_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     with _on_device(x.device):
         _check(lib.fa_quantize_kv_fp8(ctypes.byref(p), ctypes.c_void_p(_stream(x))), "quantize_kv_fp8")
     return x8, scale
+
+
+# ----------------------------------------------------------------------------------------------
+# 4-bit cache, scored attention, eviction
+# ----------------------------------------------------------------------------------------------
+
+INT4_HEAD_DIMS = (64, 128, 256)
+
+
+def _strides3(t: torch.Tensor, unit: int = 1) -> tuple[int, int, int]:
+    return _stride(t, 0) // unit, _stride(t, 1) // unit, _stride(t, 2) // unit
+
+
+def _pairs_ok(t: torch.Tensor) -> bool:
+    """Whether the kernels can read t's (scale, zero) pairs as 4-byte words."""
+    return (t.stride(-1) == 1 and t.data_ptr() % 4 == 0
+            and all(t.size(i) <= 1 or (t.stride(i) >= 0 and t.stride(i) % 2 == 0) for i in range(3)))
+
+
+def check_int4_rows(codes: torch.Tensor, scale: torch.Tensor, name: str, shape=None) -> None:
+    """4-bit rows: uint8 codes [B, Hkv, N, D/2] (or a pool of pages) and fp16 pairs [B, Hkv, N, 2]."""
+    if codes.dim() != 4 or codes.dtype != torch.uint8:
+        raise RuntimeError(f"{name} must be uint8 [B, Hkv, N, D/2], got {codes.dtype} {tuple(codes.shape)}")
+    if shape is not None and tuple(codes.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must have shape {tuple(shape)}, got {tuple(codes.shape)}")
+    want = (*codes.shape[:3], 2)
+    if not isinstance(scale, torch.Tensor) or tuple(scale.shape) != want or scale.dtype != torch.float16:
+        got = f"{scale.dtype} {tuple(scale.shape)}" if isinstance(scale, torch.Tensor) else scale
+        raise RuntimeError(f"the scale of {name} must be float16 {want}, (scale, zero) a row, got {got}")
+    if scale.device != codes.device:
+        raise RuntimeError(f"the scale of {name} must be on {codes.device}, got {scale.device}")
+
+
+def _check_int4_writable(codes: torch.Tensor, scale: torch.Tensor, name: str) -> None:
+    """Rows that are written in place cannot be copied into another layout first."""
+    sizes = range(3)
+    if codes.numel() and (codes.stride(-1) != 1 or codes.data_ptr() % 4
+                          or any(codes.size(i) > 1 and (codes.stride(i) <= 0 or codes.stride(i) % 4) for i in sizes)):
+        raise RuntimeError(f"{name} needs a unit last stride, a 4-byte aligned start and strides of whole 4-byte words")
+    if scale.numel() and not (_pairs_ok(scale) and all(scale.size(i) <= 1 or scale.stride(i) > 0 for i in sizes)):
+        raise RuntimeError(f"the scale of {name} needs a unit last stride, a 4-byte aligned start and even strides")
+
+
+def _int4_params(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> Int4Params:
+    return Int4Params(x.data_ptr(), *_strides3(x), *x.shape, _DTYPE_CODE[x.dtype], 0, codes.data_ptr(), *_strides3(codes),
+                      scale.data_ptr(), *_strides3(scale, 2))
+
+
+def _check_float_rows(x: torch.Tensor, name: str = "x") -> None:
+    if x.dim() != 4 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise RuntimeError(f"{name} must be float32, float16 or bfloat16 [B, Hkv, N, D], got {x.dtype} {tuple(x.shape)}")
+    if x.shape[-1] not in INT4_HEAD_DIMS:
+        raise RuntimeError(f"head_dim must be one of {INT4_HEAD_DIMS}, got {x.shape[-1]}")
+
+
+def quantize_kv_int4(x: torch.Tensor, out=None):
+    """x [B,Hkv,N,D] -> (codes uint8 [B,Hkv,N,D/2], (scale, zero) fp16 [B,Hkv,N,2]), into ``out`` if given."""
+    _check_float_rows(x)
+    shape = (*x.shape[:3], x.shape[3] // 2)
+    if out is not None:
+        codes, scale = out
+        check_int4_rows(codes, scale, "out", shape)
+        _check_int4_writable(codes, scale, "out")
+        _require_gpu(x, codes, scale)
+    else:
+        _require_gpu(x)
+        codes = torch.empty(shape, dtype=torch.uint8, device=x.device)
+        scale = torch.empty((*x.shape[:3], 2), dtype=torch.float16, device=x.device)
+    lib = _cache_library()
+    x = _aligned_view(x, 16 // x.element_size(), 16)
+    with _on_device(x.device):
+        _check(lib.fa_quantize_kv_int4(_int4_params(x, codes, scale), _stream(x)), "quantize_kv_int4")
+    return codes, scale
+
+
+def dequantize_kv_int4(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Values [B,Hkv,N,D] of 4-bit rows."""
+    check_int4_rows(codes, scale, "codes")
+    _require_gpu(codes, scale)
+    x = torch.empty((*codes.shape[:3], 2 * codes.shape[3]), dtype=dtype, device=codes.device)
+    _check_float_rows(x, "the result")
+    lib = _cache_library()
+    codes = _aligned_view(codes, 4, 4)
+    scale = scale if _pairs_ok(scale) else scale.clone(memory_format=torch.contiguous_format)
+    with _on_device(codes.device):
+        _check(lib.fa_dequantize_kv_int4(_int4_params(x, codes, scale), _stream(codes)), "dequantize_kv_int4")
+    return x
+
+
+def check_append(k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, block_table) -> None:
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise RuntimeError(f"k and v must have the same shape and dtype, got {k.dtype} {tuple(k.shape)} and "
+                           f"{v.dtype} {tuple(v.shape)}")
+    if k.dim() != 4:
+        raise RuntimeError(f"k and v must be [B, Hkv, new tokens, D], got {tuple(k.shape)}")
+    b, hkv, _, d = k.shape
+    for name, codes, scale in (("k_cache", k_cache, k_scale), ("v_cache", v_cache, v_scale)):
+        check_int4_rows(codes, scale, name)
+        if codes.shape[1] != hkv or codes.shape[3] * 2 != d or (block_table is None and codes.shape[0] != b):
+            raise RuntimeError(f"{name} {tuple(codes.shape)} does not fit k {tuple(k.shape)}")
+        _check_int4_writable(codes, scale, name)
+    if k_cache.shape != v_cache.shape:
+        raise RuntimeError(f"k_cache and v_cache must have the same shape, got {tuple(k_cache.shape)} and "
+                           f"{tuple(v_cache.shape)}")
+    check_lengths(seqlens_k, b)
+    if block_table is not None:
+        check_block_table(block_table, b)
+
+
+def check_lengths(seqlens_k: torch.Tensor, b: int) -> None:
+    if seqlens_k.dtype != torch.int32 or tuple(seqlens_k.shape) != (b,):
+        raise RuntimeError(f"seqlens_k must be int32 [{b}], got {seqlens_k.dtype} {tuple(seqlens_k.shape)}")
+
+
+def check_block_table(block_table: torch.Tensor, b: int) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b:
+        raise RuntimeError(f"block_table must be int32 [{b}, pages], got {block_table.dtype} {tuple(block_table.shape)}")
+
+
+def _plain_table(block_table: torch.Tensor) -> torch.Tensor:
+    ok = block_table.stride(-1) == 1 and (block_table.shape[0] <= 1 or block_table.stride(0) >= block_table.shape[1])
+    return block_table if ok else block_table.contiguous()
+
+
+def append_kv_int4(k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, block_table=None) -> None:
+    """New tokens k, v [B,Hkv,n,D] into a 4-bit cache in place, at positions seqlens_k[b] .. + n - 1."""
+    check_append(k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, block_table)
+    _check_float_rows(k, "k")
+    _require_gpu(k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, *([] if block_table is None else [block_table]))
+    lib = _cache_library()
+    vec = 16 // k.element_size()
+    k, v = _aligned_view(k, vec, 16), _aligned_view(v, vec, 16)
+    seqlens_k = seqlens_k.contiguous()
+    if k_cache.numel() == 0:
+        return
+    p = Int4AppendParams(_int4_params(k, k_cache, k_scale), _int4_params(v, v_cache, v_scale), seqlens_k.data_ptr(),
+                         k_cache.shape[2])
+    if block_table is not None:
+        if block_table.shape[1] == 0:
+            return
+        block_table = _plain_table(block_table)
+        p.block_table, p.block_table_stride = block_table.data_ptr(), block_table.stride(0)
+        p.block_table_cols, p.page_size, p.num_pages = block_table.shape[1], k_cache.shape[2], k_cache.shape[0]
+    with _on_device(k.device):
+        _check(lib.fa_append_kv_int4(p, _stream(k)), "append_kv_int4")
+
+
+def check_cache_attention(q, k, v, k_scale, v_scale, paged: bool = False) -> bool:
+    """Whether the K/V are 4-bit; raises for operands that do not describe one attention problem."""
+    if q.dim() != 4 or q.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"q must be float16 or bfloat16 [B, Hq, Nq, D], got {q.dtype} {tuple(q.shape)}")
+    int4 = k.dtype == torch.uint8
+    if not int4:
+        _check_qkv(q, k, v, "dense")
+        if k_scale is not None or v_scale is not None:
+            raise RuntimeError("k_scale and v_scale belong to 4-bit K/V (uint8)")
+        return False
+    check_int4_rows(k, k_scale, "k")
+    check_int4_rows(v, v_scale, "v", k.shape)
+    if v.device != k.device:
+        raise RuntimeError(f"all tensors must be on {k.device}, got {v.device}")
+    if k.shape[3] * 2 != q.shape[3]:
+        raise RuntimeError(f"q has head_dim {q.shape[3]}, the 4-bit rows {2 * k.shape[3]}")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1] != 0:
+        raise RuntimeError(f"H_q ({q.shape[1]}) must be a multiple of H_kv ({k.shape[1]})")
+    if not paged and k.shape[0] not in (q.shape[0], 1):
+        raise RuntimeError(f"k/v batch ({k.shape[0]}) must equal q's ({q.shape[0]}) or be 1")
+    return True
+
+
+def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split_len: int, seqlens_k=None,
+                    block_table=None, max_seqlen_k: Optional[int] = None, return_lse: bool = False, scores=None,
+                    return_scores: bool = False):
+    """Attention over a 4-bit cache (dense, or paged with ``block_table``), or scored attention over a dense cache.
+    Returns o, then the LSE and the new scores where asked for."""
+    int4 = check_cache_attention(q, k, v, k_scale, v_scale, paged=block_table is not None)
+    more = [t for t in (k_scale, v_scale, seqlens_k, block_table, scores) if t is not None]
+    _require_gpu(q, k, v, *more)
+    b, hq, nq, d = q.shape
+    hkv = k.shape[1]
+    nk = k.shape[2] if block_table is None else int(max_seqlen_k)
+    if seqlens_k is not None:
+        check_lengths(seqlens_k, b)
+        seqlens_k = seqlens_k.contiguous()
+    if scores is not None:
+        check_scores(scores, (b, hkv, nk))
+        if scores.stride(-1) != 1 and nk > 1 or min(scores.stride(0), scores.stride(1)) < 0:
+            scores = scores.contiguous()
+    lib = _cache_library()
+    q = _aligned_view(q, 8, 16)
+    vec = 16 if int4 else 8
+    k, v = _aligned_view(k, vec, 16), _aligned_view(v, vec, 16)
+    o = _new_output(q)
+    p = CacheParams(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *_strides3(q), *_strides3(k), *_strides3(v),
+                    *_strides3(o), b, hq, hkv, nq, nk, d, float(scale), int(bool(causal)), _DTYPE_CODE[q.dtype],
+                    INT4 if int4 else _DTYPE_CODE[k.dtype])
+    if int4:
+        k_scale, v_scale = (t if _pairs_ok(t) else t.clone(memory_format=torch.contiguous_format)
+                            for t in (k_scale, v_scale))
+        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        p.k_scale_stride_b, p.k_scale_stride_h, p.k_scale_stride_n = _strides3(k_scale, 2)
+        p.v_scale_stride_b, p.v_scale_stride_h, p.v_scale_stride_n = _strides3(v_scale, 2)
+    if seqlens_k is not None:
+        p.seqlens_k = seqlens_k.data_ptr()
+    if block_table is not None:
+        check_block_table(block_table, b)
+        block_table = _plain_table(block_table)
+        p.block_table, p.block_table_stride = block_table.data_ptr(), block_table.stride(0)
+        p.block_table_cols, p.page_size, p.num_pages = block_table.shape[1], k.shape[2], k.shape[0]
+    lse = torch.empty((b, hq, nq), dtype=torch.float32, device=q.device) if return_lse else None
+    if lse is not None:
+        p.lse, p.lse_stride_b, p.lse_stride_h = lse.data_ptr(), lse.stride(0), lse.stride(1)
+    new = None
+    if return_scores:
+        if b * hq * nq == 0:  # no query adds a weight
+            new = torch.zeros((b, hkv, nk), dtype=torch.float32, device=q.device) if scores is None else scores.clone()
+        else:
+            new = torch.empty((b, hkv, nk), dtype=torch.float32, device=q.device)
+        p.scores_out, p.scores_out_stride_b, p.scores_out_stride_h = new.data_ptr(), new.stride(0), new.stride(1)
+        if nk == 0:
+            p.scores_out = o.data_ptr()  # nothing is written: there are no keys
+        if scores is not None:
+            p.scores_in, p.scores_in_stride_b, p.scores_in_stride_h = scores.data_ptr(), scores.stride(0), scores.stride(1)
+    need = lib.fa_attention_cache_workspace_bytes(p, split_len)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    with _on_device(q.device):
+        _check(lib.fa_attention_cache(p, split_len, ws.data_ptr(), need, _stream(q)), "attention_cache")
+    got = (o,) + ((lse,) if return_lse else ()) + ((new,) if return_scores else ())
+    return got if len(got) > 1 else o
+
+
+def check_scores(scores: torch.Tensor, shape) -> None:
+    if scores.dtype != torch.float32 or (shape is not None and tuple(scores.shape) != tuple(shape)):
+        want = "float32" if shape is None else f"float32 {tuple(shape)}"
+        raise RuntimeError(f"scores must be {want} [B, Hkv, Nk], got {scores.dtype} {tuple(scores.shape)}")
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    last = sum((t.size(i) - 1) * t.stride(i) for i in range(t.dim()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
+    if scores.dim() != 3:
+        raise RuntimeError(f"scores must be float32 [B, Hkv, N], got {tuple(scores.shape)}")
+    check_scores(scores, None)
+    if not 0 <= recent <= keep:
+        raise RuntimeError(f"need 0 <= recent <= keep, got recent {recent}, keep {keep}")
+    if len(caches) > MAX_EVICT_TENSORS:
+        raise RuntimeError(f"at most {MAX_EVICT_TENSORS} caches, got {len(caches)}")
+    rows = min(keep, scores.shape[2])
+    for t in caches:
+        if tuple(t.shape[:3]) != tuple(scores.shape):
+            raise RuntimeError(f"a cache must be [B, Hkv, N, ...] as scores {tuple(scores.shape)}, got {tuple(t.shape)}")
+        if t[:1, :1, :1].numel() != math.prod(t.shape[3:]) and scores.numel() or math.prod(t.shape[3:]) == 0:
+            raise RuntimeError(f"a cache needs rows, got {tuple(t.shape)}")
+    if seqlens_k is not None:
+        check_lengths(seqlens_k, scores.shape[0])
+    if out is not None:
+        if len(out) != len(caches):
+            raise RuntimeError(f"out must hold one tensor for each of the {len(caches)} caches, got {len(out)}")
+        for o, t in zip(out, caches):
+            if o.dtype != t.dtype or o.dim() != t.dim() or o.shape[:2] != t.shape[:2] or o.shape[3:] != t.shape[3:] \
+                    or o.shape[2] < rows:
+                raise RuntimeError(f"out for a cache {t.dtype} {tuple(t.shape)} needs its type and at least {rows} rows, "
+                                   f"got {o.dtype} {tuple(o.shape)}")
+            if not _rows_contiguous(o) or any(o.size(i) > 1 and o.stride(i) <= 0 for i in range(3)):
+                raise RuntimeError("out needs contiguous rows and positive strides")
+            if o.size(2) > 1 and o.stride(2) < math.prod(o.shape[3:]):
+                raise RuntimeError("rows of out overlap")
+        spans = [_extent(o) for o in out if o.numel()]
+        for i, (lo, hi) in enumerate(spans):
+            others = [_extent(t) for t in (scores, *caches) if t.numel()] + spans[:i]
+            if any(lo < b and a < hi for a, b in others):
+                raise RuntimeError("out must not share memory with the caches, the scores or another out")
+
+
+def _rows_contiguous(t: torch.Tensor) -> bool:
+    want = 1
+    for i in range(t.dim() - 1, 2, -1):
+        if t.size(i) > 1 and t.stride(i) != want:
+            return False
+        want *= t.size(i)
+    return True
+
+
+def evict_kv(scores, caches, keep: int, recent: int, seqlens_k, out):
+    check_evict(scores, caches, keep, recent, seqlens_k, out)
+    _require_gpu(scores, *caches, *([] if seqlens_k is None else [seqlens_k]), *(out or ()))
+    lib = _cache_library()
+    b, h, n = scores.shape
+    keep, recent = min(keep, n), min(recent, n)
+    if n > 1 and scores.stride(-1) != 1:
+        scores = scores.contiguous()
+    caches = [t if _rows_contiguous(t) else t.contiguous() for t in caches]
+    seqlens_k = None if seqlens_k is None else seqlens_k.contiguous()
+    dev = scores.device
+    index = torch.empty((b, h, keep), dtype=torch.int32, device=dev)
+    kept = torch.empty((b, h, keep), dtype=torch.float32, device=dev)
+    lens = torch.empty((b,), dtype=torch.int32, device=dev)
+    dst = [torch.empty((b, h, keep, *t.shape[3:]), dtype=t.dtype, device=dev) for t in caches] if out is None else list(out)
+    if h == 0:
+        lens = torch.full((b,), n, dtype=torch.int32, device=dev) if seqlens_k is None else seqlens_k.clamp(0, n)
+        return dst, kept, index, lens.clamp(max=keep)
+    p = EvictParams(scores.data_ptr(), _stride(scores, 0), _stride(scores, 1),
+                    None if seqlens_k is None else seqlens_k.data_ptr(), b, h, n, keep, recent, len(caches),
+                    index.data_ptr(), kept.data_ptr(), lens.data_ptr())
+    for i, (s, d) in enumerate(zip(caches, dst)):
+        size = s.element_size()
+        p.tensors[i] = EvictTensor(s.data_ptr(), d.data_ptr(), *(x * size for x in _strides3(s)),
+                                   *(x * size for x in _strides3(d)), math.prod(s.shape[3:]) * size)
+    with _on_device(dev):
+        _check(lib.fa_evict_kv(p, _stream(scores)), "evict_kv")
+    return dst, kept, index, lens

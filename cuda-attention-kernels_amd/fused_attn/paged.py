@@ -19,8 +19,12 @@ FP8 pools (float8_e4m3fn) hold the bytes ``quantize_kv_fp8`` writes for a
 the semantics of ``attention_fp8_triton`` (fused_attn/fp8.py:125-147) on each sequence's
 gathered keys.
 
+4-bit pools (uint8) hold the codes ``quantize_kv_int4`` writes, [num_pages, Hkv, page_size, D/2], and take
+its (scale, zero) pairs, fp16 [num_pages, Hkv, page_size, 2], as ``k_scale`` / ``v_scale``; new tokens are
+written into them by ``append_kv_int4``.
+
 ``causal`` aligns each sequence's queries to the end of its own keys (bottom-right, as
-the dense op).  On the GPU this runs the split-K HIP kernel in its paged mode; page_size
+the dense op).  On the GPU this runs the split-K HIP kernel in its paged mode (4-bit pools: the 4-bit cache's kernel); page_size
 must be a multiple of 16 (64 for FP8 pools).  CPU tensors, or ``FUSED_ATTN_BACKEND=reference``, gather the
 pages and run the unfused reference per sequence.
 """
@@ -33,6 +37,7 @@ import torch
 
 from . import _hip
 from .fp8 import FP8_DTYPE, QBLOCK, dequantize_kv_fp8
+from .int4 import default_cache_split_len, dequantize_kv_int4
 from .ops import _pick_backend, default_split_len
 from .reference import attention_reference, lse_reference
 
@@ -97,11 +102,18 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
     """Decode attention over a paged K/V cache.  ``max_seqlen_k`` (the largest entry of
     ``seqlens_k``) sizes the grid; when omitted it is read from ``seqlens_k`` (a device sync).
-    FP8 pools take their per-page block scales ``k_scale`` / ``v_scale``.
+    FP8 pools take their per-page block scales ``k_scale`` / ``v_scale``, 4-bit pools (uint8) their rows' pairs.
     With ``return_lse`` also returns the natural-log LSE, fp32 [B, H_q, N_q]."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     fp8 = FP8_DTYPE is not None and k_cache.dtype == FP8_DTYPE
+    int4 = k_cache.dtype == torch.uint8
+    if int4:
+        _hip.check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, paged=True)
+        _hip.check_block_table(block_table, q.shape[0])
+        _hip.check_lengths(seqlens_k, q.shape[0])
     if not q.is_cuda or _pick_backend(q) != "hip":
+        if int4:
+            k_cache, v_cache = dequantize_kv_int4(k_cache, k_scale), dequantize_kv_int4(v_cache, v_scale)
         if fp8:
             if k_scale is None or v_scale is None:
                 raise RuntimeError("FP8 pools need k_scale and v_scale")
@@ -112,6 +124,14 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                          return_lse=return_lse)
     if max_seqlen_k is None:
         max_seqlen_k = int(seqlens_k.max().item()) if seqlens_k.numel() else 0
+    if int4:
+        if split_len is None:
+            split_len = default_cache_split_len(q.shape[2], max_seqlen_k, q.shape[0], k_cache.shape[1],
+                                                q.shape[1] // k_cache.shape[1])
+            split_len = min(split_len, max(64, (256 * k_cache.shape[2]) // 64 * 64))  # at most 257 pages
+        return _hip.cache_attention(q, k_cache, v_cache, k_scale, v_scale, causal, scale, int(split_len),
+                                    seqlens_k=seqlens_k, block_table=block_table, max_seqlen_k=max_seqlen_k,
+                                    return_lse=return_lse)
     if split_len is None:
         b, hq, nq, d = q.shape
         hkv, page_size = k_cache.shape[1], k_cache.shape[2]
@@ -187,3 +207,20 @@ def paged_from_dense_fp8(k8: torch.Tensor, k_scale: torch.Tensor, v8: torch.Tens
     block_table = perm.to(torch.int32).to(k8.device)
     seqlens_k = torch.tensor(seqlens, dtype=torch.int32, device=k8.device)
     return pages(k8), pages(v8), scale_pages(k_scale), scale_pages(v_scale), block_table, seqlens_k
+
+
+def paged_from_dense_int4(k4: torch.Tensor, k_scale: torch.Tensor, v4: torch.Tensor, v_scale: torch.Tensor,
+                          page_size: int, seqlens: Optional[list] = None, extra_pages: int = 0,
+                          generator: Optional[torch.Generator] = None):
+    """Scatter a dense 4-bit cache (``quantize_kv_int4`` output: uint8 [B, Hkv, N, D/2] and fp16 pairs [B, Hkv, N, 2])
+    into pools of ``page_size``-key pages in a random page order.
+
+    Returns (k_cache, v_cache, k_scale_pool, v_scale_pool, block_table, seqlens_k)."""
+    _hip.check_int4_rows(k4, k_scale, "k4")
+    _hip.check_int4_rows(v4, v_scale, "v4", k4.shape)
+    generator = torch.Generator().manual_seed(torch.seed() % (1 << 62)) if generator is None else generator
+    state = generator.get_state()  # the same page order for the codes and the pairs
+    k_cache, v_cache, block_table, seqlens_k = paged_from_dense(k4, v4, page_size, seqlens, extra_pages, generator)
+    generator.set_state(state)
+    ks_pool, vs_pool, _, _ = paged_from_dense(k_scale, v_scale, page_size, seqlens, extra_pages, generator)
+    return k_cache, v_cache, ks_pool, vs_pool, block_table, seqlens_k

@@ -29,7 +29,8 @@ extern "C" {
 #endif
 
 /* Raised by changes that an older caller or library does not survive; added functions keep it
-   (fa_attention_fwd_ws and its size query came within 6: look them up before use). */
+   (fa_attention_fwd_ws and its size query came within 6, and so did the functions of the 4-bit cache and of
+   eviction: look them up before use). */
 #define FA_ABI_VERSION 6
 
 /* Element types (reference: DType, csrc/flash_attn.h:7). */
@@ -37,7 +38,8 @@ typedef enum fa_dtype {
   FA_DTYPE_F16 = 0,
   FA_DTYPE_BF16 = 1,
   FA_DTYPE_F32 = 2,
-  FA_DTYPE_FP8_E4M3 = 3 /* OCP float8_e4m3fn, K/V cache only */
+  FA_DTYPE_FP8_E4M3 = 3, /* OCP float8_e4m3fn, K/V cache only */
+  FA_DTYPE_INT4 = 4      /* 4-bit codes, two a byte, with an fp16 (scale, zero) pair a row: fa_cache_params only */
 } fa_dtype;
 
 typedef enum fa_status {
@@ -210,6 +212,118 @@ typedef struct fa_quant_params {
 /* Per-(batch, head, 64-key block) absmax/448 scaling and e4m3fn rounding, bit-identical to the
    reference's torch chain quantize_kv_fp8 (fused_attn/fp8.py:31-45).  head_dim in {16, 32, 64, 128, 256}. */
 fa_status fa_quantize_kv_fp8(const fa_quant_params* p, void* stream);
+
+/*
+ * 4-bit K/V cache.  A row (one token of one kv-head, x[D]) is held as D codes of 4 bits and a (scale, zero) pair of
+ * fp16:
+ *   zero = fp16(lo), scale = fp16((hi - lo) * fp32(1/15))   lo, hi: the row's minimum and maximum, held to +-65504
+ *   code = clamp(rint((x - zero) / scale), 0, 15)           fp32, halves to even; 0 where scale is 0
+ *   value = code * scale + zero
+ * Two codes a byte, channel 2i in the low half of byte i, a row in D/2 contiguous bytes; the pair is one 4-byte word,
+ * scale first.  A NaN in a row makes its scale and zero NaN; infinities count as the row's ends.  The reference has no
+ * 4-bit cache.
+ */
+typedef struct fa_int4_params {
+  void* x; /* [batch, heads, seqlen, head_dim] F32/F16/BF16, unit head_dim stride, 16-byte aligned with 16-byte strides */
+  int64_t x_stride_b, x_stride_h, x_stride_n; /* elements */
+  int32_t batch, heads, seqlen, head_dim;     /* head_dim in {64, 128, 256} */
+  int32_t dtype;                              /* fa_dtype of x */
+  int32_t reserved;
+  void* codes; /* rows of head_dim / 2 bytes, 4-byte aligned with strides of whole 4-byte words */
+  int64_t codes_stride_b, codes_stride_h, codes_stride_n; /* bytes */
+  void* scale; /* (scale, zero) words, 4-byte aligned */
+  int64_t scale_stride_b, scale_stride_h, scale_stride_n; /* words */
+} fa_int4_params;
+
+/* x -> codes and pairs. */
+fa_status fa_quantize_kv_int4(const fa_int4_params* p, void* stream);
+/* codes and pairs -> x (rounded once to fp32, once to x's type). */
+fa_status fa_dequantize_kv_int4(const fa_int4_params* p, void* stream);
+
+/* New tokens into a cache in place, K and V in one launch: token i of sequence b is written at position
+   seqlens_k[b] + i.  k.x / v.x: [batch, heads, new tokens, head_dim], of the same sizes and type; k.codes, k.scale (v
+   likewise): the cache, whose stride_b is the one between sequences, or with a block table between pages.  A token
+   whose position is outside [0, capacity) (paged: [0, block_table_cols * page_size)), or whose page is outside
+   [0, num_pages), is not written. */
+typedef struct fa_int4_append_params {
+  fa_int4_params k, v;
+  const int32_t* seqlens_k; /* [batch], on the device: keys in the cache before the call */
+  int64_t capacity;         /* dense: keys a sequence has room for */
+  const int32_t* block_table; /* [batch, block_table_cols] or NULL for a dense cache */
+  int64_t block_table_stride;
+  int32_t block_table_cols, page_size, num_pages, reserved;
+} fa_int4_append_params;
+fa_status fa_append_kv_int4(const fa_int4_append_params* p, void* stream);
+
+/* Attention over a 4-bit cache (dense or paged), and attention that scores the keys of a dense 4-bit or 16-bit cache:
+   fa_attention_splitk's partitions, workspace rule and combine.  f16/bf16 q, head_dim in {64, 128, 256}, bottom-right
+   causal mask per sequence; rows without a visible key are zeros. */
+typedef struct fa_cache_params {
+  const void* q;
+  const void* k; /* [batch, heads_kv, seqlen_k, head_dim] in q's type, or codes; paged: pools of pages */
+  const void* v;
+  void* o;
+  int64_t q_stride_b, q_stride_h, q_stride_n;
+  int64_t k_stride_b, k_stride_h, k_stride_n; /* elements (codes: bytes), multiples of 16 bytes; paged: stride_b is */
+  int64_t v_stride_b, v_stride_h, v_stride_n; /* the page stride, stride_n the one inside a page */
+  int64_t o_stride_b, o_stride_h, o_stride_n;
+  int32_t batch, heads_q, heads_kv, seqlen_q, seqlen_k, head_dim;
+  float scale;
+  int32_t causal;
+  int32_t dtype;       /* of q and o */
+  int32_t kv_dtype;    /* FA_DTYPE_INT4, or dtype (then scores_out is needed) */
+  const void* k_scale; /* 4-bit: the pairs of K and V, 4-byte words */
+  const void* v_scale;
+  int64_t k_scale_stride_b, k_scale_stride_h, k_scale_stride_n;
+  int64_t v_scale_stride_b, v_scale_stride_h, v_scale_stride_n;
+  const int32_t* seqlens_k; /* [batch] keys per sequence, on the device, or NULL for seqlen_k each; values above
+                               seqlen_k are read as seqlen_k, negative ones as 0.  Rows past them are not read. */
+  const int32_t* block_table; /* paged (4-bit only, needs seqlens_k), or NULL; rules as fa_paged_kv */
+  int64_t block_table_stride;
+  int32_t block_table_cols, page_size, num_pages, reserved;
+  float* lse; /* optional natural-log LSE [batch, heads_q, seqlen_q] */
+  int64_t lse_stride_b, lse_stride_h;
+  /* optional scores, fp32 [batch, heads_kv, seqlen_k] with unit key stride:
+       scores_out[b, h, j] = scores_in[b, h, j] + the sum of key j's attention weights over the heads_q / heads_kv
+       q-heads and the seqlen_q queries
+     (scores_in may be NULL for zeros, or scores_out itself).  Dense caches only. */
+  const float* scores_in;
+  int64_t scores_in_stride_b, scores_in_stride_h;
+  float* scores_out;
+  int64_t scores_out_stride_b, scores_out_stride_h;
+} fa_cache_params;
+
+/* Bytes of workspace fa_attention_cache needs: fa_splitk_workspace_bytes, and with scores 4 bytes for every (q-head,
+   query, key).  0 for parameters that the call would refuse. */
+size_t fa_attention_cache_workspace_bytes(const fa_cache_params* p, int32_t split_len);
+/* split_len: keys a partition, a positive multiple of 64; workspace 16-byte aligned. */
+fa_status fa_attention_cache(const fa_cache_params* p, int32_t split_len, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Eviction.  Per (sequence, head) with n = seqlens_k[b] keys: all keys if n <= keep, else the last `recent` ones and the
+   keep - recent others of the highest scores (equal scores: the lower index; NaN above every number), in their order.
+   index gets their positions (-1 past them), scores_out their scores (0 past them), seqlens_out min(n, keep); row i of
+   dst gets row index[i] of src, for every tensor (zero bytes where it is -1). */
+#define FA_MAX_EVICT_TENSORS 8
+typedef struct fa_evict_tensor {
+  const void* src; /* [batch, heads, seqlen] rows of row_bytes contiguous bytes */
+  void* dst;       /* [batch, heads, keep] rows; must not overlap any src */
+  int64_t src_stride_b, src_stride_h, src_stride_n; /* bytes */
+  int64_t dst_stride_b, dst_stride_h, dst_stride_n;
+  int64_t row_bytes;
+} fa_evict_tensor;
+typedef struct fa_evict_params {
+  const float* scores; /* [batch, heads, seqlen], unit key stride */
+  int64_t scores_stride_b, scores_stride_h;
+  const int32_t* seqlens_k; /* [batch] on the device, or NULL for seqlen each; clamped to [0, seqlen] */
+  int32_t batch, heads, seqlen, keep, recent; /* 0 <= recent <= keep <= seqlen */
+  int32_t num_tensors;
+  int32_t* index;       /* [batch, heads, keep] */
+  float* scores_out;    /* [batch, heads, keep] */
+  int32_t* seqlens_out; /* [batch] */
+  fa_evict_tensor tensors[FA_MAX_EVICT_TENSORS];
+} fa_evict_params;
+fa_status fa_evict_kv(const fa_evict_params* p, void* stream);
 
 /* FA_ABI_VERSION of the loaded library. */
 int32_t fa_abi_version(void);
