@@ -7,7 +7,7 @@
 //
 // Decomposition.  Keys are cut into partitions of split_len; a workgroup of four waves takes one partition of one
 // (batch, kv-head) for up to 16 * RT rows, its waves every fourth 32-key tile each; the waves' (m, l, O) are merged
-// through LDS into one fp32 partial, and splitk_combine_kernel merges the partitions.  Bound by the bytes of the
+// through LDS into one fp32 partial, and cache_finish_kernel or splitk_combine_kernel merges the partitions.  Bound by the bytes of the
 // cache: D + 8 a key at 4 bits, 4 D at 16.
 //
 // No K or V goes through LDS: with v_mfma_f32_16x16x32 every operand is a lane's own load.
@@ -26,16 +26,26 @@
 // V's scale goes into P, rounded to bf16 (an fp16 product could leave fp16's range: vs is as small as V is), and the
 // sum of what was rounded takes the mean of the 1s and codes out again:
 //   o = sum_j P'_j (1 + vc_j/16) - (1 + 7.5/16) sum_j P'_j + sum_j p_j (vz_j + 7.5 vs_j),   P'_j = bf16(16 vs_j p_j)
-// so that P's rounding (2^-8 of itself) meets only (code - 7.5)/16, at most 0.47 of it.  Everything else is fp32.
+// so that P's rounding (2^-8 of itself) meets only (code - 7.5)/16, at most 0.47 of it.  For fp16 outputs, whose own
+// rounding is 2^-11, P' is the sum of two bf16 terms and takes two products.  Everything else is fp32.
 //
 // Scores.  p needs the row's final sum, which no partition has.  The s of a row and key are written as they are
-// (4 bytes: 6% of a 16-bit key's bytes at D=128 and four rows, 12% of a 4-bit one's), and score_finish_kernel turns them into
-// weights once the combine has written the rows' log-sum-exp.  A second pass over K would read half the cache again.
+// (4 bytes: 6% of a 16-bit key's bytes at D=128 and four rows, 12% of a 4-bit one's), and cache_finish_kernel turns them into
+// weights once the partitions' sums are there.  A second pass over K would read half the cache again.
 #include <algorithm>
 
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
 
+#ifndef AHEADV
+#define AHEADV 1
+#endif
+#ifndef NTV
+#define NTV (RT == 1 ? 2 : 0)
+#endif
+#ifndef WPE
+#define WPE __attribute__((amdgpu_waves_per_eu(RT == 4 ? 1 : RT == 2 ? (D == 256 ? 1 : 2) : D == 256 ? 1 : 3)))
+#endif
 namespace fa {
 
 namespace {
@@ -58,39 +68,44 @@ __device__ __forceinline__ float sum_xor16(float x) {
 __device__ __forceinline__ float max_groups(float x) { return max_xor32(max_xor16(x)); }
 __device__ __forceinline__ float sum_groups(float x) { return sum_xor32(sum_xor16(x)); }
 
-// Nibble n (0..3) of both halves of x as two 16-bit floats 1 + code/16.
-template <class E, int N>
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-  constexpr int at = std::is_same<E, BF16>::value ? 3 : 6;  // the top four bits of the mantissa
-  constexpr uint32_t mask = (0xfu << at) * 0x10001u, one = std::is_same<E, BF16>::value ? 0x3f803f80u : 0x3c003c00u;
-  constexpr int sh = 4 * N - at;
-  const uint32_t y = sh >= 0 ? x >> (sh & 31) : x << ((-sh) & 31);
-  return (y & mask) | one;
-}
+// Nibble n (0..3) of both halves of a word as two 16-bit floats 1 + code/16: a shift to the top of the mantissa and
+// one v_and_or.  That takes one scalar operand and no literal, so the mask is kept in a vector register.
+template <class E>
+struct Codes {
+  static constexpr int at = std::is_same<E, BF16>::value ? 3 : 6;
+  uint32_t mask, one;
+  __device__ __forceinline__ Codes() {
+    mask = (0xfu << at) * 0x10001u;
+    one = std::is_same<E, BF16>::value ? 0x3f803f80u : 0x3c003c00u;
+    __asm__("" : "+v"(mask));
+    __asm__("" : "+s"(one));
+  }
+  template <int N>
+  __device__ __forceinline__ uint32_t get(uint32_t x) const {
+    constexpr int sh = 4 * N - at;
+    const uint32_t y = sh >= 0 ? x >> (sh & 31) : x << ((-sh) & 31);
+    return (y & mask) | one;
+  }
+};
 
 // halves {a.lo, b.lo} and {a.hi, b.hi}
 __device__ __forceinline__ uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <int W>
-struct Words {
-  uint32_t w[W];
-};
-
-// W words (W = 0: one 16-bit half) of a buffer, or of memory
-template <int W>
+// W words (W = 0: one 16-bit half) of a buffer, or of memory; read once: non-temporal
+template <int W, int AUX>
 __device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, uint32_t* out) {
   if constexpr (W == 0) {
-    out[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    out[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, AUX);
   } else if constexpr (W == 1) {
-    out[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    out[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, AUX);
   } else if constexpr (W == 2) {
-    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, AUX));
     out[0] = v[0], out[1] = v[1];
   } else {
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) {
-      const u32x4 v = buffer_load16<false>(r, off + 16 * i);
+      const u32x4 v = buffer_load16<AUX != 0>(r, off + 16 * i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) out[4 * i + j] = v[j];
     }
@@ -116,7 +131,7 @@ __device__ __forceinline__ void memory_words(const uint8_t* p, uint32_t* out) {
 }
 
 template <int D, class E, bool I4, bool PAGED, bool SCORES, int RT>
-__global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const CacheArgs a) {
+__global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const CacheArgs a) {
   static_assert(!PAGED || I4, "16-bit pools have kernels of their own");
   constexpr int ROW_BYTES = I4 ? D / 2 : 2 * D;
   constexpr int KS = D / 32;                      // k-steps of S^T
@@ -124,8 +139,10 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
   constexpr int VN = D / 16;                      // channels of a key that a lane holds, for V
   constexpr int VW = I4 ? VN / 8 : VN / 2;        // and their words (I4, D=64: 0, a half)
   constexpr int VR = VW == 0 ? 1 : VW;            // registers
+  constexpr int AHEAD = AHEADV;                   // 4 bits: tiles in flight
   constexpr float NEG_INF = -__builtin_inff();
   using PV = typename std::conditional<I4, BF16, E>::type;  // element type of the second product
+  constexpr bool LOW = I4 && std::is_same<E, F16>::value;   // P as two bf16 terms: fp16 outputs keep their precision
 
   __shared__ int table[PAGED ? kMaxSlots : 1];
   // (scale, zero) of a wave's tile as the products use them: K's 32 keys, then V's
@@ -155,15 +172,31 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
     kvh = item % a.hkv;
     b = item / a.hkv;
   }
-  const int seq_q = a.nq;
+  const int seq_q = a.nq, klo = part * a.split_len;
+  const int tid = (int)threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // paged: the partition's block-table entries; -1 where the page lies outside the pool.  Bounded by the grid's largest
+  // length, so that they do not wait for this sequence's.
+  int first_slot = 0;
+  auto slot_of = [&](int n) __attribute__((always_inline)) {  // n / page_size
+    return (int)(((uint64_t)(uint32_t)n * a.page_magic) >> a.page_magic_shift);
+  };
+  if constexpr (PAGED) {
+    first_slot = slot_of(klo);
+    const int end = min(a.nk, klo + a.split_len);
+    const int slots = end > klo ? slot_of(end - 1) - first_slot + 1 : 0;  // <= kMaxSlots (host)
+    for (int i = tid; i < slots; i += kCacheWaves * 64) {
+      const int page = a.block_table[b * a.sbt + first_slot + i];
+      table[i] = (uint32_t)page < (uint32_t)a.num_pages ? page : -1;
+    }
+    __syncthreads();
+  }
   const int seq_k = a.seqlens_k != nullptr ? min(max(__builtin_amdgcn_readfirstlane(a.seqlens_k[b]), 0), a.nk) : a.nk;
-  const int klo = part * a.split_len;
   // partitions past the sequence's end are not written, and not read by the combine
   if (a.seqlens_k != nullptr && klo >= seq_k) return;
 
   const int R = a.group * seq_q, r0 = rb * 16 * RT;
-  const int tid = (int)threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // keys that any row, and that every row, of the block sees
   const int offset = seq_k - seq_q;  // bottom-right causal alignment
@@ -181,19 +214,112 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
   const uint8_t* kbase = (const uint8_t*)a.k + ((PAGED ? 0 : b * a.skb) + kvh * a.skh) * (I4 ? 1 : 2);
   const uint8_t* vbase = (const uint8_t*)a.v + ((PAGED ? 0 : b * a.svb) + kvh * a.svh) * (I4 ? 1 : 2);
 
-  // paged: the partition's block-table entries; -1 where the page lies outside the pool
-  int first_slot = 0;
-  auto slot_of = [&](int n) __attribute__((always_inline)) {  // n / page_size
-    return (int)(((uint64_t)(uint32_t)n * a.page_magic) >> a.page_magic_shift);
+  const float cs = a.qk_scale;  // of any sign, or 0: masked scores are set to -inf after it
+
+  // ---- loads ------------------------------------------------------------------------------------------------
+  // K block u, row c: key 8 (c / 4) + 4 u + c % 4 of the tile, words of channel group g.  V slot i: key 8 g + i.
+  struct Tile {
+    uint32_t k[2][KW], v[8][VR], pair;
   };
-  if constexpr (PAGED) {
-    first_slot = slot_of(klo);
-    const int slots = khi > klo ? slot_of(khi - 1) - first_slot + 1 : 0;  // <= 257 (host)
-    for (int i = tid; i < slots; i += kCacheWaves * 64) {
-      const int page = a.block_table[b * a.sbt + first_slot + i];
-      table[i] = (uint32_t)page < (uint32_t)a.num_pages ? page : -1;
+  const int kkey = 8 * (c >> 2) + (c & 3);
+  const int kpart = I4 ? g * KW * 4 : g * 16;  // bytes into the row (16 bit: + 64 a k-step)
+  const int vpart = c * (VN * (I4 ? 1 : 4)) / 2;
+  // rows that follow each other directly: the loads of a lane differ by constants, which the instructions hold
+  const bool packed = krow == ROW_BYTES && vrow == ROW_BYTES;
+  auto load_k_row = [&](auto&& get, uint32_t* w) __attribute__((always_inline)) {
+    if constexpr (I4) {
+      get(std::integral_constant<int, KW>{}, 0, w);
+    } else {
+#pragma unroll
+      for (int m = 0; m < KS; ++m) get(std::integral_constant<int, 4>{}, 64 * m, w + 4 * m);
     }
-    __syncthreads();
+  };
+  // Dense: a descriptor a tile; a load past its limit returns zeros (rows at or past khi).
+  auto load_k_dense = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    const int valid = min(khi - n0, kTile);
+    const auto r = make_rsrc(kbase + n0 * krow, (uint32_t)(valid - 1) * (uint32_t)krow + ROW_BYTES);
+    auto rows = [&](int row) __attribute__((always_inline)) {
+      const int at = kkey * row + kpart;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        load_k_row([&](auto w, int off, uint32_t* out) { buffer_words<decltype(w)::value, NTV>(r, at + 4 * u * row + off, out); },
+                   t.k[u]);
+    };
+    if (packed) rows(ROW_BYTES); else rows((int)krow);
+  };
+  auto load_v_dense = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    const int valid = min(khi - n0, kTile);
+    const auto r = make_rsrc(vbase + n0 * vrow, (uint32_t)(valid - 1) * (uint32_t)vrow + ROW_BYTES);
+    auto rows = [&](int row) __attribute__((always_inline)) {
+      const int at = 8 * g * row + vpart;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) buffer_words<VW, NTV>(r, at + i * row, t.v[i]);
+    };
+    if (packed) rows(ROW_BYTES); else rows((int)vrow);
+  };
+  // (scale, zero) words: lane l holds K's (l < 32) or V's of key l % 32 of the tile, zero past khi
+  const bool vlane = lane >= kTile;
+  const int64_t pstep = (vlane ? a.svsn : a.sksn) * 4;
+  const uint8_t* pbase = (const uint8_t*)(vlane ? a.v_scale : a.k_scale) + kvh * (vlane ? a.svsh : a.sksh) * 4;
+  if constexpr (I4 && !PAGED) pbase += b * (vlane ? a.svsb : a.sksb) * 4 + (int64_t)(lane & 31) * pstep;
+  auto load_pair_dense = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    if constexpr (I4) {
+      t.pair = 0;
+      if (n0 + (lane & 31) < khi) t.pair = *(const uint32_t*)(pbase + n0 * pstep);
+    }
+  };
+  // Paged: page sizes are multiples of 16, so each half of a tile lies in one page: a scalar base each, of which a lane
+  // takes the one of its keys.  Halves past khi and pages outside the pool read page 0, which exists; their pairs are
+  // zero (zero keys, or masked ones).
+  auto load_paged = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    const uint8_t *kp[2], *vp[2];
+    int64_t at[2];
+    int off[2];
+    bool ok[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = n0 + 16 * h, slot = slot_of(key);
+      const int page = key < khi ? __builtin_amdgcn_readfirstlane(table[slot - first_slot]) : -1;
+      ok[h] = page >= 0;
+      at[h] = max(page, 0);
+      off[h] = ok[h] ? key - slot * a.page_size : 0;
+      kp[h] = kbase + at[h] * a.skb + off[h] * krow;
+      vp[h] = vbase + at[h] * a.svb + off[h] * vrow;
+    }
+    const uint8_t* k = (c >= 8 ? kp[1] : kp[0]) + (kkey & 15) * (int)krow + kpart;
+    const uint8_t* v = (g >= 2 ? vp[1] : vp[0]) + 8 * (g & 1) * (int)vrow + vpart;
+    auto rows = [&](int kr, int vr) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) memory_words<KW>(k + 4 * u * kr, t.k[u]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) memory_words<VW>(v + i * vr, t.v[i]);
+    };
+    if (packed) rows(ROW_BYTES, ROW_BYTES); else rows((int)krow, (int)vrow);
+    const int h = (lane >> 4) & 1;
+    t.pair = 0;
+    if ((h ? ok[1] : ok[0]) && n0 + (lane & 31) < khi) {
+      const int64_t word = (h ? at[1] : at[0]) * (vlane ? a.svsb : a.sksb) * 4 + ((h ? off[1] : off[0]) + (lane & 15)) * pstep;
+      t.pair = *(const uint32_t*)(pbase + word);
+    }
+  };
+  auto load_tile = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+      load_paged(n0, t);
+    } else {
+      load_k_dense(n0, t);
+      load_pair_dense(n0, t);
+      load_v_dense(n0, t);
+    }
+  };
+
+  // the first tiles are on their way before anything waits for Q
+  constexpr int STEP = kCacheWaves * kTile;
+  const int last = klo + (n_tiles - 1) * kTile;  // the last tile's first key
+  int n0 = klo + wave * kTile;
+  Tile tiles[I4 ? AHEAD + 1 : 1];
+#pragma unroll
+  for (int i = 0; i < (I4 ? AHEAD : 1); ++i) {
+    if (n0 + i * STEP <= last) load_tile(n0 + i * STEP, tiles[i]);
   }
 
   // ---- Q: B operands, and the sum of each row -------------------------------------------------------------
@@ -224,84 +350,6 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
     qsum[t] = I4 ? sum_groups(s) : 0.f;
   }
 
-  const float cs = a.qk_scale;  // of any sign, or 0: masked scores are set to -inf after it
-
-  // ---- loads ------------------------------------------------------------------------------------------------
-  // K block t, row c: key 8 (c / 4) + 4 t + c % 4 of the tile, words of channel group g.  V slot s: key 8 g + s.
-  const int kkey = 8 * (c >> 2) + (c & 3);
-  const int kpart = I4 ? g * KW * 4 : g * 16;  // bytes into the row (16 bit: + 64 a k-step)
-  const int vpart = c * (VN * (I4 ? 1 : 4)) / 2;
-  struct KTile {
-    uint32_t w[2][KW];
-  };
-  struct VTile {
-    uint32_t w[8][VR];
-  };
-  auto load_k_row = [&](auto&& get, uint32_t* w) __attribute__((always_inline)) {
-    if constexpr (I4) {
-      get(std::integral_constant<int, KW>{}, 0, w);
-    } else {
-#pragma unroll
-      for (int m = 0; m < KS; ++m) get(std::integral_constant<int, 4>{}, 64 * m, w + 4 * m);
-    }
-  };
-  // paged: a lane's rows of a tile lie in one page each for K and V (runs of 8 keys; pages are multiples of 16).
-  // Keys past khi and pages outside the pool read page 0, which exists, and count as zero keys or are masked.
-  auto page_row = [&](const uint8_t* base, int64_t spage, int64_t srow, int key) __attribute__((always_inline)) {
-    const int slot = slot_of(key);
-    const int page = key < khi ? table[slot - first_slot] : -1;
-    const int64_t row = page >= 0 ? (int64_t)(key - slot * a.page_size) : 0;
-    return base + max(page, 0) * spage + row * srow;
-  };
-  auto load_k = [&](int n0, KTile& t) __attribute__((always_inline)) {
-    if constexpr (PAGED) {
-      const uint8_t* p = page_row(kbase, a.skb, krow, n0 + 8 * (c >> 2)) + (c & 3) * krow + kpart;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        load_k_row([&](auto w, int off, uint32_t* out) { memory_words<decltype(w)::value>(p + 4 * u * krow + off, out); },
-                   t.w[u]);
-    } else {
-      // a load past the limit returns zeros: rows at or past khi
-      const int valid = min(khi - n0, kTile);
-      const auto r = make_rsrc(kbase + n0 * krow, (uint32_t)(valid - 1) * (uint32_t)krow + ROW_BYTES);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        load_k_row([&](auto w, int off, uint32_t* out) {
-          buffer_words<decltype(w)::value>(r, (kkey + 4 * u) * (int)krow + kpart + off, out);
-        }, t.w[u]);
-    }
-  };
-  auto load_v = [&](int n0, VTile& t) __attribute__((always_inline)) {
-    if constexpr (PAGED) {
-      const uint8_t* p = page_row(vbase, a.svb, vrow, n0 + 8 * g) + vpart;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) memory_words<VW>(p + s * vrow, t.w[s]);
-    } else {
-      const int valid = min(khi - n0, kTile);
-      const auto r = make_rsrc(vbase + n0 * vrow, (uint32_t)(valid - 1) * (uint32_t)vrow + ROW_BYTES);
-#pragma unroll
-      for (int s = 0; s < 8; ++s) buffer_words<VW>(r, (8 * g + s) * (int)vrow + vpart, t.w[s]);
-    }
-  };
-  // lane l: the pair of K (l < 32) or V of key l % 32 of the tile; zero past khi and outside the pool
-  auto load_pair = [&](int n0) __attribute__((always_inline)) -> uint32_t {
-    if constexpr (!I4) return 0u;
-    const int key = n0 + (lane & 31);
-    const bool kv = lane >= 32;
-    const uint32_t* base = (const uint32_t*)(kv ? a.v_scale : a.k_scale) + kvh * (kv ? a.svsh : a.sksh);
-    int64_t at = b, slot = key;
-    bool ok = key < khi;
-    if constexpr (PAGED) {
-      const int sl = slot_of(key);
-      at = ok ? table[sl - first_slot] : -1;
-      ok = at >= 0;
-      slot = key - sl * a.page_size;
-    }
-    uint32_t v = 0;
-    if (ok) v = base[at * (kv ? a.svsb : a.sksb) + slot * (kv ? a.svsn : a.sksn)];
-    return v;
-  };
-
   f32x4 oacc[RT][VN];
   float m_run[RT], l_run[RT], psum[RT], zsum[RT];
 #pragma unroll
@@ -312,9 +360,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
     l_run[t] = psum[t] = zsum[t] = 0.f;
   }
 
-  // ---- one tile: s (log2 domain), then p and O ---------------------------------------------------------------
-  auto scores_of = [&](const KTile& kt, int n0, float(&s)[RT][8]) __attribute__((always_inline)) {
-    f32x4 acc[RT][2];
+  // ---- one tile -----------------------------------------------------------------------------------------------
+  const Codes<E> kcodes;
+  const Codes<BF16> vcodes;
+  // S^T = K Q^T (4 bits: from -sum(q), so that it is q . code / 16)
+  auto product_k = [&](const Tile& kt, f32x4(&acc)[RT][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[t][0] = acc[t][1] = f32x4{-qsum[t], -qsum[t], -qsum[t], -qsum[t]};
 #pragma unroll
@@ -323,115 +373,134 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
       for (int u = 0; u < 2; ++u) {
         u32x4 ka;
         if constexpr (I4) {
-          const uint32_t w = kt.w[u][m];
-          ka = u32x4{codes2<E, 0>(w), codes2<E, 1>(w), codes2<E, 2>(w), codes2<E, 3>(w)};
+          const uint32_t w = kt.k[u][m];
+          ka = u32x4{kcodes.template get<0>(w), kcodes.template get<1>(w), kcodes.template get<2>(w),
+                     kcodes.template get<3>(w)};
         } else {
-          ka = u32x4{kt.w[u][4 * m], kt.w[u][4 * m + 1], kt.w[u][4 * m + 2], kt.w[u][4 * m + 3]};
+          ka = u32x4{kt.k[u][4 * m], kt.k[u][4 * m + 1], kt.k[u][4 * m + 2], kt.k[u][4 * m + 3]};
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t) acc[t][u] = mfma16<E>(ka, qf[t][m], acc[t][u]);
       }
     }
-    if constexpr (I4) {
-      const f32x4* kp = (const f32x4*)&pairs[wave][8 * g * 2];  // keys 8g..8g+7: (scale, zero) each
+  };
+  // p = 2^(s - m), and O += P V
+  auto product_v = [&](const Tile& vt, f32x4(&acc)[RT][2], int n0) __attribute__((always_inline)) {
+    u32x4 pf[RT], pl[RT];
+    f32x4 kp[4], vp[4];
+    if constexpr (I4) {  // keys 8g .. 8g+7: (multiplier of the product, multiplier of sum(q)), and V's two
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 p = kp[i];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          s[t][2 * i] = __builtin_fmaf(acc[t][i >> 1][(2 * i) & 3], p[0], p[1] * qsum[t]);
-          s[t][2 * i + 1] = __builtin_fmaf(acc[t][i >> 1][(2 * i + 1) & 3], p[2], p[3] * qsum[t]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[t][i] = acc[t][i >> 2][i & 3] * cs;
+        kp[i] = ((const f32x4*)&pairs[wave][8 * g * 2])[i];
+        vp[i] = ((const f32x4*)&pairs[wave][2 * kTile + 8 * g * 2])[i];
       }
     }
-    if constexpr (SCORES) {
+    const bool masked = n0 + kTile > mask_from;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < RT; ++t) {
+      const int end = a.causal ? min(khi, qlim[t] + 1) : khi;
+      // the scores less `m` (log2 domain)
+      auto scores_less = [&](float m, float(&s)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = acc[t][i >> 2][i & 3];
+          if constexpr (I4) {
+            s[i] = __builtin_fmaf(x, kp[i >> 1][2 * (i & 1)], __builtin_fmaf(kp[i >> 1][2 * (i & 1) + 1], qsum[t], -m));
+          } else {
+            s[i] = __builtin_fmaf(x, cs, -m);
+          }
+        }
+      };
+      auto mask = [&](float(&s)[8]) __attribute__((always_inline)) {
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[i] = n0 + 8 * g + i < end ? s[i] : NEG_INF;
+        }
+      };
+      float s[8];
+      if constexpr (SCORES) {
+        scores_less(0.f, s);
         const int row = r0 + 16 * t + c;
         if (row < R) {
           float* out = a.raw + ((int64_t)(b * a.hkv + kvh) * R + row) * a.raw_stride + n0 + 8 * g;
-          st16(out, __builtin_bit_cast(u32x4, f32x4{s[t][0], s[t][1], s[t][2], s[t][3]}));
-          st16(out + 4, __builtin_bit_cast(u32x4, f32x4{s[t][4], s[t][5], s[t][6], s[t][7]}));
+          st16(out, __builtin_bit_cast(u32x4, f32x4{s[0], s[1], s[2], s[3]}));
+          st16(out + 4, __builtin_bit_cast(u32x4, f32x4{s[4], s[5], s[6], s[7]}));
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] -= m_run[t];
+      } else {
+        scores_less(m_run[t], s);
       }
-    }
-    if (n0 + kTile > mask_from) {
+      mask(s);
+      // The maximum follows only when a row outgrows it by 2^8 (p <= 256 until then: O and l share it): most tiles need
+      // no exchange between the lanes of a row.  The first tile's m is -inf, and s then +inf.
+      float mt = s[0];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int end = a.causal ? min(khi, qlim[t] + 1) : khi;
+      for (int i = 1; i < 8; ++i) mt = vmax(mt, s[i]);
+      if (__builtin_amdgcn_ballot_w64(mt > kRescaleLog2) != 0) {
+        scores_less(0.f, s);
+        mask(s);
+        mt = s[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[t][i] = n0 + 8 * g + i < end ? s[t][i] : NEG_INF;
-      }
-    }
-  };
-  auto add_values = [&](const VTile& vt, float(&s)[RT][8]) __attribute__((always_inline)) {
-    u32x4 pf[RT];
-    f32x4 vp[4];
-    if constexpr (I4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) vp[i] = ((const f32x4*)&pairs[wave][2 * kTile + 8 * g * 2])[i];
-    }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      float mt = s[t][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) mt = vmax(mt, s[t][i]);
-      const float m_new = vmax(m_run[t], max_groups(mt));
-      // the maximum follows only when a row outgrows it by 2^8 (p <= 256 until then: O and l share it)
-      if (__builtin_amdgcn_ballot_w64(m_new > m_run[t] + kRescaleLog2) != 0) {
-        const float alpha = fast_exp2(m_run[t] - (m_new == NEG_INF ? 0.f : m_new));
+        for (int i = 1; i < 8; ++i) mt = vmax(mt, s[i]);
+        const float m_new = vmax(m_run[t], max_groups(mt)), m = m_new == NEG_INF ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run[t] - m);
         l_run[t] *= alpha, psum[t] *= alpha, zsum[t] *= alpha;
 #pragma unroll
         for (int n = 0; n < VN; ++n) oacc[t][n] *= alpha;
         m_run[t] = m_new;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] -= m;
       }
-      const float m = m_run[t] == NEG_INF ? 0.f : m_run[t];
       float p[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p[i] = fast_exp2(s[t][i] - m);
+        p[i] = fast_exp2(s[i]);
         l_run[t] += p[i];
       }
-      if constexpr (I4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (I4) {
           zsum[t] = __builtin_fmaf(p[2 * i], vp[i][1], zsum[t]);
           zsum[t] = __builtin_fmaf(p[2 * i + 1], vp[i][3], zsum[t]);
-          pf[t][i] = pack2<PV>(p[2 * i] * vp[i][0], p[2 * i + 1] * vp[i][2]);
-          psum[t] = sum2<PV>(pf[t][i], psum[t]);
+          const float x = p[2 * i] * vp[i][0], y = p[2 * i + 1] * vp[i][2];
+          pf[t][i] = pack2<BF16>(x, y);
+          psum[t] = sum2<BF16>(pf[t][i], psum[t]);
+          if constexpr (LOW) {
+            pl[t][i] = pack2<BF16>(x - lo_f32<BF16>(pf[t][i]), y - hi_f32<BF16>(pf[t][i]));
+            psum[t] = sum2<BF16>(pl[t][i], psum[t]);
+          }
+        } else {
+          pf[t][i] = pack2<E>(p[2 * i], p[2 * i + 1]);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pf[t][i] = pack2<PV>(p[2 * i], p[2 * i + 1]);
       }
     }
     // A operands of channel n: its value for keys 8g .. 8g+7, two a register
+    auto channel = [&](int n, const u32x4& v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        oacc[t][n] = mfma16<PV>(v, pf[t], oacc[t][n]);
+        if constexpr (LOW) oacc[t][n] = mfma16<PV>(v, pl[t], oacc[t][n]);
+      }
+    };
     if constexpr (I4) {
 #pragma unroll
-      for (int h = 0; h < (VN + 3) / 4; ++h) {  // halves of 4 channels
+      for (int h = 0; h < VN / 4; ++h) {  // halves of 4 channels
         uint32_t x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t ka = vt.w[2 * j][h / 2], kb = vt.w[2 * j + 1][h / 2];
+          const uint32_t ka = vt.v[2 * j][h / 2], kb = vt.v[2 * j + 1][h / 2];
           x[j] = h & 1 ? pair_hi(ka, kb) : pair_lo(ka, kb);
         }
-        const u32x4 v0 = {codes2<BF16, 0>(x[0]), codes2<BF16, 0>(x[1]), codes2<BF16, 0>(x[2]), codes2<BF16, 0>(x[3])};
-        const u32x4 v1 = {codes2<BF16, 1>(x[0]), codes2<BF16, 1>(x[1]), codes2<BF16, 1>(x[2]), codes2<BF16, 1>(x[3])};
-        const u32x4 v2 = {codes2<BF16, 2>(x[0]), codes2<BF16, 2>(x[1]), codes2<BF16, 2>(x[2]), codes2<BF16, 2>(x[3])};
-        const u32x4 v3 = {codes2<BF16, 3>(x[0]), codes2<BF16, 3>(x[1]), codes2<BF16, 3>(x[2]), codes2<BF16, 3>(x[3])};
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          oacc[t][4 * h] = mfma16<PV>(v0, pf[t], oacc[t][4 * h]);
-          oacc[t][4 * h + 1] = mfma16<PV>(v1, pf[t], oacc[t][4 * h + 1]);
-          oacc[t][4 * h + 2] = mfma16<PV>(v2, pf[t], oacc[t][4 * h + 2]);
-          oacc[t][4 * h + 3] = mfma16<PV>(v3, pf[t], oacc[t][4 * h + 3]);
-        }
+        auto nibble = [&](auto n) __attribute__((always_inline)) {
+          constexpr int N = decltype(n)::value;
+          channel(4 * h + N, u32x4{vcodes.template get<N>(x[0]), vcodes.template get<N>(x[1]), vcodes.template get<N>(x[2]),
+                                   vcodes.template get<N>(x[3])});
+        };
+        nibble(std::integral_constant<int, 0>{});
+        nibble(std::integral_constant<int, 1>{});
+        nibble(std::integral_constant<int, 2>{});
+        nibble(std::integral_constant<int, 3>{});
       }
     } else {
 #pragma unroll
@@ -439,14 +508,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
         u32x4 lo, hi;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          lo[j] = pair_lo(vt.w[2 * j][h], vt.w[2 * j + 1][h]);
-          hi[j] = pair_hi(vt.w[2 * j][h], vt.w[2 * j + 1][h]);
+          lo[j] = pair_lo(vt.v[2 * j][h], vt.v[2 * j + 1][h]);
+          hi[j] = pair_hi(vt.v[2 * j][h], vt.v[2 * j + 1][h]);
         }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          oacc[t][2 * h] = mfma16<PV>(lo, pf[t], oacc[t][2 * h]);
-          oacc[t][2 * h + 1] = mfma16<PV>(hi, pf[t], oacc[t][2 * h + 1]);
-        }
+        channel(2 * h, lo);
+        channel(2 * h + 1, hi);
       }
     }
   };
@@ -454,48 +520,39 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
   auto store_pair = [&](uint32_t w) __attribute__((always_inline)) {
     if constexpr (I4) {
       const float sc = lo_f32<F16>(w), z = hi_f32<F16>(w);
-      const bool kv = lane >= 32;
-      const f32x2 v = {16.f * sc * (kv ? 1.f : cs), kv ? __builtin_fmaf(7.5f, sc, z) : z * cs};
+      const f32x2 v = {16.f * sc * (vlane ? 1.f : cs), vlane ? __builtin_fmaf(7.5f, sc, z) : z * cs};
       *(f32x2*)&pairs[wave][2 * lane] = v;
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
   };
 
-  if (wave < n_tiles) {
-    KTile kt;
-    VTile vt;
-    float s[RT][8];
-    int n0 = klo + wave * kTile;
-    load_k(n0, kt);
-    uint32_t pr = load_pair(n0);
-    load_v(n0, vt);
-    for (int t = wave; t < n_tiles; t += kCacheWaves, n0 += kCacheWaves * kTile) {
-      const bool more = t + kCacheWaves < n_tiles;
-      const int next = n0 + kCacheWaves * kTile;
-      if constexpr (I4) {
-        // the next tile's words are few: all of them are in flight while this tile is worked on
-        KTile kn;
-        VTile vn;
-        uint32_t pn = 0;
-        store_pair(pr);
-        if (more) {
-          load_k(next, kn);
-          pn = load_pair(next);
-          load_v(next, vn);
-        }
-        scores_of(kt, n0, s);
-        add_values(vt, s);
-        kt = kn;
-        vt = vn;
-        pr = pn;
-      } else {
-        // K's registers are refilled once its product has read them, V's likewise
-        scores_of(kt, n0, s);
-        if (more) load_k(next, kt);
-        add_values(vt, s);
-        if (more) load_v(next, vt);
+  if constexpr (I4) {
+    // AHEAD tiles are in flight while one is worked on (a ring of registers: the loop is unrolled by its size)
+    auto step = [&](Tile& cur, Tile& next) __attribute__((always_inline)) {
+      store_pair(cur.pair);
+      if (n0 + AHEAD * STEP <= last) load_tile(n0 + AHEAD * STEP, next);
+      f32x4 acc[RT][2];
+      product_k(cur, acc);
+      product_v(cur, acc, n0);
+      n0 += STEP;
+    };
+    while (n0 <= last) {
+#pragma unroll
+      for (int i = 0; i <= AHEAD; ++i) {
+        if (i > 0 && n0 > last) break;
+        step(tiles[i], tiles[(i + AHEAD) % (AHEAD + 1)]);
       }
+    }
+  } else {
+    // K's registers are refilled once its product has read them, V's likewise
+    Tile& t = tiles[0];
+    for (; n0 <= last; n0 += STEP) {
+      f32x4 acc[RT][2];
+      product_k(t, acc);
+      if (n0 + STEP <= last) load_k_dense(n0 + STEP, t);
+      product_v(t, acc, n0);
+      if (n0 + STEP <= last) load_v_dense(n0 + STEP, t);
     }
   }
 
@@ -572,33 +629,156 @@ __global__ void __launch_bounds__(kCacheWaves * 64) attn_cache_kernel(const Cach
   }
 }
 
-// score_j = before_j + sum over the rows of 2^(s_rj - lse2_r), for the keys that a row sees.
-// Four keys a thread; the rows' log-sum-exps are read through the scalar cache.
-__global__ void __launch_bounds__(256) score_finish_kernel(const FinishArgs a) {
-  const int bh = (int)(blockIdx.x / (uint32_t)a.chunks), b = bh / a.hkv, kvh = bh - b * a.hkv;
-  const int seq_k = a.seqlens_k != nullptr ? min(max(a.seqlens_k[b], 0), a.nk) : a.nk;
-  const int j = ((int)(blockIdx.x - (uint32_t)bh * (uint32_t)a.chunks) * 256 + (int)threadIdx.x) * 4;
-  if (j >= a.nk) return;
-  f32x4 w = {};
-  if (j < seq_k) {
-    const int R = a.group * a.nq, offset = seq_k - a.nq;
-    const float* raw = a.raw + (int64_t)bh * R * a.raw_stride + j;
-    for (int r = 0; r < R; ++r) {
-      const int gi = r / a.nq, qi = r - gi * a.nq;
-      const float lse = a.lse[b * a.slb + (kvh * a.group + gi) * a.slh + qi] * kLog2e;
-      const int end = a.causal ? min(seq_k, qi + offset + 1) : seq_k;
-      if (j >= end || lse == -__builtin_inff()) continue;  // (-inf: every key of the row scores -inf)
-      const f32x4 s = __builtin_bit_cast(f32x4, ld16(raw + r * a.raw_stride));
+// What follows the partitions' partials: blocks below a.merge_blocks merge a row's partials into its output, the others
+// turn scores into weights.  Both start from the partitions' (max, sum), so neither waits for the other: one launch.
+// For up to kMergeSplits partitions (more: splitk_combine_kernel, which spreads a row's partials over a workgroup, and
+// then this kernel with the log-sum-exps that it wrote).
+constexpr int kMergeSplits = 16;
+constexpr int kFinishRows = 512;  // rows whose log-sum-exps a block holds at a time
+
+// D/4 lanes a row, rows of a block one after another; log-sum-exp merge as splitk_combine_kernel:
+//   m = max_s m_s,  w_s = 2^(m_s - m) l_s,  O = sum_s w_s O_s / sum_s w_s
+template <int D, class E>
+__device__ __forceinline__ void merge_rows(const FinishArgs& a) {
+  constexpr int LPR = D / 4, CH = 4;
+  constexpr float NEG_INF = -__builtin_inff();
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + (int)threadIdx.x / LPR;
+  if (row >= a.rows) return;
+  const int d = (int)threadIdx.x % LPR * 4;
+  const uint32_t bh = (uint32_t)row / (uint32_t)a.nq, qi = (uint32_t)row - bh * (uint32_t)a.nq;
+  const uint32_t b = bh / (uint32_t)a.hq, hq = bh - b * (uint32_t)a.hq;
+  int S = a.n_split;  // partitions that start below the sequence's end: the others were not written
+  if (a.seqlens_k != nullptr) S = min(S, (min(max(a.seqlens_k[b], 0), a.nk) + a.split_len - 1) / a.split_len);
+  const float* ml = a.ml + row * a.n_split * 2;
+  const float* part = a.part + row * a.n_split * D + d;
+  float m = NEG_INF, l = 0.f;
+  f32x4 acc = {};
+  for (int s0 = 0; s0 < S; s0 += CH) {
+    f32x2 st[CH];
+    f32x4 o[CH];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] += j + i < end ? fast_exp2(s[i] - lse) : 0.f;
+    for (int u = 0; u < CH; ++u) {  // past the last: the last again, which weighs 0
+      const int s = min(s0 + u, S - 1);
+      st[u] = __builtin_bit_cast(f32x2, ld8(ml + 2 * s));
+      o[u] = __builtin_bit_cast(f32x4, ld16(part + s * D));
+      if (s0 + u >= S) st[u] = f32x2{NEG_INF, 0.f};
+    }
+    float m_new = m;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) m_new = fmaxf(m_new, st[u][0]);
+    const float ref = m_new == NEG_INF ? 0.f : m_new, alpha = fast_exp2(m - ref);
+    l *= alpha;
+    acc *= alpha;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const float w = fast_exp2(st[u][0] - ref) * st[u][1];
+      l += w;
+      acc += s0 + u < S ? w * o[u] : f32x4{};
+    }
+    m = m_new;
+  }
+  const float l_safe = l == 0.f ? 1.f : l, inv = 1.f / l_safe;
+  if (a.lse != nullptr && d == 0) a.lse[b * a.slb + hq * a.slh + qi] = (m + __log2f(l_safe)) * kLn2;
+  st8((uint16_t*)a.o + b * a.sob + hq * a.soh + qi * a.son + d,
+      u32x2{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv)});
+}
+
+// score_j = before_j + sum over the rows of 2^(s_rj - lse2_r), for the keys that a row sees.  Four keys a lane; NW waves
+// share 256 keys and take every NW-th row each (their sums are added in order), and a block has 4 / NW such sets.
+template <int NW>
+__device__ __forceinline__ void finish_scores(const FinishArgs& a) {
+  constexpr int THREADS = NW <= 4 ? 256 : NW * 64, SETS = THREADS / 64 / NW;
+  constexpr float NEG_INF = -__builtin_inff();
+  __shared__ float lse2[kFinishRows];
+  __shared__ __align__(16) float sums[NW > 1 ? NW : 1][NW > 1 ? 256 : 4];
+  const uint32_t blk = blockIdx.x - (uint32_t)a.merge_blocks;
+  const int bh = (int)(blk / (uint32_t)a.chunks), b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int seq_k = a.seqlens_k != nullptr ? min(max(__builtin_amdgcn_readfirstlane(a.seqlens_k[b]), 0), a.nk) : a.nk;
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int block0 = (int)(blk - (uint32_t)bh * (uint32_t)a.chunks) * (256 * SETS);
+  const int j0 = block0 + wave / NW * 256, j = j0 + 4 * lane;
+  const int R = a.group * a.nq, offset = seq_k - a.nq, w0 = wave % NW;
+  const int S = a.seqlens_k != nullptr ? min(a.n_split, (seq_k + a.split_len - 1) / a.split_len) : a.n_split;
+  const int64_t prow = ((int64_t)b * a.hq + kvh * a.group) * a.nq;  // (row r of the group: prow + r)
+  const float* raw = a.raw + (int64_t)bh * R * a.raw_stride + j;
+  f32x4 w = {};
+  for (int r0 = 0; r0 < R && block0 < seq_k; r0 += kFinishRows) {
+    const int rows = min(kFinishRows, R - r0);
+    if (r0 > 0) __syncthreads();
+    for (int r = (int)threadIdx.x; r < rows; r += THREADS) {
+      float x;
+      if (a.use_lse) {
+        const int gi = (r0 + r) / a.nq;
+        x = a.lse[b * a.slb + (kvh * a.group + gi) * a.slh + (r0 + r - gi * a.nq)] * kLog2e;
+      } else {
+        const float* ml = a.ml + (prow + r0 + r) * a.n_split * 2;
+        float m = NEG_INF, l = 0.f;
+        for (int s = 0; s < S; ++s) m = fmaxf(m, ml[2 * s]);
+        const float ref = m == NEG_INF ? 0.f : m;
+        for (int s = 0; s < S; ++s) l += fast_exp2(ml[2 * s] - ref) * ml[2 * s + 1];
+        x = m + __log2f(l == 0.f ? 1.f : l);
+      }
+      lse2[r] = x;
+    }
+    __syncthreads();
+    if (j0 < seq_k) {
+#pragma unroll 8
+      for (int r = w0; r < rows; r += NW) {
+        const float l2 = lse2[r];
+        int end = a.causal ? min(seq_k, (r0 + r) % a.nq + offset + 1) : seq_k;
+        end = l2 == NEG_INF ? 0 : end;  // (every key of the row scores -inf)
+        f32x4 s = {};
+        if (j < end) s = __builtin_bit_cast(f32x4, ld16(raw + (r0 + r) * a.raw_stride));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += j + i < end ? fast_exp2(s[i] - l2) : 0.f;
+      }
     }
   }
   const float* in = a.in != nullptr ? a.in + b * a.sib + kvh * a.sih : nullptr;
-  float* out = a.out + b * a.sob + kvh * a.soh;
+  float* out = a.out + b * a.sob_s + kvh * a.soh_s;
+  if constexpr (NW > 1) {
+    *(f32x4*)&sums[wave][4 * lane] = w;
+    __syncthreads();
+    const int t = (int)threadIdx.x, key = block0 + t;
+    if (t >= 256 || key >= a.nk) return;
+    float x = sums[0][t];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (j + i < a.nk) out[j + i] = w[i] + (in != nullptr ? in[j + i] : 0.f);
+    for (int i = 1; i < NW; ++i) x += sums[i][t];
+    out[key] = in != nullptr ? x + in[key] : x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (j + i < a.nk) out[j + i] = in != nullptr ? w[i] + in[j + i] : w[i];
+    }
   }
+}
+
+template <int D, class E, int NW>
+__global__ void __launch_bounds__(NW <= 4 ? 256 : NW * 64) cache_finish_kernel(const FinishArgs a) {
+  if ((int)blockIdx.x < a.merge_blocks) {
+    if (threadIdx.x < 256) merge_rows<D, E>(a);
+  } else {
+    finish_scores<NW>(a);
+  }
+}
+
+template <int D, class E>
+hipError_t launch_finish(FinishArgs a, bool merge, bool scores, hipStream_t stream, const char** err) {
+  const int R = a.group * a.nq, nw = R >= 64 ? 16 : 1, keys = nw == 16 ? 256 : 1024;
+  a.chunks = (a.nk + keys - 1) / keys;
+  const int64_t mb = merge ? (a.rows + 1024 / D - 1) / (1024 / D) : 0, fb = scores ? (int64_t)a.batch * a.hkv * a.chunks : 0;
+  if (mb + fb > INT32_MAX) {
+    *err = "grid too large";
+    return hipErrorInvalidConfiguration;
+  }
+  a.merge_blocks = (int32_t)mb;
+  if (mb + fb == 0) return hipSuccess;
+  if (nw == 16 && scores) {
+    hipLaunchKernelGGL((cache_finish_kernel<D, E, 16>), dim3((unsigned)(mb + fb)), dim3(1024), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((cache_finish_kernel<D, E, 1>), dim3((unsigned)(mb + fb)), dim3(256), 0, stream, a);
+  }
+  return hipGetLastError();
 }
 
 template <int D, class E, bool I4, bool PAGED, bool SCORES>
@@ -606,8 +786,11 @@ hipError_t launch_rows(const CacheArgs& a, int rt, hipStream_t stream) {
   if (rt == 1) {
     hipLaunchKernelGGL((attn_cache_kernel<D, E, I4, PAGED, SCORES, 1>), dim3((unsigned)a.total), dim3(kCacheWaves * 64),
                        0, stream, a);
-  } else {
+  } else if (rt == 2) {
     hipLaunchKernelGGL((attn_cache_kernel<D, E, I4, PAGED, SCORES, 2>), dim3((unsigned)a.total), dim3(kCacheWaves * 64),
+                       0, stream, a);
+  } else if constexpr (D != 256) {
+    hipLaunchKernelGGL((attn_cache_kernel<D, E, I4, PAGED, SCORES, 4>), dim3((unsigned)a.total), dim3(kCacheWaves * 64),
                        0, stream, a);
   }
   return hipGetLastError();
@@ -667,7 +850,7 @@ fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace
       return FA_ERR_UNSUPPORTED;
     }
   }
-  const int rows = a.group * p.seqlen_q, rt = rows <= 16 ? 1 : 2;
+  const int rows = a.group * p.seqlen_q, rt = rows <= 16 ? 1 : rows <= 32 || p.head_dim == 256 ? 2 : 4;
   a.n_rowblk = (rows + 16 * rt - 1) / (16 * rt);
   const int64_t items = (int64_t)p.batch * p.heads_kv * S, out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
   const int64_t total = (p.seqlens_k != nullptr ? (items + 7) / 8 * 8 : items) * a.n_rowblk;
@@ -699,31 +882,37 @@ fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace
   }
   if (e != hipSuccess) return hip_status(e, err);
 
-  CombineArgs c{};
-  c.opart = a.part, c.ml = a.ml, c.o = p.o;
-  c.sob = p.o_stride_b, c.soh = p.o_stride_h, c.son = p.o_stride_n;
-  c.lse = lse, c.slb = slb, c.slh = slh;
-  c.hq = p.heads_q, c.group = a.group, c.nq = p.seqlen_q, c.n_split = S;
-  c.seqlens_k = p.seqlens_k, c.nk = p.seqlen_k, c.split_len = split_len;
-  const fa_status st = run_combine(c, p.head_dim, bf, out_rows, stream, err);
-  if (st != FA_OK || !scores) return st;
-
-  FinishArgs f{};
-  f.raw = a.raw, f.raw_stride = a.raw_stride;
-  f.lse = lse, f.slb = slb, f.slh = slh;
-  f.in = p.scores_in, f.sib = p.scores_in_stride_b, f.sih = p.scores_in_stride_h;
-  f.out = p.scores_out, f.sob = p.scores_out_stride_b, f.soh = p.scores_out_stride_h;
-  f.seqlens_k = p.seqlens_k;
-  f.hkv = p.heads_kv, f.group = a.group, f.nq = p.seqlen_q, f.nk = p.seqlen_k, f.causal = a.causal;
-  if (p.seqlen_k == 0) return FA_OK;
-  f.chunks = (p.seqlen_k - 1) / 1024 + 1;
-  const int64_t blocks = (int64_t)p.batch * p.heads_kv * f.chunks;
-  if (blocks > INT32_MAX) {
-    *err = "grid too large";
-    return FA_ERR_UNSUPPORTED;
+  const bool merge = S <= kMergeSplits;
+  if (!merge) {
+    CombineArgs c{};
+    c.opart = a.part, c.ml = a.ml, c.o = p.o;
+    c.sob = p.o_stride_b, c.soh = p.o_stride_h, c.son = p.o_stride_n;
+    c.lse = lse, c.slb = slb, c.slh = slh;
+    c.hq = p.heads_q, c.group = a.group, c.nq = p.seqlen_q, c.n_split = S;
+    c.seqlens_k = p.seqlens_k, c.nk = p.seqlen_k, c.split_len = split_len;
+    const fa_status st = run_combine(c, p.head_dim, bf, out_rows, stream, err);
+    if (st != FA_OK) return st;
   }
-  hipLaunchKernelGGL(score_finish_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, f);
-  return hip_status(hipGetLastError(), err);
+  FinishArgs f{};
+  f.part = a.part, f.ml = a.ml, f.o = p.o;
+  f.sob = p.o_stride_b, f.soh = p.o_stride_h, f.son = p.o_stride_n;
+  f.raw = a.raw, f.raw_stride = a.raw_stride;
+  f.lse = merge ? p.lse : lse, f.slb = slb, f.slh = slh;
+  f.use_lse = merge ? 0 : 1;
+  f.in = p.scores_in, f.sib = p.scores_in_stride_b, f.sih = p.scores_in_stride_h;
+  f.out = p.scores_out, f.sob_s = p.scores_out_stride_b, f.soh_s = p.scores_out_stride_h;
+  f.seqlens_k = p.seqlens_k;
+  f.rows = out_rows;
+  f.batch = p.batch, f.hq = p.heads_q, f.hkv = p.heads_kv, f.group = a.group, f.nq = p.seqlen_q, f.nk = p.seqlen_k;
+  f.causal = a.causal, f.n_split = S, f.split_len = split_len;
+  if (p.head_dim == 64) {
+    e = bf ? launch_finish<64, BF16>(f, merge, scores, stream, err) : launch_finish<64, F16>(f, merge, scores, stream, err);
+  } else if (p.head_dim == 128) {
+    e = bf ? launch_finish<128, BF16>(f, merge, scores, stream, err) : launch_finish<128, F16>(f, merge, scores, stream, err);
+  } else {
+    e = bf ? launch_finish<256, BF16>(f, merge, scores, stream, err) : launch_finish<256, F16>(f, merge, scores, stream, err);
+  }
+  return hip_status(e, err);
 }
 
 }  // namespace fa

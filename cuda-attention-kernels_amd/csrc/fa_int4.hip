@@ -109,69 +109,93 @@ __device__ __forceinline__ uint32_t encode(const Chunk<T>& c, uint32_t& pair) {
   return codes;
 }
 
-// Bulk writer.  Workgroup blk: rows blk * ROWS .. of the flattened [B, H, N].
-template <class T, int D, int UNROLL>
+// Where the rows of a lane are.  A workgroup takes UNROLL * RPS rows, RPS a step: those of one (batch, head) from n0 on,
+// or where a head has fewer rows than half of that (FLAT: pages, single tokens) those of the flattened [B, H, N], at two
+// divisions a row.
+template <bool FLAT, int RPS, int UNROLL>
+struct RowPlace {
+  int b[UNROLL], h[UNROLL], n[UNROLL];
+  bool ok[UNROLL];
+  __device__ __forceinline__ RowPlace(const Int4Args& a, int first) {
+    if constexpr (FLAT) {
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int64_t row = (int64_t)blockIdx.x * (RPS * UNROLL) + first + u * RPS;
+        ok[u] = row < a.rows;
+        const uint32_t r = ok[u] ? (uint32_t)row : 0u, bh = r / (uint32_t)a.n;
+        n[u] = (int)(r - bh * (uint32_t)a.n);
+        b[u] = (int)(bh / (uint32_t)a.h);
+        h[u] = (int)(bh - (uint32_t)b[u] * (uint32_t)a.h);
+      }
+    } else {
+      const uint32_t bh = blockIdx.x / (uint32_t)a.chunks, b0 = bh / (uint32_t)a.h;
+      const int n0 = (int)(blockIdx.x - bh * (uint32_t)a.chunks) * (RPS * UNROLL) + first;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        b[u] = (int)b0;
+        h[u] = (int)(bh - b0 * (uint32_t)a.h);
+        n[u] = n0 + u * RPS;
+        ok[u] = n[u] < a.n;
+      }
+    }
+  }
+  __device__ __forceinline__ int64_t at(int u, int64_t sb, int64_t sh, int64_t sn) const {
+    return b[u] * sb + h[u] * sh + n[u] * sn;
+  }
+};
+
+// Bulk writer.
+template <class T, int D, int UNROLL, bool FLAT>
 __global__ void __launch_bounds__(kBlock) quantize_kv_int4_kernel(const Int4Args a) {
   constexpr int LPR = D / 8, RPS = kBlock / LPR;  // lanes a row, rows a step
   const int lane = (int)threadIdx.x % LPR;
-  const int64_t row0 = (int64_t)blockIdx.x * (RPS * UNROLL) + (int)threadIdx.x / LPR;
+  const RowPlace<FLAT, RPS, UNROLL> at(a, (int)threadIdx.x / LPR);
   Chunk<T> c[UNROLL];
-  int b[UNROLL], h[UNROLL], n[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    const int64_t row = row0 + u * RPS;
-    if (row >= a.rows) continue;
-    const uint32_t bh = (uint32_t)row / (uint32_t)a.n;  // rows < 2^31 (host)
-    n[u] = (int)((uint32_t)row - bh * (uint32_t)a.n);
-    b[u] = (int)(bh / (uint32_t)a.h);
-    h[u] = (int)(bh - (uint32_t)b[u] * (uint32_t)a.h);
-    c[u] = load_chunk((const T*)a.x + b[u] * a.sxb + h[u] * a.sxh + n[u] * a.sxn + 8 * lane);
+    if (at.ok[u]) c[u] = load_chunk((const T*)a.x + at.at(u, a.sxb, a.sxh, a.sxn) + 8 * lane);
   }
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    if (row0 + u * RPS >= a.rows) continue;  // whole rows: their lanes leave together
+    if (!at.ok[u]) return;  // whole rows: their lanes leave together
     uint32_t pair;
-    const uint32_t codes = encode<T, LPR>(c[u], pair);
-    *(uint32_t*)(a.codes + b[u] * a.scb + h[u] * a.sch + n[u] * a.scn + 4 * lane) = codes;
-    if (lane == 0) a.pairs[b[u] * a.ssb + h[u] * a.ssh + n[u] * a.ssn] = pair;
+    const uint32_t w = encode<T, LPR>(c[u], pair);
+    *(uint32_t*)(a.codes + at.at(u, a.scb, a.sch, a.scn) + 4 * lane) = w;
+    if (lane == 0) a.pairs[at.at(u, a.ssb, a.ssh, a.ssn)] = pair;
   }
 }
 
 // The reader: floats from codes.  code * scale is exact in fp32, so a value takes one rounding there and one to T.
-template <class T, int D, int UNROLL>
+template <class T, int D, int UNROLL, bool FLAT>
 __global__ void __launch_bounds__(kBlock) dequantize_kv_int4_kernel(const Int4Args a) {
   constexpr int LPR = D / 8, RPS = kBlock / LPR;
   const int lane = (int)threadIdx.x % LPR;
-  const int64_t row0 = (int64_t)blockIdx.x * (RPS * UNROLL) + (int)threadIdx.x / LPR;
-  uint32_t codes[UNROLL], pair[UNROLL];
-  T* out[UNROLL];
+  const RowPlace<FLAT, RPS, UNROLL> at(a, (int)threadIdx.x / LPR);
+  uint32_t w[UNROLL], pair[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    const int64_t row = row0 + u * RPS;
-    if (row >= a.rows) continue;
-    const uint32_t bh = (uint32_t)row / (uint32_t)a.n;
-    const int n = (int)((uint32_t)row - bh * (uint32_t)a.n), b = (int)(bh / (uint32_t)a.h);
-    const int h = (int)(bh - (uint32_t)b * (uint32_t)a.h);
-    codes[u] = *(const uint32_t*)(a.codes + b * a.scb + h * a.sch + n * a.scn + 4 * lane);
-    pair[u] = a.pairs[b * a.ssb + h * a.ssh + n * a.ssn];
-    out[u] = (T*)a.x + b * a.sxb + h * a.sxh + n * a.sxn + 8 * lane;
+    if (at.ok[u]) {
+      w[u] = *(const uint32_t*)(a.codes + at.at(u, a.scb, a.sch, a.scn) + 4 * lane);
+      pair[u] = a.pairs[at.at(u, a.ssb, a.ssh, a.ssn)];
+    }
   }
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    if (row0 + u * RPS >= a.rows) continue;
+    if (!at.ok[u]) return;
     const float scale = lo_f32<F16>(pair[u]), zero = hi_f32<F16>(pair[u]);
+    T* out = (T*)a.x + at.at(u, a.sxb, a.sxh, a.sxn) + 8 * lane;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = rounded(__builtin_fmaf((float)((codes[u] >> (4 * e)) & 15u), scale, zero));
+    for (int e = 0; e < 8; ++e) v[e] = rounded(__builtin_fmaf((float)((w[u] >> (4 * e)) & 15u), scale, zero));
     if constexpr (sizeof(T) == 4) {
       __builtin_nontemporal_store(u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                                        __float_as_uint(v[3])}, (u32x4*)out[u]);
+                                        __float_as_uint(v[3])}, (u32x4*)out);
       __builtin_nontemporal_store(u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]),
-                                        __float_as_uint(v[7])}, (u32x4*)out[u] + 1);
+                                        __float_as_uint(v[7])}, (u32x4*)out + 1);
     } else {
       using Tag = typename std::conditional<std::is_same<T, __bf16>::value, BF16, F16>::type;
       __builtin_nontemporal_store(u32x4{pack2<Tag>(v[0], v[1]), pack2<Tag>(v[2], v[3]), pack2<Tag>(v[4], v[5]),
-                                        pack2<Tag>(v[6], v[7])}, (u32x4*)out[u]);
+                                        pack2<Tag>(v[6], v[7])}, (u32x4*)out);
     }
   }
 }
@@ -227,13 +251,20 @@ Int4Args int4_args(const fa_int4_params& p) {
 constexpr int kUnroll = 4;
 
 template <class T, int D>
-hipError_t launch_rows(const Int4Args& a, bool read, hipStream_t stream) {
+hipError_t launch_rows(Int4Args a, bool read, hipStream_t stream, const char** err) {
   constexpr int per = kBlock / (D / 8) * kUnroll;
-  const dim3 grid((unsigned)((a.rows + per - 1) / per));
+  const bool flat = a.n < per / 2 && a.rows <= INT32_MAX;
+  a.chunks = (a.n - 1) / per + 1;
+  const int64_t blocks = flat ? (a.rows + per - 1) / per : a.rows / a.n * a.chunks;
+  if (blocks > INT32_MAX) {
+    *err = "too many rows";
+    return hipErrorInvalidConfiguration;
+  }
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, stream, a); };
   if (read) {
-    hipLaunchKernelGGL((dequantize_kv_int4_kernel<T, D, kUnroll>), grid, dim3(kBlock), 0, stream, a);
+    flat ? launch(dequantize_kv_int4_kernel<T, D, kUnroll, true>) : launch(dequantize_kv_int4_kernel<T, D, kUnroll, false>);
   } else {
-    hipLaunchKernelGGL((quantize_kv_int4_kernel<T, D, kUnroll>), grid, dim3(kBlock), 0, stream, a);
+    flat ? launch(quantize_kv_int4_kernel<T, D, kUnroll, true>) : launch(quantize_kv_int4_kernel<T, D, kUnroll, false>);
   }
   return hipGetLastError();
 }
@@ -260,12 +291,12 @@ hipError_t by_type(int dtype, int d, F&& f) {
 
 fa_status run_int4_rows(const fa_int4_params& p, bool read, hipStream_t stream, const char** err) {
   const Int4Args a = int4_args(p);
-  if (a.rows > INT32_MAX - kBlock * kUnroll) {
+  if (p.seqlen > (1 << 30)) {
     *err = "too many rows";
     return FA_ERR_UNSUPPORTED;
   }
   return hip_status(by_type(p.dtype, p.head_dim, [&](auto t, auto d) {
-    return launch_rows<decltype(t), decltype(d)::value>(a, read, stream);
+    return launch_rows<decltype(t), decltype(d)::value>(a, read, stream, err);
   }), err);
 }
 

@@ -89,6 +89,7 @@ struct Int4Args {
   int64_t sxb, sxh, sxn, scb, sch, scn, ssb, ssh, ssn;
   int64_t rows;  // batch * h * n
   int32_t h, n;
+  int32_t chunks;  // workgroups per (batch, head)
 };
 
 struct AppendArgs {
@@ -119,13 +120,16 @@ struct CacheArgs {
 };
 
 struct FinishArgs {
+  const float* part;  // partials and their (max, sum), as CacheArgs
+  const float* ml;
+  void* o;
+  float* lse;  // written by the merge (may be NULL), or read where use_lse
   const float* raw;
-  const float* lse;
   const float* in;
   float* out;
-  int64_t raw_stride, slb, slh, sib, sih, sob, soh;
+  int64_t sob, soh, son, slb, slh, raw_stride, sib, sih, sob_s, soh_s, rows;
   const int32_t* seqlens_k;
-  int32_t hkv, group, nq, nk, causal, chunks;
+  int32_t batch, hq, hkv, group, nq, nk, causal, n_split, split_len, chunks, merge_blocks, use_lse;
 };
 
 // Eviction (fa_evict.hip): strides of the tensors in bytes.
@@ -141,10 +145,9 @@ struct EvictArgs {
   int64_t ssb, ssh;
   const int32_t* seqlens_k;
   int32_t* index;
-  float* scores_out;
   int32_t* seqlens_out;
   int32_t h, nk, keep, recent, chunks;
-  EvictTensor tensors[FA_MAX_EVICT_TENSORS];
+  EvictTensor tensors[FA_MAX_EVICT_TENSORS + 1];  // the scores first
 };
 
 // Number of rows (q-heads x queries) one split-K workgroup covers, and the
@@ -156,7 +159,7 @@ TileArgs common_args(const fa_fwd_params& p);
 
 inline fa_status hip_status(hipError_t e, const char** err) {
   if (e == hipSuccess) return FA_OK;
-  *err = hipGetErrorString(e);
+  if (*err == nullptr) *err = hipGetErrorString(e);  // (a launcher may have said more)
   return FA_ERR_HIP;
 }
 
