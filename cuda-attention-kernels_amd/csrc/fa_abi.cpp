@@ -171,6 +171,9 @@ fa_status validate_cache(const fa_cache_params* p, int32_t split_len) {
   // tiles of 32 rows are addressed with 32-bit byte offsets
   if (p->k_stride_n < 0 || p->v_stride_n < 0 || p->k_stride_n * kvb >= (1 << 24) || p->v_stride_n * kvb >= (1 << 24))
     return fail(FA_ERR_UNSUPPORTED, "k/v token stride must be below 16 MiB");
+  if (i4 && (p->k_scale_stride_n < 0 || p->v_scale_stride_n < 0 || p->k_scale_stride_n >= (1 << 22) ||
+             p->v_scale_stride_n >= (1 << 22)))
+    return fail(FA_ERR_UNSUPPORTED, "k/v scale token stride must be below 16 MiB");
   if (p->lse != nullptr && (p->lse_stride_b < 0 || p->lse_stride_h < 0))
     return fail(FA_ERR_INVALID_ARGUMENT, "negative LSE stride");
   if (!aligned(p->scores_in, 4) || !aligned(p->scores_out, 4) || !aligned(p->seqlens_k, 4))

@@ -31,7 +31,8 @@
 //
 // Scores.  p needs the row's final sum, which no partition has.  The s of a row and key are written as they are
 // (4 bytes: 6% of a 16-bit key's bytes at D=128 and four rows, 12% of a 4-bit one's), and cache_finish_kernel turns them into
-// weights once the partitions' sums are there.  A second pass over K would read half the cache again.
+// weights once the partitions' sums are there.  They lie tile by tile, the rows of 32 keys
+// together, so that a workgroup writes one run of memory.  A second pass over K would read half the cache again.
 #include <algorithm>
 
 #include "fa_device.hpp"
@@ -385,6 +386,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
     }
   };
   // p = 2^(s - m), and O += P V
+  float raw[SCORES ? RT : 1][8];  // scored: this tile's scores
   auto product_v = [&](const Tile& vt, f32x4(&acc)[RT][2], int n0) __attribute__((always_inline)) {
     u32x4 pf[RT], pl[RT];
     f32x4 kp[4], vp[4];
@@ -420,14 +422,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       float s[8];
       if constexpr (SCORES) {
         scores_less(0.f, s);
-        const int row = r0 + 16 * t + c;
-        if (row < R) {
-          float* out = a.raw + ((int64_t)(b * a.hkv + kvh) * R + row) * a.raw_stride + n0 + 8 * g;
-          st16(out, __builtin_bit_cast(u32x4, f32x4{s[0], s[1], s[2], s[3]}));
-          st16(out + 4, __builtin_bit_cast(u32x4, f32x4{s[4], s[5], s[6], s[7]}));
-        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] -= m_run[t];
+        for (int i = 0; i < 8; ++i) {
+          raw[t][i] = s[i];
+          s[i] -= m_run[t];
+        }
       } else {
         scores_less(m_run[t], s);
       }
@@ -516,6 +515,22 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       }
     }
   };
+  // Rows past R are beyond the descriptor's limit and dropped, without a branch around the stores (loads and stores share
+  // one counter: a wait after stores that may have been skipped waits for too much).
+  auto store_scores = [&](int n0) __attribute__((always_inline)) {
+    if constexpr (SCORES) {
+      const float* out = a.raw + ((int64_t)(b * a.hkv + kvh) * a.raw_tiles + n0 / kTile) * R * kTile;
+      const auto r = make_rsrc(out, (uint32_t)R * kTile * 4);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int at = ((r0 + 16 * t + c) * kTile + 8 * g) * 4;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(u32x4, f32x4{raw[t][i], raw[t][i + 1], raw[t][i + 2], raw[t][i + 3]}), r, at + 4 * i, 0, 0);
+      }
+    }
+  };
   // the tile's pairs through LDS: each lane converts one, every lane reads eight keys'
   auto store_pair = [&](uint32_t w) __attribute__((always_inline)) {
     if constexpr (I4) {
@@ -535,6 +550,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       f32x4 acc[RT][2];
       product_k(cur, acc);
       product_v(cur, acc, n0);
+      store_scores(n0);
       n0 += STEP;
     };
     while (n0 <= last) {
@@ -553,6 +569,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       if (n0 + STEP <= last) load_k_dense(n0 + STEP, t);
       product_v(t, acc, n0);
       if (n0 + STEP <= last) load_v_dense(n0 + STEP, t);
+      store_scores(n0);
     }
   }
 
@@ -700,7 +717,7 @@ __device__ __forceinline__ void finish_scores(const FinishArgs& a) {
   const int R = a.group * a.nq, offset = seq_k - a.nq, w0 = wave % NW;
   const int S = a.seqlens_k != nullptr ? min(a.n_split, (seq_k + a.split_len - 1) / a.split_len) : a.n_split;
   const int64_t prow = ((int64_t)b * a.hq + kvh * a.group) * a.nq;  // (row r of the group: prow + r)
-  const float* raw = a.raw + (int64_t)bh * R * a.raw_stride + j;
+  const float* raw = a.raw + ((int64_t)bh * a.raw_tiles + j / kTile) * R * kTile + j % kTile;
   f32x4 w = {};
   for (int r0 = 0; r0 < R && block0 < seq_k; r0 += kFinishRows) {
     const int rows = min(kFinishRows, R - r0);
@@ -728,7 +745,7 @@ __device__ __forceinline__ void finish_scores(const FinishArgs& a) {
         int end = a.causal ? min(seq_k, (r0 + r) % a.nq + offset + 1) : seq_k;
         end = l2 == NEG_INF ? 0 : end;  // (every key of the row scores -inf)
         f32x4 s = {};
-        if (j < end) s = __builtin_bit_cast(f32x4, ld16(raw + (r0 + r) * a.raw_stride));
+        if (j < end) s = __builtin_bit_cast(f32x4, ld16(raw + (r0 + r) * kTile));
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] += j + i < end ? fast_exp2(s[i] - l2) : 0.f;
       }
@@ -804,7 +821,7 @@ hipError_t launch_cache(const CacheArgs& a, bool i4, bool paged, bool scores, in
                 : launch_rows<D, E, true, false, false>(a, rt, stream);
 }
 
-int64_t raw_stride(const fa_cache_params& p) { return ((int64_t)p.seqlen_k + kTile - 1) / kTile * kTile; }
+int raw_tiles(const fa_cache_params& p) { return (p.seqlen_k + kTile - 1) / kTile; }
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -818,7 +835,7 @@ size_t cache_workspace_bytes(const fa_cache_params& p, int32_t split_len) {
   size_t need = align16(fa_splitk_workspace_bytes(p.batch, p.heads_q, p.seqlen_q, p.head_dim, splits(p, split_len)));
   if (p.scores_out != nullptr) {
     const size_t rows = (size_t)p.batch * p.heads_q * p.seqlen_q;
-    need += align16(rows * sizeof(float)) + rows * (size_t)raw_stride(p) * sizeof(float);
+    need += align16(rows * sizeof(float)) + rows * (size_t)raw_tiles(p) * kTile * sizeof(float);
   }
   return need;
 }
@@ -868,7 +885,7 @@ fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace
   if (scores) {
     float* own = (float*)(ws + align16(fa_splitk_workspace_bytes(p.batch, p.heads_q, p.seqlen_q, p.head_dim, S)));
     a.raw = (float*)((uint8_t*)own + align16((size_t)out_rows * sizeof(float)));
-    a.raw_stride = raw_stride(p);
+    a.raw_tiles = raw_tiles(p);
     if (lse == nullptr) lse = own, slb = (int64_t)p.heads_q * p.seqlen_q, slh = p.seqlen_q;
   }
   const bool bf = p.dtype == FA_DTYPE_BF16;
@@ -896,7 +913,7 @@ fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace
   FinishArgs f{};
   f.part = a.part, f.ml = a.ml, f.o = p.o;
   f.sob = p.o_stride_b, f.soh = p.o_stride_h, f.son = p.o_stride_n;
-  f.raw = a.raw, f.raw_stride = a.raw_stride;
+  f.raw = a.raw, f.raw_tiles = a.raw_tiles;
   f.lse = merge ? p.lse : lse, f.slb = slb, f.slh = slh;
   f.use_lse = merge ? 0 : 1;
   f.in = p.scores_in, f.sib = p.scores_in_stride_b, f.sih = p.scores_in_stride_h;

@@ -106,13 +106,13 @@ struct CacheArgs {
   const void *q, *k, *v, *k_scale, *v_scale;
   float* part;  // normalised fp32 partials [B, Hq, Nq, S, D]
   float* ml;    // their (max, sum)
-  float* raw;   // scored: log2-domain scores [B, Hkv, G * Nq, raw_stride]
+  float* raw;   // scored: log2-domain scores [B, Hkv, raw_tiles, G * Nq, 32 keys]
   int64_t sqb, sqh, sqn, skb, skh, skn, svb, svh, svn;
   int64_t sksb, sksh, sksn, svsb, svsh, svsn;
-  int64_t raw_stride, sbt;
+  int64_t sbt;
   const int32_t* seqlens_k;
   const int32_t* block_table;
-  int32_t batch, hq, hkv, group, nq, nk;
+  int32_t batch, hq, hkv, group, nq, nk, raw_tiles;
   int32_t n_rowblk, n_split, split_len, n_items, total;
   int32_t causal, page_size, num_pages, page_magic_shift;
   uint32_t page_magic;
@@ -127,9 +127,9 @@ struct FinishArgs {
   const float* raw;
   const float* in;
   float* out;
-  int64_t sob, soh, son, slb, slh, raw_stride, sib, sih, sob_s, soh_s, rows;
+  int64_t sob, soh, son, slb, slh, sib, sih, sob_s, soh_s, rows;
   const int32_t* seqlens_k;
-  int32_t batch, hq, hkv, group, nq, nk, causal, n_split, split_len, chunks, merge_blocks, use_lse;
+  int32_t batch, hq, hkv, group, nq, nk, causal, n_split, split_len, chunks, merge_blocks, use_lse, raw_tiles;
 };
 
 // Eviction (fa_evict.hip): strides of the tensors in bytes.

@@ -891,25 +891,39 @@ INT4_HEAD_DIMS = (64, 128, 256)
 
 
 def _strides3(t: torch.Tensor, unit: int = 1) -> tuple[int, int, int]:
-    return _stride(t, 0) // unit, _stride(t, 1) // unit, _stride(t, 2) // unit
+    z, s = t.shape, t.stride()
+    return (s[0] // unit if z[0] > 1 else 0, s[1] // unit if z[1] > 1 else 0, s[2] // unit if z[2] > 1 else 0)
+
+
+def _aligned_rows(t: torch.Tensor, vec: int) -> torch.Tensor:
+    """``_aligned_view`` for rows of whole 16 bytes: a contiguous tensor needs only its start looked at."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _aligned_view(t, vec, 16)
 
 
 def _pairs_ok(t: torch.Tensor) -> bool:
     """Whether the kernels can read t's (scale, zero) pairs as 4-byte words."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 4 == 0
-            and all(t.size(i) <= 1 or (t.stride(i) >= 0 and t.stride(i) % 2 == 0) for i in range(3)))
+    if t.data_ptr() % 4:
+        return False
+    return t.is_contiguous() or (t.stride(-1) == 1 and all(
+        t.size(i) <= 1 or (t.stride(i) >= 0 and t.stride(i) % 2 == 0) for i in range(3)))
+
+
+def _word_pairs(t: torch.Tensor) -> torch.Tensor:
+    ok = _pairs_ok(t) and t.stride(2) * 2 < TOKEN_STRIDE_LIMIT_BYTES
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def check_int4_rows(codes: torch.Tensor, scale: torch.Tensor, name: str, shape=None) -> None:
     """4-bit rows: uint8 codes [B, Hkv, N, D/2] (or a pool of pages) and fp16 pairs [B, Hkv, N, 2]."""
-    if codes.dim() != 4 or codes.dtype != torch.uint8:
-        raise RuntimeError(f"{name} must be uint8 [B, Hkv, N, D/2], got {codes.dtype} {tuple(codes.shape)}")
-    if shape is not None and tuple(codes.shape) != tuple(shape):
-        raise RuntimeError(f"{name} must have shape {tuple(shape)}, got {tuple(codes.shape)}")
-    want = (*codes.shape[:3], 2)
-    if not isinstance(scale, torch.Tensor) or tuple(scale.shape) != want or scale.dtype != torch.float16:
-        got = f"{scale.dtype} {tuple(scale.shape)}" if isinstance(scale, torch.Tensor) else scale
-        raise RuntimeError(f"the scale of {name} must be float16 {want}, (scale, zero) a row, got {got}")
+    cs = codes.shape
+    if len(cs) != 4 or codes.dtype != torch.uint8:
+        raise RuntimeError(f"{name} must be uint8 [B, Hkv, N, D/2], got {codes.dtype} {tuple(cs)}")
+    if shape is not None and cs != shape:
+        raise RuntimeError(f"{name} must have shape {tuple(shape)}, got {tuple(cs)}")
+    ss = scale.shape if isinstance(scale, torch.Tensor) else ()
+    if len(ss) != 4 or ss[3] != 2 or ss[:3] != cs[:3] or scale.dtype != torch.float16:
+        got = f"{scale.dtype} {tuple(ss)}" if isinstance(scale, torch.Tensor) else scale
+        raise RuntimeError(f"the scale of {name} must be float16 {(*cs[:3], 2)}, (scale, zero) a row, got {got}")
     if scale.device != codes.device:
         raise RuntimeError(f"the scale of {name} must be on {codes.device}, got {scale.device}")
 
@@ -939,7 +953,8 @@ def _check_float_rows(x: torch.Tensor, name: str = "x") -> None:
 def quantize_kv_int4(x: torch.Tensor, out=None):
     """x [B,Hkv,N,D] -> (codes uint8 [B,Hkv,N,D/2], (scale, zero) fp16 [B,Hkv,N,2]), into ``out`` if given."""
     _check_float_rows(x)
-    shape = (*x.shape[:3], x.shape[3] // 2)
+    b, h, n, d = x.shape
+    shape = (b, h, n, d // 2)
     if out is not None:
         codes, scale = out
         check_int4_rows(codes, scale, "out", shape)
@@ -948,9 +963,9 @@ def quantize_kv_int4(x: torch.Tensor, out=None):
     else:
         _require_gpu(x)
         codes = torch.empty(shape, dtype=torch.uint8, device=x.device)
-        scale = torch.empty((*x.shape[:3], 2), dtype=torch.float16, device=x.device)
+        scale = torch.empty((b, h, n, 2), dtype=torch.float16, device=x.device)
     lib = _cache_library()
-    x = _aligned_view(x, 16 // x.element_size(), 16)
+    x = _aligned_rows(x, 16 // x.element_size())
     with _on_device(x.device):
         _check(lib.fa_quantize_kv_int4(_int4_params(x, codes, scale), _stream(x)), "quantize_kv_int4")
     return codes, scale
@@ -964,7 +979,7 @@ def dequantize_kv_int4(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dt
     _check_float_rows(x, "the result")
     lib = _cache_library()
     codes = _aligned_view(codes, 4, 4)
-    scale = scale if _pairs_ok(scale) else scale.clone(memory_format=torch.contiguous_format)
+    scale = _word_pairs(scale)
     with _on_device(codes.device):
         _check(lib.fa_dequantize_kv_int4(_int4_params(x, codes, scale), _stream(codes)), "dequantize_kv_int4")
     return x
@@ -1012,7 +1027,7 @@ def append_kv_int4(k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, block_ta
     _require_gpu(k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, *([] if block_table is None else [block_table]))
     lib = _cache_library()
     vec = 16 // k.element_size()
-    k, v = _aligned_view(k, vec, 16), _aligned_view(v, vec, 16)
+    k, v = _aligned_rows(k, vec), _aligned_rows(v, vec)
     seqlens_k = seqlens_k.contiguous()
     if k_cache.numel() == 0:
         return
@@ -1051,7 +1066,29 @@ def check_cache_attention(q, k, v, k_scale, v_scale, paged: bool = False) -> boo
     return True
 
 
-def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split_len: int, seqlens_k=None,
+# Default partitions: workgroups that they make (of up to 32 rows, of 64), the shortest and longest (keys), the most
+CACHE_TARGET_WGS = {16: 1024, 32: 1024, 64: 320}
+MIN_CACHE_KEYS = 128
+MAX_CACHE_KEYS = 4096
+MAX_CACHE_SPLITS = 128
+
+
+def default_cache_split_len(seqlen_q: int, seqlen_k: int, batch: int, heads_kv: int, group: int, head_dim: int) -> int:
+    """Keys per partition when the caller does not choose: as long as the grid keeps about CACHE_TARGET_WGS
+    workgroups, in whole rounds of a workgroup's four waves of 32 keys.
+
+    A workgroup costs about 4 us before and after its tiles, and more with 64 rows, whose merge moves 64 KiB through LDS
+    (8 heads, 128 rows each, 8191 keys, D=128 16-bit: 37 us at 512 keys, 72 at 128).  A lone long sequence is cut into 128
+    at most: the merge of more costs more than they save (2 x 54738 keys, D=256: 18 us at 512 keys, 34 at 128)."""
+    rows = group * seqlen_q
+    block = 16 if rows <= 16 else 32 if rows <= 32 or head_dim == 256 else 64  # rows of a workgroup
+    items = max(1, batch * heads_kv * -(-rows // block))
+    keys = -(-max(seqlen_k, 1) // min(max(1, CACHE_TARGET_WGS[block] // items), MAX_CACHE_SPLITS))
+    return int(min(max(-(-keys // 128) * 128, MIN_CACHE_KEYS), MAX_CACHE_KEYS))
+
+
+def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split_len: Optional[int],
+                    seqlens_k=None,
                     block_table=None, max_seqlen_k: Optional[int] = None, return_lse: bool = False, scores=None,
                     return_scores: bool = False):
     """Attention over a 4-bit cache (dense, or paged with ``block_table``), or scored attention over a dense cache.
@@ -1059,32 +1096,32 @@ def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split
     int4 = check_cache_attention(q, k, v, k_scale, v_scale, paged=block_table is not None)
     more = [t for t in (k_scale, v_scale, seqlens_k, block_table, scores) if t is not None]
     _require_gpu(q, k, v, *more)
-    b, hq, nq, d = q.shape
-    hkv = k.shape[1]
+    (b, hq, nq, d), hkv = q.shape, k.shape[1]
     nk = k.shape[2] if block_table is None else int(max_seqlen_k)
     if seqlens_k is not None:
         check_lengths(seqlens_k, b)
         seqlens_k = seqlens_k.contiguous()
     if scores is not None:
         check_scores(scores, (b, hkv, nk))
-        if scores.stride(-1) != 1 and nk > 1 or min(scores.stride(0), scores.stride(1)) < 0:
+        if scores.stride(-1) != 1 and nk > 1:
             scores = scores.contiguous()
+    if split_len is None:
+        split_len = default_cache_split_len(nq, nk, b, hkv, hq // hkv, d)
+        if block_table is not None:  # a partition spans at most 257 pages
+            split_len = min(split_len, max(64, 256 * k.shape[2] // 64 * 64))
+    split_len = int(split_len)
     lib = _cache_library()
-    q = _aligned_view(q, 8, 16)
     vec = 16 if int4 else 8
-    k, v = _aligned_view(k, vec, 16), _aligned_view(v, vec, 16)
+    q, k, v = _aligned_rows(q, 8), _aligned_rows(k, vec), _aligned_rows(v, vec)
     o = _new_output(q)
+    if int4:
+        k_scale, v_scale = _word_pairs(k_scale), _word_pairs(v_scale)
+        pairs = (k_scale.data_ptr(), v_scale.data_ptr(), *_strides3(k_scale, 2), *_strides3(v_scale, 2))
+    else:
+        pairs = (None, None, 0, 0, 0, 0, 0, 0)
     p = CacheParams(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *_strides3(q), *_strides3(k), *_strides3(v),
                     *_strides3(o), b, hq, hkv, nq, nk, d, float(scale), int(bool(causal)), _DTYPE_CODE[q.dtype],
-                    INT4 if int4 else _DTYPE_CODE[k.dtype])
-    if int4:
-        k_scale, v_scale = (t if _pairs_ok(t) else t.clone(memory_format=torch.contiguous_format)
-                            for t in (k_scale, v_scale))
-        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        p.k_scale_stride_b, p.k_scale_stride_h, p.k_scale_stride_n = _strides3(k_scale, 2)
-        p.v_scale_stride_b, p.v_scale_stride_h, p.v_scale_stride_n = _strides3(v_scale, 2)
-    if seqlens_k is not None:
-        p.seqlens_k = seqlens_k.data_ptr()
+                    INT4 if int4 else _DTYPE_CODE[k.dtype], *pairs, None if seqlens_k is None else seqlens_k.data_ptr())
     if block_table is not None:
         check_block_table(block_table, b)
         block_table = _plain_table(block_table)
@@ -1118,6 +1155,13 @@ def check_scores(scores: torch.Tensor, shape) -> None:
         raise RuntimeError(f"scores must be {want} [B, Hkv, Nk], got {scores.dtype} {tuple(scores.shape)}")
 
 
+def _row_elems(t: torch.Tensor) -> int:
+    n = 1
+    for z in t.shape[3:]:
+        n *= z
+    return n
+
+
 def _extent(t: torch.Tensor) -> tuple[int, int]:
     last = sum((t.size(i) - 1) * t.stride(i) for i in range(t.dim()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
@@ -1133,9 +1177,9 @@ def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
         raise RuntimeError(f"at most {MAX_EVICT_TENSORS} caches, got {len(caches)}")
     rows = min(keep, scores.shape[2])
     for t in caches:
-        if tuple(t.shape[:3]) != tuple(scores.shape):
+        if t.shape[:3] != scores.shape:
             raise RuntimeError(f"a cache must be [B, Hkv, N, ...] as scores {tuple(scores.shape)}, got {tuple(t.shape)}")
-        if t[:1, :1, :1].numel() != math.prod(t.shape[3:]) and scores.numel() or math.prod(t.shape[3:]) == 0:
+        if _row_elems(t) == 0:
             raise RuntimeError(f"a cache needs rows, got {tuple(t.shape)}")
     if seqlens_k is not None:
         check_lengths(seqlens_k, scores.shape[0])
@@ -1149,7 +1193,7 @@ def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
                                    f"got {o.dtype} {tuple(o.shape)}")
             if not _rows_contiguous(o) or any(o.size(i) > 1 and o.stride(i) <= 0 for i in range(3)):
                 raise RuntimeError("out needs contiguous rows and positive strides")
-            if o.size(2) > 1 and o.stride(2) < math.prod(o.shape[3:]):
+            if o.size(2) > 1 and o.stride(2) < _row_elems(o):
                 raise RuntimeError("rows of out overlap")
         spans = [_extent(o) for o in out if o.numel()]
         for i, (lo, hi) in enumerate(spans):
@@ -1159,6 +1203,8 @@ def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
 
 
 def _rows_contiguous(t: torch.Tensor) -> bool:
+    if t.is_contiguous():
+        return True
     want = 1
     for i in range(t.dim() - 1, 2, -1):
         if t.size(i) > 1 and t.stride(i) != want:
@@ -1181,7 +1227,7 @@ def evict_kv(scores, caches, keep: int, recent: int, seqlens_k, out):
     index = torch.empty((b, h, keep), dtype=torch.int32, device=dev)
     kept = torch.empty((b, h, keep), dtype=torch.float32, device=dev)
     lens = torch.empty((b,), dtype=torch.int32, device=dev)
-    dst = [torch.empty((b, h, keep, *t.shape[3:]), dtype=t.dtype, device=dev) for t in caches] if out is None else list(out)
+    dst = [t.new_empty((b, h, keep, *t.shape[3:])) for t in caches] if out is None else out
     if h == 0:
         lens = torch.full((b,), n, dtype=torch.int32, device=dev) if seqlens_k is None else seqlens_k.clamp(0, n)
         return dst, kept, index, lens.clamp(max=keep)
@@ -1191,7 +1237,7 @@ def evict_kv(scores, caches, keep: int, recent: int, seqlens_k, out):
     for i, (s, d) in enumerate(zip(caches, dst)):
         size = s.element_size()
         p.tensors[i] = EvictTensor(s.data_ptr(), d.data_ptr(), *(x * size for x in _strides3(s)),
-                                   *(x * size for x in _strides3(d)), math.prod(s.shape[3:]) * size)
+                                   *(x * size for x in _strides3(d)), _row_elems(s) * size)
     with _on_device(dev):
         _check(lib.fa_evict_kv(p, _stream(scores)), "evict_kv")
     return dst, kept, index, lens

@@ -18,7 +18,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _hip
-from .int4 import attention_lengths_reference, default_cache_split_len, dequantize_kv_int4
+from .int4 import attention_lengths_reference, dequantize_kv_int4
 from .ops import _pick_backend
 
 
@@ -37,21 +37,18 @@ def attention_scored(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scores: 
 
     Made for decode steps, and for the last queries of a prompt: the scores of every (q-head, query, key) are held for
     the duration of the call, 4 bytes each."""
-    int4 = _hip.check_cache_attention(q, k, v, k_scale, v_scale)
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if q.is_cuda and _pick_backend(q) == "hip":
+        return _hip.cache_attention(q, k, v, k_scale, v_scale, causal, scale, split_len, seqlens_k=seqlens_k, scores=scores,
+                                    return_scores=True)
+    if _hip.check_cache_attention(q, k, v, k_scale, v_scale):
+        k, v = dequantize_kv_int4(k, k_scale), dequantize_kv_int4(v, v_scale)
     if scores is not None:
         _hip.check_scores(scores, (q.shape[0], k.shape[1], k.shape[2]))
-    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-    if not q.is_cuda or _pick_backend(q) != "hip":
-        if seqlens_k is not None:
-            _hip.check_lengths(seqlens_k, q.shape[0])
-        if int4:
-            k, v = dequantize_kv_int4(k, k_scale), dequantize_kv_int4(v, v_scale)
-        o, _, weights = attention_lengths_reference(q, k, v, causal, scale, seqlens_k)
-        return o, weights if scores is None else scores + weights
-    if split_len is None:
-        split_len = default_cache_split_len(q.shape[2], k.shape[2], q.shape[0], k.shape[1], q.shape[1] // k.shape[1])
-    return _hip.cache_attention(q, k, v, k_scale, v_scale, causal, scale, int(split_len), seqlens_k=seqlens_k,
-                                scores=scores, return_scores=True)
+    if seqlens_k is not None:
+        _hip.check_lengths(seqlens_k, q.shape[0])
+    o, _, weights = attention_lengths_reference(q, k, v, causal, scale, seqlens_k)
+    return o, weights if scores is None else scores + weights
 
 
 def evict_kv(scores: torch.Tensor, caches: Sequence[torch.Tensor], keep: int, recent: int = 0,

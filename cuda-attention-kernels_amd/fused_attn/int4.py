@@ -28,10 +28,6 @@ from .ops import _pick_backend
 from .reference import attention_reference, lse_reference
 
 FP16_MAX = 65504.0
-# Workgroups that the default partitions make, and the shortest and longest partitions (keys)
-CACHE_TARGET_WGS = 1024
-MIN_CACHE_KEYS = 128
-MAX_CACHE_KEYS = 4096
 
 
 def quantize_kv_int4(x: torch.Tensor, out: Optional[tuple] = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -100,15 +96,6 @@ def append_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, k_sc
                 codes[at, :, pos], scale[at, :, pos] = c[b, :, i], s[b, :, i]
 
 
-def default_cache_split_len(seqlen_q: int, seqlen_k: int, batch: int, heads_kv: int, group: int) -> int:
-    """Keys per partition when the caller does not choose: as long as the grid keeps about CACHE_TARGET_WGS
-    workgroups, in whole rounds of a workgroup's four waves of 32 keys."""
-    rows = group * seqlen_q
-    items = max(1, batch * heads_kv * -(-rows // (16 if rows <= 16 else 32)))
-    keys = -(-max(seqlen_k, 1) // max(1, CACHE_TARGET_WGS // items))
-    return int(min(max(-(-keys // 128) * 128, MIN_CACHE_KEYS), MAX_CACHE_KEYS))
-
-
 def attention_lengths_reference(q, k, v, causal: bool, scale: float, seqlens_k=None):
     """The unfused path over the first ``seqlens_k[b]`` keys of each sequence: (o, lse, weights [B, Hkv, Nk])."""
     b, hq, nq, _ = q.shape
@@ -139,17 +126,15 @@ def attention_int4(q: torch.Tensor, k4: torch.Tensor, k_scale: torch.Tensor, v4:
     ``seqlens_k`` (int32 [B], on the device): only the first seqlens_k[b] rows of sequence b are keys, and ``causal``
     aligns its queries to their end; the rows behind them are not read.  Any number of queries is accepted; the kernel
     is made for decode (few queries)."""
-    _hip.check_cache_attention(q, k4, v4, k_scale, v_scale)
     if k4.dtype != torch.uint8:
         raise RuntimeError(f"attention_int4 needs 4-bit K/V (uint8), got {k4.dtype}")
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if not q.is_cuda or _pick_backend(q) != "hip":
+        _hip.check_cache_attention(q, k4, v4, k_scale, v_scale)
         if seqlens_k is not None:
             _hip.check_lengths(seqlens_k, q.shape[0])
         k, v = dequantize_kv_int4(k4, k_scale), dequantize_kv_int4(v4, v_scale)
         o, lse, _ = attention_lengths_reference(q, k, v, causal, scale, seqlens_k)
         return (o, lse) if return_lse else o
-    if split_len is None:
-        split_len = default_cache_split_len(q.shape[2], k4.shape[2], q.shape[0], k4.shape[1], q.shape[1] // k4.shape[1])
-    return _hip.cache_attention(q, k4, v4, k_scale, v_scale, causal, scale, int(split_len), seqlens_k=seqlens_k,
+    return _hip.cache_attention(q, k4, v4, k_scale, v_scale, causal, scale, split_len, seqlens_k=seqlens_k,
                                 return_lse=return_lse)

@@ -37,7 +37,7 @@ import torch
 
 from . import _hip
 from .fp8 import FP8_DTYPE, QBLOCK, dequantize_kv_fp8
-from .int4 import default_cache_split_len, dequantize_kv_int4
+from .int4 import dequantize_kv_int4
 from .ops import _pick_backend, default_split_len
 from .reference import attention_reference, lse_reference
 
@@ -107,12 +107,11 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     fp8 = FP8_DTYPE is not None and k_cache.dtype == FP8_DTYPE
     int4 = k_cache.dtype == torch.uint8
-    if int4:
-        _hip.check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, paged=True)
-        _hip.check_block_table(block_table, q.shape[0])
-        _hip.check_lengths(seqlens_k, q.shape[0])
     if not q.is_cuda or _pick_backend(q) != "hip":
         if int4:
+            _hip.check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, paged=True)
+            _hip.check_block_table(block_table, q.shape[0])
+            _hip.check_lengths(seqlens_k, q.shape[0])
             k_cache, v_cache = dequantize_kv_int4(k_cache, k_scale), dequantize_kv_int4(v_cache, v_scale)
         if fp8:
             if k_scale is None or v_scale is None:
@@ -125,13 +124,8 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if max_seqlen_k is None:
         max_seqlen_k = int(seqlens_k.max().item()) if seqlens_k.numel() else 0
     if int4:
-        if split_len is None:
-            split_len = default_cache_split_len(q.shape[2], max_seqlen_k, q.shape[0], k_cache.shape[1],
-                                                q.shape[1] // k_cache.shape[1])
-            split_len = min(split_len, max(64, (256 * k_cache.shape[2]) // 64 * 64))  # at most 257 pages
-        return _hip.cache_attention(q, k_cache, v_cache, k_scale, v_scale, causal, scale, int(split_len),
-                                    seqlens_k=seqlens_k, block_table=block_table, max_seqlen_k=max_seqlen_k,
-                                    return_lse=return_lse)
+        return _hip.cache_attention(q, k_cache, v_cache, k_scale, v_scale, causal, scale, split_len, seqlens_k=seqlens_k,
+                                    block_table=block_table, max_seqlen_k=max_seqlen_k, return_lse=return_lse)
     if split_len is None:
         b, hq, nq, d = q.shape
         hkv, page_size = k_cache.shape[1], k_cache.shape[2]

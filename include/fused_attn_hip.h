@@ -272,7 +272,7 @@ typedef struct fa_cache_params {
   int32_t causal;
   int32_t dtype;       /* of q and o */
   int32_t kv_dtype;    /* FA_DTYPE_INT4, or dtype (then scores_out is needed) */
-  const void* k_scale; /* 4-bit: the pairs of K and V, 4-byte words */
+  const void* k_scale; /* 4-bit: the pairs of K and V, 4-byte words; stride_n below 2^22 words */
   const void* v_scale;
   int64_t k_scale_stride_b, k_scale_stride_h, k_scale_stride_n;
   int64_t v_scale_stride_b, v_scale_stride_h, v_scale_stride_n;
