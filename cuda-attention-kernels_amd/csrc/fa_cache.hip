@@ -54,6 +54,7 @@ namespace {
 constexpr int kCacheWaves = 4;
 constexpr int kTile = 32;         // keys a wave step
 constexpr int kMaxSlots = 258;    // block-table entries of a partition (paged)
+constexpr int kStageFloats = 2048;  // scores that a wave holds back
 
 __device__ __forceinline__ float max_xor16(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
@@ -148,6 +149,9 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   __shared__ int table[PAGED ? kMaxSlots : 1];
   // (scale, zero) of a wave's tile as the products use them: K's 32 keys, then V's
   __shared__ __align__(16) float pairs[I4 ? kCacheWaves : 1][I4 ? 2 * kTile * 2 : 4];
+  // scored, up to 16 rows: the scores of a wave's last tiles, written out together
+  constexpr bool STAGED = SCORES && RT == 1;
+  __shared__ __align__(16) float stage[STAGED ? kCacheWaves : 1][STAGED ? kStageFloats : 4];
   __shared__ __align__(16) float merge_o[2][16 * RT][D + 4];
   __shared__ float merge_ml[2][16 * RT][2];
 
@@ -314,9 +318,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   };
 
   // the first tiles are on their way before anything waits for Q
-  constexpr int STEP = kCacheWaves * kTile;
-  const int last = klo + (n_tiles - 1) * kTile;  // the last tile's first key
-  int n0 = klo + wave * kTile;
+  // (staged scores: a wave's tiles follow each other, else the waves take every fourth)
+  constexpr int STEP = STAGED ? kTile : kCacheWaves * kTile;
+  const int share = (n_tiles + kCacheWaves - 1) / kCacheWaves;
+  int n0 = klo + (STAGED ? wave * share : wave) * kTile;
+  const int last = klo + ((STAGED ? min((wave + 1) * share, n_tiles) : n_tiles) - 1) * kTile;  // the last tile's first key
   Tile tiles[I4 ? AHEAD + 1 : 1];
 #pragma unroll
   for (int i = 0; i < (I4 ? AHEAD : 1); ++i) {
@@ -515,10 +521,29 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       }
     }
   };
-  // Rows past R are beyond the descriptor's limit and dropped, without a branch around the stores (loads and stores share
-  // one counter: a wait after stores that may have been skipped waits for too much).
+  // Staged: 33 MB of scores beside 1 GB of keys cost 60 us of 219 when every tile wrote its 512 bytes, 50
+  // so (what is left is the memory's turning between reads and writes: writes that stay in the L2 cost 10).
+  // Direct: rows past R are beyond the descriptor's limit and dropped, without a branch around the stores (loads and
+  // stores share one counter: a wait after stores that may have been skipped waits for too much).
+  const int stage_tiles = STAGED ? kStageFloats / (R * kTile) : 1;
+  int staged = 0;
+  auto flush_scores = [&](int n0) __attribute__((always_inline)) {  // n0: the last staged tile
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float* out = a.raw + ((int64_t)(b * a.hkv + kvh) * a.raw_tiles + n0 / kTile - (staged - 1)) * R * kTile;
+    for (int i = 4 * lane; i < staged * R * kTile; i += 256) st16(out + i, ld16(&stage[STAGED ? wave : 0][i]));
+    __builtin_amdgcn_wave_barrier();
+    staged = 0;
+  };
   auto store_scores = [&](int n0) __attribute__((always_inline)) {
-    if constexpr (SCORES) {
+    if constexpr (STAGED) {
+      if (c < R) {
+        float* at = &stage[wave][(staged * R + c) * kTile + 8 * g];
+        st16(at, __builtin_bit_cast(u32x4, f32x4{raw[0][0], raw[0][1], raw[0][2], raw[0][3]}));
+        st16(at + 4, __builtin_bit_cast(u32x4, f32x4{raw[0][4], raw[0][5], raw[0][6], raw[0][7]}));
+      }
+      if (++staged == stage_tiles || n0 == last) flush_scores(n0);
+    } else if constexpr (SCORES) {
       const float* out = a.raw + ((int64_t)(b * a.hkv + kvh) * a.raw_tiles + n0 / kTile) * R * kTile;
       const auto r = make_rsrc(out, (uint32_t)R * kTile * 4);
 #pragma unroll
@@ -718,7 +743,17 @@ __device__ __forceinline__ void finish_scores(const FinishArgs& a) {
   const int S = a.seqlens_k != nullptr ? min(a.n_split, (seq_k + a.split_len - 1) / a.split_len) : a.n_split;
   const int64_t prow = ((int64_t)b * a.hq + kvh * a.group) * a.nq;  // (row r of the group: prow + r)
   const float* raw = a.raw + ((int64_t)bh * a.raw_tiles + j / kTile) * R * kTile + j % kTile;
-  f32x4 w = {};
+  // the first rows' scores are on their way while their log-sum-exps are formed
+  constexpr int PRE = 8;
+  const bool masked = a.causal && a.nq > 1;  // (one query sees every key)
+  auto end_of = [&](int r) __attribute__((always_inline)) { return masked ? min(seq_k, r % a.nq + offset + 1) : seq_k; };
+  f32x4 w = {}, first[PRE];
+#pragma unroll
+  for (int u = 0; u < PRE; ++u) {
+    const int r = w0 + u * NW;
+    first[u] = f32x4{};
+    if (r < R && j < end_of(r)) first[u] = __builtin_bit_cast(f32x4, ld16(raw + r * kTile));
+  }
   for (int r0 = 0; r0 < R && block0 < seq_k; r0 += kFinishRows) {
     const int rows = min(kFinishRows, R - r0);
     if (r0 > 0) __syncthreads();
@@ -729,25 +764,40 @@ __device__ __forceinline__ void finish_scores(const FinishArgs& a) {
         x = a.lse[b * a.slb + (kvh * a.group + gi) * a.slh + (r0 + r - gi * a.nq)] * kLog2e;
       } else {
         const float* ml = a.ml + (prow + r0 + r) * a.n_split * 2;
+        f32x2 st[kMergeSplits];  // all loads in flight
+#pragma unroll
+        for (int s = 0; s < kMergeSplits; ++s) st[s] = s < S ? __builtin_bit_cast(f32x2, ld8(ml + 2 * s)) : f32x2{NEG_INF, 0.f};
         float m = NEG_INF, l = 0.f;
-        for (int s = 0; s < S; ++s) m = fmaxf(m, ml[2 * s]);
+#pragma unroll
+        for (int s = 0; s < kMergeSplits; ++s) m = fmaxf(m, st[s][0]);
         const float ref = m == NEG_INF ? 0.f : m;
-        for (int s = 0; s < S; ++s) l += fast_exp2(ml[2 * s] - ref) * ml[2 * s + 1];
+#pragma unroll
+        for (int s = 0; s < kMergeSplits; ++s) l += fast_exp2(st[s][0] - ref) * st[s][1];
         x = m + __log2f(l == 0.f ? 1.f : l);
       }
       lse2[r] = x;
     }
     __syncthreads();
+    auto add = [&](int r, const f32x4& s) __attribute__((always_inline)) {  // r: below this chunk's rows
+      const float l2 = lse2[r];
+      const int end = l2 == NEG_INF ? 0 : end_of(r0 + r);  // (-inf: every key of the row scores -inf)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += j + i < end ? fast_exp2(s[i] - l2) : 0.f;
+    };
+    int done = 0;
+    if (r0 == 0) {
+#pragma unroll
+      for (int u = 0; u < PRE; ++u) {
+        if (w0 + u * NW < rows) add(w0 + u * NW, first[u]);
+      }
+      done = PRE * NW;
+    }
     if (j0 < seq_k) {
 #pragma unroll 8
-      for (int r = w0; r < rows; r += NW) {
-        const float l2 = lse2[r];
-        int end = a.causal ? min(seq_k, (r0 + r) % a.nq + offset + 1) : seq_k;
-        end = l2 == NEG_INF ? 0 : end;  // (every key of the row scores -inf)
+      for (int r = done + w0; r < rows; r += NW) {
         f32x4 s = {};
-        if (j < end) s = __builtin_bit_cast(f32x4, ld16(raw + (r0 + r) * kTile));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] += j + i < end ? fast_exp2(s[i] - l2) : 0.f;
+        if (j < end_of(r0 + r)) s = __builtin_bit_cast(f32x4, ld16(raw + (r0 + r) * kTile));
+        add(r, s);
       }
     }
   }
@@ -762,6 +812,9 @@ __device__ __forceinline__ void finish_scores(const FinishArgs& a) {
 #pragma unroll
     for (int i = 1; i < NW; ++i) x += sums[i][t];
     out[key] = in != nullptr ? x + in[key] : x;
+  } else if (a.wide && j + 4 <= a.nk) {
+    if (in != nullptr) w += __builtin_bit_cast(f32x4, ld16(in + j));
+    st16(out + j, __builtin_bit_cast(u32x4, w));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -918,6 +971,7 @@ fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace
   f.use_lse = merge ? 0 : 1;
   f.in = p.scores_in, f.sib = p.scores_in_stride_b, f.sih = p.scores_in_stride_h;
   f.out = p.scores_out, f.sob_s = p.scores_out_stride_b, f.soh_s = p.scores_out_stride_h;
+  f.wide = (((uintptr_t)f.in | (uintptr_t)f.out) % 16 == 0 && (f.sib | f.sih | f.sob_s | f.soh_s) % 4 == 0) ? 1 : 0;
   f.seqlens_k = p.seqlens_k;
   f.rows = out_rows;
   f.batch = p.batch, f.hq = p.heads_q, f.hkv = p.heads_kv, f.group = a.group, f.nq = p.seqlen_q, f.nk = p.seqlen_k;

@@ -130,6 +130,7 @@ struct FinishArgs {
   int64_t sob, soh, son, slb, slh, sib, sih, sob_s, soh_s, rows;
   const int32_t* seqlens_k;
   int32_t batch, hq, hkv, group, nq, nk, causal, n_split, split_len, chunks, merge_blocks, use_lse, raw_tiles;
+  int32_t wide;  // the scores' rows start at 16 bytes
 };
 
 // Eviction (fa_evict.hip): strides of the tensors in bytes.
