@@ -45,7 +45,7 @@
 #define NTV (RT == 1 ? 2 : 0)
 #endif
 #ifndef WPE
-#define WPE __attribute__((amdgpu_waves_per_eu(RT == 4 ? 1 : RT == 2 ? (D == 256 ? 1 : 2) : D == 256 ? 1 : 3)))
+#define WPE __attribute__((amdgpu_waves_per_eu(RT == 4 ? (I4 && D == 64 ? 2 : 1) : RT == 2 ? (D == 256 && !I4 ? 1 : 2) : D == 256 ? 1 : 3)))
 #endif
 namespace fa {
 
@@ -141,6 +141,9 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   constexpr int VN = D / 16;                      // channels of a key that a lane holds, for V
   constexpr int VW = I4 ? VN / 8 : VN / 2;        // and their words (I4, D=64: 0, a half)
   constexpr int VR = VW == 0 ? 1 : VW;            // registers
+  // Q's operands in LDS where two waves then fit a SIMD (8 x 8 heads x 64 rows, 20000 keys: D=256 178 us with one wave,
+  // 146 so; D=64 77 and 75; at D=128 64 rows spill: 67 and 79)
+  constexpr bool QLDS = I4 && ((RT == 4 && D == 64) || (D == 256 && RT == 2));
   constexpr int AHEAD = AHEADV;                   // 4 bits: tiles in flight
   constexpr float NEG_INF = -__builtin_inff();
   using PV = typename std::conditional<I4, BF16, E>::type;  // element type of the second product
@@ -154,6 +157,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   __shared__ __align__(16) float stage[STAGED ? kCacheWaves : 1][STAGED ? kStageFloats : 4];
   __shared__ __align__(16) float merge_o[2][16 * RT][D + 4];
   __shared__ float merge_ml[2][16 * RT][2];
+  u32x4(*const qlds)[64] = (u32x4(*)[64])merge_o;  // until the merge
 
   // ---- work item --------------------------------------------------------------------------------------------
   int rb, part, kvh, b;
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   // Paged: page sizes are multiples of 16, so each half of a tile lies in one page: a scalar base each, of which a lane
   // takes the one of its keys.  Halves past khi and pages outside the pool read page 0, which exists; their pairs are
   // zero (zero keys, or masked ones).
-  auto load_paged = [&](int n0, Tile& t) __attribute__((always_inline)) {
+  auto load_paged = [&](int n0, Tile& t, auto do_k, auto do_v) __attribute__((always_inline)) {
     const uint8_t *kp[2], *vp[2];
     int64_t at[2];
     int off[2];
@@ -294,12 +298,17 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
     const uint8_t* k = (c >= 8 ? kp[1] : kp[0]) + (kkey & 15) * (int)krow + kpart;
     const uint8_t* v = (g >= 2 ? vp[1] : vp[0]) + 8 * (g & 1) * (int)vrow + vpart;
     auto rows = [&](int kr, int vr) __attribute__((always_inline)) {
+      if constexpr (do_k) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) memory_words<KW>(k + 4 * u * kr, t.k[u]);
+        for (int u = 0; u < 2; ++u) memory_words<KW>(k + 4 * u * kr, t.k[u]);
+      }
+      if constexpr (do_v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) memory_words<VW>(v + i * vr, t.v[i]);
+        for (int i = 0; i < 8; ++i) memory_words<VW>(v + i * vr, t.v[i]);
+      }
     };
     if (packed) rows(ROW_BYTES, ROW_BYTES); else rows((int)krow, (int)vrow);
+    if constexpr (!do_k) return;
     const int h = (lane >> 4) & 1;
     t.pair = 0;
     if ((h ? ok[1] : ok[0]) && n0 + (lane & 31) < khi) {
@@ -307,13 +316,29 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       t.pair = *(const uint32_t*)(pbase + word);
     }
   };
-  auto load_tile = [&](int n0, Tile& t) __attribute__((always_inline)) {
+  using Yes = std::true_type;
+  using No = std::false_type;
+  auto load_k = [&](int n0, Tile& t) __attribute__((always_inline)) {  // and the pairs
     if constexpr (PAGED) {
-      load_paged(n0, t);
+      load_paged(n0, t, Yes{}, No{});
     } else {
       load_k_dense(n0, t);
       load_pair_dense(n0, t);
+    }
+  };
+  auto load_v = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+      load_paged(n0, t, No{}, Yes{});
+    } else {
       load_v_dense(n0, t);
+    }
+  };
+  auto load_tile = [&](int n0, Tile& t) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+      load_paged(n0, t, Yes{}, Yes{});
+    } else {
+      load_k(n0, t);
+      load_v(n0, t);
     }
   };
 
@@ -323,14 +348,15 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   const int share = (n_tiles + kCacheWaves - 1) / kCacheWaves;
   int n0 = klo + (STAGED ? wave * share : wave) * kTile;
   const int last = klo + ((STAGED ? min((wave + 1) * share, n_tiles) : n_tiles) - 1) * kTile;  // the last tile's first key
-  Tile tiles[I4 ? AHEAD + 1 : 1];
+  constexpr bool REFILL = !I4 || QLDS;  // one tile's registers, refilled as they are read
+  Tile tiles[REFILL ? 1 : AHEAD + 1];
 #pragma unroll
-  for (int i = 0; i < (I4 ? AHEAD : 1); ++i) {
+  for (int i = 0; i < (REFILL ? 1 : AHEAD); ++i) {
     if (n0 + i * STEP <= last) load_tile(n0 + i * STEP, tiles[i]);
   }
 
   // ---- Q: B operands, and the sum of each row -------------------------------------------------------------
-  u32x4 qf[RT][KS];
+  u32x4 qf[QLDS ? 1 : RT][QLDS ? 1 : KS];
   float qsum[RT];
   int qlim[RT];
 #pragma unroll
@@ -352,10 +378,15 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
         for (int j = 0; j < 4; ++j) s += lo_f32<E>(v[j]) + hi_f32<E>(v[j]);
         v = u32x4{pair_lo(v[0], v[2]), pair_hi(v[0], v[2]), pair_lo(v[1], v[3]), pair_hi(v[1], v[3])};
       }
-      qf[t][m] = v;
+      if constexpr (QLDS) {
+        if (m % kCacheWaves == wave) qlds[t * KS + m][lane] = v;  // every wave holds the same
+      } else {
+        qf[t][m] = v;
+      }
     }
     qsum[t] = I4 ? sum_groups(s) : 0.f;
   }
+  if constexpr (QLDS) __syncthreads();
 
   f32x4 oacc[RT][VN];
   float m_run[RT], l_run[RT], psum[RT], zsum[RT];
@@ -387,7 +418,13 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
           ka = u32x4{kt.k[u][4 * m], kt.k[u][4 * m + 1], kt.k[u][4 * m + 2], kt.k[u][4 * m + 3]};
         }
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t][u] = mfma16<E>(ka, qf[t][m], acc[t][u]);
+        for (int t = 0; t < RT; ++t) {
+          if constexpr (QLDS) {
+            acc[t][u] = mfma16<E>(ka, qlds[t * KS + m][lane], acc[t][u]);
+          } else {
+            acc[t][u] = mfma16<E>(ka, qf[t][m], acc[t][u]);
+          }
+        }
       }
     }
   };
@@ -396,13 +433,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   auto product_v = [&](const Tile& vt, f32x4(&acc)[RT][2], int n0) __attribute__((always_inline)) {
     u32x4 pf[RT], pl[RT];
     f32x4 kp[4], vp[4];
-    if constexpr (I4) {  // keys 8g .. 8g+7: (multiplier of the product, multiplier of sum(q)), and V's two
+    if constexpr (I4) {  // keys 8g .. 8g+7: (multiplier of the product, multiplier of sum(q))
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        kp[i] = ((const f32x4*)&pairs[wave][8 * g * 2])[i];
-        vp[i] = ((const f32x4*)&pairs[wave][2 * kTile + 8 * g * 2])[i];
-      }
+      for (int i = 0; i < 4; ++i) kp[i] = ((const f32x4*)&pairs[wave][8 * g * 2])[i];
     }
+    float p[RT][8];
     const bool masked = n0 + kTile > mask_from;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -457,18 +492,24 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] -= m;
       }
-      float p[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p[i] = fast_exp2(s[i]);
-        l_run[t] += p[i];
+        p[t][i] = fast_exp2(s[i]);
+        l_run[t] += p[t][i];
       }
+    }
+    if constexpr (I4) {  // V's: 16 scale, and zero + 7.5 scale
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vp[i] = ((const f32x4*)&pairs[wave][2 * kTile + 8 * g * 2])[i];
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (I4) {
-          zsum[t] = __builtin_fmaf(p[2 * i], vp[i][1], zsum[t]);
-          zsum[t] = __builtin_fmaf(p[2 * i + 1], vp[i][3], zsum[t]);
-          const float x = p[2 * i] * vp[i][0], y = p[2 * i + 1] * vp[i][2];
+          zsum[t] = __builtin_fmaf(p[t][2 * i], vp[i][1], zsum[t]);
+          zsum[t] = __builtin_fmaf(p[t][2 * i + 1], vp[i][3], zsum[t]);
+          const float x = p[t][2 * i] * vp[i][0], y = p[t][2 * i + 1] * vp[i][2];
           pf[t][i] = pack2<BF16>(x, y);
           psum[t] = sum2<BF16>(pf[t][i], psum[t]);
           if constexpr (LOW) {
@@ -476,7 +517,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
             psum[t] = sum2<BF16>(pl[t][i], psum[t]);
           }
         } else {
-          pf[t][i] = pack2<E>(p[2 * i], p[2 * i + 1]);
+          pf[t][i] = pack2<E>(p[t][2 * i], p[t][2 * i + 1]);
         }
       }
     }
@@ -567,7 +608,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
     }
   };
 
-  if constexpr (I4) {
+  if constexpr (!REFILL) {
     // AHEAD tiles are in flight while one is worked on (a ring of registers: the loop is unrolled by its size)
     auto step = [&](Tile& cur, Tile& next) __attribute__((always_inline)) {
       store_pair(cur.pair);
@@ -590,14 +631,16 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
     Tile& t = tiles[0];
     for (; n0 <= last; n0 += STEP) {
       f32x4 acc[RT][2];
+      store_pair(t.pair);
       product_k(t, acc);
-      if (n0 + STEP <= last) load_k_dense(n0 + STEP, t);
+      if (n0 + STEP <= last) load_k(n0 + STEP, t);
       product_v(t, acc, n0);
-      if (n0 + STEP <= last) load_v_dense(n0 + STEP, t);
+      if (n0 + STEP <= last) load_v(n0 + STEP, t);
       store_scores(n0);
     }
   }
 
+  if constexpr (QLDS) __syncthreads();  // every wave has read its Q
   // ---- merge the waves, 2 and 3 into 0 and 1, then 1 into 0 ------------------------------------------------------
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
