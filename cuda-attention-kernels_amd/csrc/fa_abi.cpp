@@ -146,7 +146,8 @@ fa_status validate_cache(const fa_cache_params* p, int32_t split_len) {
   if (!i4 && p->kv_dtype != p->dtype) return fail(FA_ERR_INVALID_ARGUMENT, "k/v must be 4-bit codes or have q's dtype");
   if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
     return fail(FA_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
-  if (!(p->scale - p->scale == 0.f)) return fail(FA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (!(p->scale <= 1e30f && p->scale >= -1e30f))
+    return fail(FA_ERR_INVALID_ARGUMENT, "scale must be finite, at most 1e30 in size");
   if (split_len <= 0 || split_len % 64 != 0 || split_len > (1 << 30))
     return fail(FA_ERR_INVALID_ARGUMENT, "split_len must be a positive multiple of 64, at most 2^30");
   if (!i4 && (p->scores_out == nullptr || paged))

@@ -147,6 +147,9 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   constexpr int AHEAD = AHEADV;                   // 4 bits: tiles in flight
   constexpr float NEG_INF = -__builtin_inff();
   using PV = typename std::conditional<I4, BF16, E>::type;  // element type of the second product
+  // 4 bits, bf16: Q is taken 2^10 smaller (exact down to 2^-116) and the scores' multiplier larger, so that sum(q) and the
+  // sums of q (1 + code/16) stay finite for every finite q
+  constexpr float QDOWN = I4 && std::is_same<E, BF16>::value ? 1.f / 1024.f : 1.f;
   constexpr bool LOW = I4 && std::is_same<E, F16>::value;   // P as two bf16 terms: fp16 outputs keep their precision
 
   __shared__ int table[PAGED ? kMaxSlots : 1];
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   const uint8_t* kbase = (const uint8_t*)a.k + ((PAGED ? 0 : b * a.skb) + kvh * a.skh) * (I4 ? 1 : 2);
   const uint8_t* vbase = (const uint8_t*)a.v + ((PAGED ? 0 : b * a.svb) + kvh * a.svh) * (I4 ? 1 : 2);
 
-  const float cs = a.qk_scale;  // of any sign, or 0: masked scores are set to -inf after it
+  const float cs = a.qk_scale / QDOWN;  // of any sign, or 0: masked scores are set to -inf after it
 
   // ---- loads ------------------------------------------------------------------------------------------------
   // K block u, row c: key 8 (c / 4) + 4 u + c % 4 of the tile, words of channel group g.  V slot i: key 8 g + i.
@@ -374,6 +377,10 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       const int w = I4 ? g * KS + m : 4 * m + g;
       u32x4 v = ld16(qp + 8 * w) & keep;
       if constexpr (I4) {
+        if constexpr (QDOWN != 1.f) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = pack2<E>(lo_f32<E>(v[j]) * QDOWN, hi_f32<E>(v[j]) * QDOWN);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) s += lo_f32<E>(v[j]) + hi_f32<E>(v[j]);
         v = u32x4{pair_lo(v[0], v[2]), pair_hi(v[0], v[2]), pair_lo(v[1], v[3]), pair_hi(v[1], v[3])};
@@ -473,11 +480,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       }
       mask(s);
       // The maximum follows only when a row outgrows it by 2^8 (p <= 256 until then: O and l share it): most tiles need
-      // no exchange between the lanes of a row.  The first tile's m is -inf, and s then +inf.
+      // no exchange between the lanes of a row.  The first tile's m is -inf, and s then +inf (or NaN, of a score -inf).
       float mt = s[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) mt = vmax(mt, s[i]);
-      if (__builtin_amdgcn_ballot_w64(mt > kRescaleLog2) != 0) {
+      if (__builtin_amdgcn_ballot_w64(!(mt <= kRescaleLog2)) != 0) {
         scores_less(0.f, s);
         mask(s);
         mt = s[0];

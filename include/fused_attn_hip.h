@@ -268,7 +268,7 @@ typedef struct fa_cache_params {
   int64_t v_stride_b, v_stride_h, v_stride_n; /* the page stride, stride_n the one inside a page */
   int64_t o_stride_b, o_stride_h, o_stride_n;
   int32_t batch, heads_q, heads_kv, seqlen_q, seqlen_k, head_dim;
-  float scale;
+  float scale; /* of at most 1e30 in size */
   int32_t causal;
   int32_t dtype;       /* of q and o */
   int32_t kv_dtype;    /* FA_DTYPE_INT4, or dtype (then scores_out is needed) */

@@ -274,6 +274,9 @@ PAGED = dict(block_table=0x20000, seqlens_k=0x20000, block_table_cols=4, block_t
     (dict(seqlen_k=(1 << 30) + 1), _hip.FA_ERR_UNSUPPORTED, "2\\^30"),
     (dict(scale=math.nan), _hip.FA_ERR_INVALID_ARGUMENT, "finite"),
     (dict(scale=math.inf), _hip.FA_ERR_INVALID_ARGUMENT, "finite"),
+    (dict(scale=-2e30), _hip.FA_ERR_INVALID_ARGUMENT, "1e30"),
+    (dict(k_scale_stride_n=1 << 22), _hip.FA_ERR_UNSUPPORTED, "scale token stride"),
+    (dict(v_scale_stride_n=-1), _hip.FA_ERR_UNSUPPORTED, "scale token stride"),
     (dict(k=0), _hip.FA_ERR_INVALID_ARGUMENT, "non-NULL"),
     (dict(k_scale=0), _hip.FA_ERR_INVALID_ARGUMENT, "k_scale"),
     (dict(k=0x10008), _hip.FA_ERR_INVALID_ARGUMENT, "aligned"),

@@ -61,6 +61,20 @@ def test_scored_lengths(int4, nq, causal):
 
 
 @pytest.mark.parametrize("int4", [False, True])
+@pytest.mark.parametrize("split", [64, 1024])  # 33 and 3 partitions
+@pytest.mark.parametrize("hq,nq", [(4, 1), (32, 1), (8, 25), (8, 130)])  # 2, 16, 100 and 520 rows
+def test_scored_many_rows_and_partitions(int4, split, hq, nq):
+    announce(f"scored rows int4={int4} split={split} hq={hq} nq={nq}")
+    lens = [2100, 1111]
+    q = torch.randn(2, hq, nq, 64, device="cuda", generator=gen(1)).half()
+    k, v, extra, kv, vv, pairs = _case(int4, 2, 2, 2100, 64, torch.float16, lens)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = oracle.attention(q, kv, vv, True, lens=lens)
+    got, w = fused_attn.attention_scored(q, k, v, causal=True, seqlens_k=sl, split_len=split, **extra)
+    check(got, *want, q, kv.nan_to_num(), vv.nan_to_num(), pairs, got_w=w)
+
+
+@pytest.mark.parametrize("int4", [False, True])
 def test_scored_scales_and_ragged_layouts(int4):
     announce(f"scored layouts int4={int4}")
     q = torch.randn(2, 3, 4, 64, device="cuda", generator=gen(1)).half().transpose(1, 2)
@@ -114,6 +128,35 @@ def _scores(b, h, n, kind, seed=0):
     s = torch.where((u > 0.1) & (u < 0.2), torch.full_like(s, math.inf), s)
     s = torch.where((u > 0.2) & (u < 0.3), torch.full_like(s, -math.inf), s)
     return torch.where((u > 0.3) & (u < 0.4), s * 1e-42, s)
+
+
+@pytest.mark.parametrize("n,keep,recent", [(33000, 9000, 500), (70001, 35000, 0), (150000, 149000, 7)])
+@pytest.mark.parametrize("kind", ["weights", "ties", "any"])
+def test_evict_many_keys(kind, n, keep, recent):
+    """More candidates than are held in registers at a time; ties that fill the whole threshold digit."""
+    announce(f"evict many {kind} n={n}")
+    scores = _scores(1, 2, n, kind, n)
+    _, s2, index, _ = fused_attn.evict_kv(scores, [], keep, recent)
+    s = scores.cpu().nan_to_num(nan=math.inf, posinf=3e38) + 0.0  # (NaN above +inf, -0 as 0)
+    s = torch.where(scores.cpu().isnan(), torch.full_like(s, math.inf), s)
+    old = n - recent
+    best = torch.sort(s[..., :old], dim=-1, descending=True, stable=True).indices[..., :keep - recent]
+    want = torch.cat([torch.sort(best, dim=-1).values, torch.arange(old, n).expand(1, 2, recent)], -1)
+    assert torch.equal(index.cpu().long(), want)
+    assert torch.equal(s2.cpu().view(torch.int32), scores.cpu().gather(-1, want).view(torch.int32))
+
+
+def test_evict_other_types():
+    announce("evict types")
+    scores = _scores(2, 2, 50, "weights")
+    caches = [torch.randn(2, 2, 50, 16, device="cuda").to(torch.float8_e4m3fn), torch.rand(2, 2, 50, device="cuda") > 0.5,
+              torch.randn(2, 2, 50, 3, device="cuda", dtype=torch.complex64)]
+    got, _, index, _ = fused_attn.evict_kv(scores, caches, 20)
+    for g, c in zip(got, caches):
+        at = index.long()
+        for i in range(2):
+            for j in range(2):
+                assert torch.equal(g[i, j].view(torch.uint8), c[i, j].view(torch.uint8)[at[i, j]])
 
 
 @pytest.mark.parametrize("kind", ["weights", "ties", "equal", "any"])

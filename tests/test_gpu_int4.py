@@ -127,6 +127,41 @@ def test_attention(dtype, d, nk, hq, hkv, nq, causal):
         check(got, *want, q, k, v, (ks, vs), got_lse=lse)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("nq", [1, 6, 30])  # 4, 24 and 120 rows
+@pytest.mark.parametrize("split", [64, 128, 1024])  # 40, 20 and 3 partitions: the merges of many and of few
+def test_attention_many_partitions(d, nq, split):
+    announce(f"int4 partitions d={d} nq={nq} split={split}")
+    lens = [2500, 1300, 0]
+    q = torch.randn(3, 8, nq, d, device="cuda", generator=gen(1)).half()
+    (k4, ks), (v4, vs) = cache(3, 2, 2500, d, 1), cache(3, 2, 2500, d, 2)
+    k, v = oracle.values(k4, ks), oracle.values(v4, vs)
+    for sl in (None, torch.tensor(lens, dtype=torch.int32, device="cuda")):
+        want = oracle.attention(q, k, v, True, lens=None if sl is None else lens)
+        got, lse = fused_attn.attention_int4(q, k4, ks, v4, vs, causal=True, seqlens_k=sl, split_len=split, return_lse=True)
+        check(got, *want, q, k, v, (ks, vs), got_lse=lse)
+
+
+def test_attention_of_infinite_and_nan_keys():
+    """A score of -inf (finite operands whose product is not) weighs nothing; a NaN key makes the rows that see it NaN."""
+    announce("int4 infinite scores")
+    q = torch.full((1, 2, 2, 64), 3e38, device="cuda").bfloat16()
+    k = torch.randn(1, 1, 70, 64, device="cuda", generator=gen(1)) * 1e-38
+    k[0, 0, 5], k[0, 0, 40] = -6e4, -6e4
+    k4, ks = fused_attn.quantize_kv_int4(k)
+    v4, vs = cache(1, 1, 70, 64, 2)
+    got = fused_attn.attention_int4(q, k4, ks, v4, vs, scale=1e-3)
+    keep = [j for j in range(70) if j not in (5, 40)]
+    want = fused_attn.attention_int4(q, k4[:, :, keep], ks[:, :, keep], v4[:, :, keep], vs[:, :, keep], scale=1e-3)
+    assert torch.isfinite(got).all() and (got.float() - want.float()).abs().max() < 0.05
+    ks = ks.clone()
+    ks[0, 0, 69] = math.nan
+    got = fused_attn.attention_int4(q.clamp(max=1.0), k4, ks, v4, vs)
+    assert torch.isnan(got).all()
+    got = fused_attn.attention_int4(q.clamp(max=1.0), k4, ks, v4, vs, seqlens_k=torch.tensor([69], device="cuda").int())
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("lens", [[0, 1, 700, 64], [-5, 9999, 33, 2]])
 @pytest.mark.parametrize("nq,causal", [(1, True), (4, True), (4, False), (20, True)])
 def test_attention_lengths(lens, nq, causal):
@@ -222,6 +257,18 @@ def test_paged(dtype, d, page, nq):
     again = fused_attn.attention_paged(q, turned[0], turned[1], bt, sl, causal=True, max_seqlen_k=500, k_scale=turned[2],
                                        v_scale=turned[3], split_len=64)
     assert torch.equal(again, got)
+
+
+def test_paged_without_keys_and_with_a_short_maximum():
+    announce("int4 paged empty")
+    q = torch.randn(2, 4, 1, 64, device="cuda").half()
+    (k4, ks), (v4, vs) = cache(2, 2, 64, 64, 1), cache(2, 2, 64, 64, 2)
+    kp, vp, ksp, vsp, bt, sl = fused_attn.paged_from_dense_int4(k4, ks, v4, vs, 16, generator=torch.Generator().manual_seed(1))
+    got, lse = fused_attn.attention_paged(q, kp, vp, bt, torch.zeros_like(sl), k_scale=ksp, v_scale=vsp, return_lse=True)
+    assert (got == 0).all() and torch.isneginf(lse).all()
+    got = fused_attn.attention_paged(q, kp, vp, bt, sl, max_seqlen_k=40, k_scale=ksp, v_scale=vsp)  # read as 40
+    want = fused_attn.attention_int4(q, k4[:, :, :40], ks[:, :, :40], v4[:, :, :40], vs[:, :, :40])
+    assert (got.float() - want.float()).abs().max() < 1e-3
 
 
 def test_paged_pages_outside_the_pool_are_zero_keys():
