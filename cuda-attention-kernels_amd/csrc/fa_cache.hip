@@ -7,8 +7,11 @@
 //
 // Decomposition.  Keys are cut into partitions of split_len; a workgroup of four waves takes one partition of one
 // (batch, kv-head) for up to 16 * RT rows, its waves every fourth 32-key tile each; the waves' (m, l, O) are merged
-// through LDS into one fp32 partial, and cache_finish_kernel or splitk_combine_kernel merges the partitions.  Bound by the bytes of the
-// cache: D + 8 a key at 4 bits, 4 D at 16.
+// through LDS into one fp32 partial, and cache_finish_kernel or splitk_combine_kernel merges the partitions.  Bound by
+// the bytes of the cache (D + 8 a key at 4 bits, 4 D at 16) up to 16 rows of D=128: bf16, 32 x 8 heads x 32768 keys
+// (1.14 GB) 177 us = 6.4 TB/s.  Bound by the vector unit beyond that (codes, exponentials: 8 x 8 heads x 64 rows of
+// D=256, 20000 keys, 342 MB and 84 GFLOP: 146 us) and at D=64, where a key's few bytes need the same exponentials (48 x
+// 8 heads of ragged lengths to 8000, 103 MB: 47 us).
 //
 // No K or V goes through LDS: with v_mfma_f32_16x16x32 every operand is a lane's own load.
 //   S^T = K Q^T      A: lane (r = l % 16, g = l / 16) holds 8 channels of one key as it lies in memory.  The channels'
@@ -30,23 +33,14 @@
 // rounding is 2^-11, P' is the sum of two bf16 terms and takes two products.  Everything else is fp32.
 //
 // Scores.  p needs the row's final sum, which no partition has.  The s of a row and key are written as they are
-// (4 bytes: 6% of a 16-bit key's bytes at D=128 and four rows, 12% of a 4-bit one's), and cache_finish_kernel turns them into
-// weights once the partitions' sums are there.  They lie tile by tile, the rows of 32 keys
-// together, so that a workgroup writes one run of memory.  A second pass over K would read half the cache again.
+// (4 bytes: 3% of a 16-bit key's bytes at D=128 and four rows, 12% of a 4-bit one's), and cache_finish_kernel turns them
+// into weights once the partitions' sums are there.  They lie tile by tile, the rows of 32 keys together, so that a
+// workgroup writes one run of memory.  A second pass over K would read half the cache again.
 #include <algorithm>
 
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
 
-#ifndef AHEADV
-#define AHEADV 1
-#endif
-#ifndef NTV
-#define NTV (RT == 1 ? 2 : 0)
-#endif
-#ifndef WPE
-#define WPE __attribute__((amdgpu_waves_per_eu(RT == 4 ? (I4 && D == 64 ? 2 : 1) : RT == 2 ? (D == 256 && !I4 ? 1 : 2) : D == 256 ? 1 : 3)))
-#endif
 namespace fa {
 
 namespace {
@@ -94,7 +88,7 @@ struct Codes {
 __device__ __forceinline__ uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// W words (W = 0: one 16-bit half) of a buffer, or of memory; read once: non-temporal
+// W words (W = 0: one 16-bit half) of a buffer (AUX: its cache policy), or of memory
 template <int W, int AUX>
 __device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, uint32_t* out) {
   if constexpr (W == 0) {
@@ -132,8 +126,19 @@ __device__ __forceinline__ void memory_words(const uint8_t* p, uint32_t* out) {
   }
 }
 
+// Waves a SIMD, which bound the registers: as many as fit without spilling.  One row block of D <= 128 holds three (32
+// x 8 heads x 32768 keys: 177 us, with two 188); more rows hold O in more registers.  D = 256 with 32 rows spills some
+// at two waves, and is faster so than with one (148 and 178 us).
+template <int D, bool I4, int RT>
+constexpr int waves_per_simd() {
+  if (RT == 4) return I4 && D == 64 ? 2 : 1;
+  if (RT == 2) return D == 256 && !I4 ? 1 : 2;
+  return D == 256 ? 1 : 3;
+}
+
 template <int D, class E, bool I4, bool PAGED, bool SCORES, int RT>
-__global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const CacheArgs a) {
+__global__ void __launch_bounds__(kCacheWaves * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd<D, I4, RT>())))
+attn_cache_kernel(const CacheArgs a) {
   static_assert(!PAGED || I4, "16-bit pools have kernels of their own");
   constexpr int ROW_BYTES = I4 ? D / 2 : 2 * D;
   constexpr int KS = D / 32;                      // k-steps of S^T
@@ -144,7 +149,9 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   // Q's operands in LDS where two waves then fit a SIMD (8 x 8 heads x 64 rows, 20000 keys: D=256 178 us with one wave,
   // 146 so; D=64 77 and 75; at D=128 64 rows spill: 67 and 79)
   constexpr bool QLDS = I4 && ((RT == 4 && D == 64) || (D == 256 && RT == 2));
-  constexpr int AHEAD = AHEADV;                   // 4 bits: tiles in flight
+  // A cache row that one row block reads is read once: non-temporal (32 x 8 heads x 32768 keys: 183 us, cached 203).
+  // Where several row blocks share it, the later ones find it in L2 (8 heads x 128 rows, 8191 keys: 24 us cached, 29 not).
+  constexpr int AUX = RT == 1 ? 2 : 0;
   constexpr float NEG_INF = -__builtin_inff();
   using PV = typename std::conditional<I4, BF16, E>::type;  // element type of the second product
   // 4 bits, bf16: Q is taken 2^10 smaller (exact down to 2^-116) and the scores' multiplier larger, so that sum(q) and the
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       const int at = kkey * row + kpart;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        load_k_row([&](auto w, int off, uint32_t* out) { buffer_words<decltype(w)::value, NTV>(r, at + 4 * u * row + off, out); },
+        load_k_row([&](auto w, int off, uint32_t* out) { buffer_words<decltype(w)::value, AUX>(r, at + 4 * u * row + off, out); },
                    t.k[u]);
     };
     if (packed) rows(ROW_BYTES); else rows((int)krow);
@@ -265,7 +272,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
     auto rows = [&](int row) __attribute__((always_inline)) {
       const int at = 8 * g * row + vpart;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) buffer_words<VW, NTV>(r, at + i * row, t.v[i]);
+      for (int i = 0; i < 8; ++i) buffer_words<VW, AUX>(r, at + i * row, t.v[i]);
     };
     if (packed) rows(ROW_BYTES); else rows((int)vrow);
   };
@@ -352,11 +359,8 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   int n0 = klo + (STAGED ? wave * share : wave) * kTile;
   const int last = klo + ((STAGED ? min((wave + 1) * share, n_tiles) : n_tiles) - 1) * kTile;  // the last tile's first key
   constexpr bool REFILL = !I4 || QLDS;  // one tile's registers, refilled as they are read
-  Tile tiles[REFILL ? 1 : AHEAD + 1];
-#pragma unroll
-  for (int i = 0; i < (REFILL ? 1 : AHEAD); ++i) {
-    if (n0 + i * STEP <= last) load_tile(n0 + i * STEP, tiles[i]);
-  }
+  Tile tiles[REFILL ? 1 : 2];
+  if (n0 <= last) load_tile(n0, tiles[0]);
 
   // ---- Q: B operands, and the sum of each row -------------------------------------------------------------
   u32x4 qf[QLDS ? 1 : RT][QLDS ? 1 : KS];
@@ -569,8 +573,8 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       }
     }
   };
-  // Staged: 33 MB of scores beside 1 GB of keys cost 60 us of 219 when every tile wrote its 512 bytes, 50
-  // so (what is left is the memory's turning between reads and writes: writes that stay in the L2 cost 10).
+  // Staged: 33 MB of scores beside 1 GB of keys cost 60 us of 219 when every tile wrote its 512 bytes, 50 so (what is
+  // left is the memory's turning between reads and writes: writes that stay in the L2 cost 10).
   // Direct: rows past R are beyond the descriptor's limit and dropped, without a branch around the stores (loads and
   // stores share one counter: a wait after stores that may have been skipped waits for too much).
   const int stage_tiles = STAGED ? kStageFloats / (R * kTile) : 1;
@@ -616,10 +620,11 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
   };
 
   if constexpr (!REFILL) {
-    // AHEAD tiles are in flight while one is worked on (a ring of registers: the loop is unrolled by its size)
+    // The next tile is in flight while one is worked on (two or three ahead, or two tiles a step at D = 64, gain nothing
+    // or spill).
     auto step = [&](Tile& cur, Tile& next) __attribute__((always_inline)) {
       store_pair(cur.pair);
-      if (n0 + AHEAD * STEP <= last) load_tile(n0 + AHEAD * STEP, next);
+      if (n0 + STEP <= last) load_tile(n0 + STEP, next);
       f32x4 acc[RT][2];
       product_k(cur, acc);
       product_v(cur, acc, n0);
@@ -627,11 +632,9 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
       n0 += STEP;
     };
     while (n0 <= last) {
-#pragma unroll
-      for (int i = 0; i <= AHEAD; ++i) {
-        if (i > 0 && n0 > last) break;
-        step(tiles[i], tiles[(i + AHEAD) % (AHEAD + 1)]);
-      }
+      step(tiles[0], tiles[1]);
+      if (n0 > last) break;
+      step(tiles[1], tiles[0]);
     }
   } else {
     // K's registers are refilled once its product has read them, V's likewise
@@ -724,7 +727,7 @@ __global__ void __launch_bounds__(kCacheWaves * 64) WPE attn_cache_kernel(const 
 // What follows the partitions' partials: blocks below a.merge_blocks merge a row's partials into its output, the others
 // turn scores into weights.  Both start from the partitions' (max, sum), so neither waits for the other: one launch.
 // For up to kMergeSplits partitions (more: splitk_combine_kernel, which spreads a row's partials over a workgroup, and
-// then this kernel with the log-sum-exps that it wrote).
+// then this kernel with the log-sum-exps that it wrote: 5 us more in all for 32 x 8 heads x 8 rows that score 8191 keys).
 constexpr int kMergeSplits = 16;
 constexpr int kFinishRows = 512;  // rows whose log-sum-exps a block holds at a time
 
@@ -776,7 +779,9 @@ __device__ __forceinline__ void merge_rows(const FinishArgs& a) {
 }
 
 // score_j = before_j + sum over the rows of 2^(s_rj - lse2_r), for the keys that a row sees.  Four keys a lane; NW waves
-// share 256 keys and take every NW-th row each (their sums are added in order), and a block has 4 / NW such sets.
+// share 256 keys and take every NW-th row each (their sums are added in order), and a block has 4 / NW such sets.  16
+// waves from 64 rows on (8 heads x 128 rows, 8191 keys: 12 us, one wave 34), else one (16 x 8 heads x 4 rows, 16384
+// keys: 12 us, sixteen 116).
 template <int NW>
 __device__ __forceinline__ void finish_scores(const FinishArgs& a) {
   constexpr int THREADS = NW <= 4 ? 256 : NW * 64, SETS = THREADS / 64 / NW;

@@ -9,7 +9,9 @@
 //     digits found so far.  Integer counts in LDS: the result does not depend on the order of the additions.  A last
 //     pass writes the indices in order (the candidates above the threshold and the first of those equal to it).
 //   * gather_rows_kernel: the scores and the rows of up to eight tensors in one launch; a thread copies units of the widest
-//     power of two (16 bytes at most) that a tensor's rows, strides and addresses allow.  HBM-bound.
+//     power of two (16 bytes at most) that a tensor's rows, strides and addresses allow.  HBM-bound: 16 x 8 heads, 4096
+//     of 8192 keys with 4-bit rows of D=128, 45 us; 8 heads, 16384 of 65536 with bf16 rows of D=128, 31 us (134 MB: 4.3
+//     TB/s).  Kept 64-byte rows lie scattered, so most 128-byte lines are read for half of what they hold.
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
 
@@ -44,9 +46,11 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 }
 
 // A thread holds the keys of four candidates of each of CH chunks of 4096 in registers, all loads in flight; up to
-// CH * 4096 candidates are read once, more again in every pass (16 chunks do not fit the 128 registers of 1024 threads:
-// 65536 keys took 58 us with spills and 44 as two spans of 8).  Digits of 11, 11 and 10 bits: the first already tells
-// a quarter of an octave apart; the candidates that share it are gathered in LDS if they fit, and the others count those.
+// CH * 4096 candidates are read once, more again in every pass.  Two chunks where they hold every key (16 x 8 heads x
+// 8192 keys: 12 us, with eight 23), else eight (8 heads x 65536 keys: 47 us; two chunks 53, sixteen do not fit the 128
+// registers of 1024 threads and spill, 58).  Digits of 11, 11 and 10 bits: the first already tells a quarter of an octave
+// apart; the candidates that share it are gathered in LDS if they fit, and the others count those.  One workgroup a head:
+// bound by its own instructions and waits, not by memory.
 template <int CH>
 __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs a) {
   constexpr int CHUNK = kThreads * kItems, SPAN = CH * CHUNK;
@@ -123,7 +127,8 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
             if (who == 0) continue;
             uint32_t at = 0;
             if (lane == 0) at = atomicAdd(&found[2], (uint32_t)__popcll(who));
-            at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+            at = __builtin_amdgcn_readfirstlane(at) +
+                 __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
             if (in) list[at] = held[i][e];
           }
         }

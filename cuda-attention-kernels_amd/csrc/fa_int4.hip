@@ -13,7 +13,8 @@
 // keys) let rows be appended and picked one at a time.
 //
 // HBM-bound.  A lane holds 8 channels (16 bytes of 16-bit input, one 4-byte word of codes), so D/8 lanes hold a
-// row and its ends are a reduction over them; UNROLL rows a lane are loaded before any is worked on.
+// row and its ends are a reduction over them; UNROLL rows a lane are loaded before any is worked on.  16 x 8 x 32768 rows
+// of D=128 bf16 (1.36 GB): written in 250 us, read back in 235, 5.4 and 5.8 TB/s.
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
 
@@ -111,7 +112,8 @@ __device__ __forceinline__ uint32_t encode(const Chunk<T>& c, uint32_t& pair) {
 
 // Where the rows of a lane are.  A workgroup takes UNROLL * RPS rows, RPS a step: those of one (batch, head) from n0 on,
 // or where a head has fewer rows than half of that (FLAT: pages, single tokens) those of the flattened [B, H, N], at two
-// divisions a row.
+// divisions a row (2053 pages of 8 heads x 16 tokens, D=64: read in 9 us, 12 without; 16 x 8 x 32768 rows: written in
+// 311 us, 250 without).
 template <bool FLAT, int RPS, int UNROLL>
 struct RowPlace {
   int b[UNROLL], h[UNROLL], n[UNROLL];
