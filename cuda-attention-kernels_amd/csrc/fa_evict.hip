@@ -10,8 +10,8 @@
 //     pass writes the indices in order (the candidates above the threshold and the first of those equal to it).
 //   * gather_rows_kernel: the scores and the rows of up to eight tensors in one launch; a thread copies units of the widest
 //     power of two (16 bytes at most) that a tensor's rows, strides and addresses allow.  HBM-bound: 16 x 8 heads, 4096
-//     of 8192 keys with 4-bit rows of D=128, 45 us; 8 heads, 16384 of 65536 with bf16 rows of D=128, 31 us (134 MB: 4.3
-//     TB/s).  Kept 64-byte rows lie scattered, so most 128-byte lines are read for half of what they hold.
+//     of 8192 keys with 4-bit rows of D=128, 33 us (161 MB moved: 4.9 TB/s); 8 heads, 16384 of 65536 with bf16 rows of
+//     D=128, 27 us (139 MB: 5.1 TB/s).  A branch around each load, so that one waits for another: 45 and 31 us.
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
 
@@ -238,23 +238,24 @@ __device__ __forceinline__ void gather_units(const EvictTensor& t, const EvictAr
   const int32_t* index = a.index + (int64_t)bh * a.keep;
   const uint32_t units = (uint32_t)t.units, all = (uint32_t)a.keep * units;  // < 2^31 (host)
   const uint32_t u0 = (uint32_t)(blockIdx.x % (uint32_t)a.chunks) * (256 * STEP) + threadIdx.x;
-  U v[STEP];
-  char* to[STEP];
+  if (u0 - threadIdx.x >= all) return;  // (another tensor's rows have more units)
+  // No branch around the loads (units past the last are the last one's, and -1 reads row 0, which a tensor with rows to
+  // fill has), so all of a kind are in flight together.
+  uint32_t r[STEP], c[STEP];
+  int j[STEP];
 #pragma unroll
   for (int i = 0; i < STEP; ++i) {
-    const uint32_t u = u0 + 256 * i;
-    to[i] = nullptr;
-    if (u < all) {
-      const uint32_t r = t.shift >= 0 ? u >> t.shift : u / units, c = u - r * units;
-      const int j = index[r];
-      to[i] = dst + r * t.dn + c * sizeof(U);
-      v[i] = U{};
-      if (j >= 0) v[i] = *(const U*)(src + j * t.sn + c * sizeof(U));
-    }
+    const uint32_t u = min(u0 + 256 * i, all - 1);
+    r[i] = t.shift >= 0 ? u >> t.shift : u / units, c[i] = u - r[i] * units;
+    j[i] = index[r[i]];
   }
+  U v[STEP];
+#pragma unroll
+  for (int i = 0; i < STEP; ++i) v[i] = *(const U*)(src + max(j[i], 0) * t.sn + c[i] * sizeof(U));
 #pragma unroll
   for (int i = 0; i < STEP; ++i) {
-    if (to[i] != nullptr) *(U*)to[i] = v[i];
+    const U x = j[i] >= 0 ? v[i] : U{};
+    if (u0 + 256 * i < all) *(U*)(dst + r[i] * t.dn + c[i] * sizeof(U)) = x;
   }
 }
 
