@@ -473,7 +473,12 @@ fa_status fa_attention_cache(const fa_cache_params* p, int32_t split_len, void* 
   return FA_OK;
 }
 
-fa_status fa_evict_kv(const fa_evict_params* p, void* stream) {
+size_t fa_evict_kv_workspace_bytes(const fa_evict_params* p) {
+  if (p == nullptr || p->batch <= 0 || p->heads <= 0 || p->seqlen <= 0 || p->seqlen > (1 << 30)) return 0;
+  return fa::evict_workspace_bytes(*p);
+}
+
+fa_status fa_evict_kv(const fa_evict_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   g_last_error.clear();
   if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
   if (p->batch < 0 || p->heads < 0 || p->seqlen < 0 || p->seqlen > (1 << 30))
@@ -501,8 +506,15 @@ fa_status fa_evict_kv(const fa_evict_params* p, void* stream) {
       return fail(FA_ERR_INVALID_ARGUMENT, "negative stride");
     if (p->keep > 1 && t.dst_stride_n < t.row_bytes) return fail(FA_ERR_INVALID_ARGUMENT, "dst rows overlap");
   }
+  const size_t need = fa::evict_workspace_bytes(*p);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
+    char buf[128];
+    snprintf(buf, sizeof(buf), "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return fail(FA_ERR_WORKSPACE, buf);
+  }
+  if (!aligned(workspace, 16)) return fail(FA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   const char* err = nullptr;
-  const fa_status st = fa::run_evict(*p, reinterpret_cast<hipStream_t>(stream), &err);
+  const fa_status st = fa::run_evict(*p, workspace, reinterpret_cast<hipStream_t>(stream), &err);
   if (st != FA_OK) return fail(st, err ? err : "launch failed");
   return FA_OK;
 }

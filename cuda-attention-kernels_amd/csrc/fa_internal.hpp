@@ -148,6 +148,8 @@ struct EvictArgs {
   int32_t* index;
   int32_t* seqlens_out;
   int32_t h, nk, keep, recent, chunks;
+  int32_t groups, group_len;  // long caches: workgroups of a (sequence, kv-head), keys of each
+  uint32_t *counts, *list;    // and their workspace
   EvictTensor tensors[FA_MAX_EVICT_TENSORS + 1];  // the scores first
 };
 
@@ -191,7 +193,8 @@ fa_status run_int4_rows(const fa_int4_params& p, bool read, hipStream_t stream, 
 fa_status run_append_int4(const fa_int4_append_params& p, hipStream_t stream, const char** err);
 size_t cache_workspace_bytes(const fa_cache_params& p, int32_t split_len);
 fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace, hipStream_t stream, const char** err);
-fa_status run_evict(const fa_evict_params& p, hipStream_t stream, const char** err);
+size_t evict_workspace_bytes(const fa_evict_params& p);
+fa_status run_evict(const fa_evict_params& p, void* workspace, hipStream_t stream, const char** err);
 // kv: paged K/V (nullptr for a dense cache)
 fa_status run_splitk(const fa_fwd_params& p, int32_t split_len, void* workspace, hipStream_t stream,
                      const char** err, const fa_paged_kv* kv = nullptr);

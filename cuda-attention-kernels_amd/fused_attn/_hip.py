@@ -299,7 +299,9 @@ def _bind(lib: ctypes.CDLL) -> None:
         lib.fa_attention_cache.argtypes = [ctypes.POINTER(CacheParams), ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t,
                                            ctypes.c_void_p]
         lib.fa_attention_cache.restype = ctypes.c_int
-        lib.fa_evict_kv.argtypes = [ctypes.POINTER(EvictParams), ctypes.c_void_p]
+        lib.fa_evict_kv_workspace_bytes.argtypes = [ctypes.POINTER(EvictParams)]
+        lib.fa_evict_kv_workspace_bytes.restype = ctypes.c_size_t
+        lib.fa_evict_kv.argtypes = [ctypes.POINTER(EvictParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.fa_evict_kv.restype = ctypes.c_int
     lib.fa_device_supported.argtypes = [ctypes.c_int32]
     lib.fa_device_supported.restype = ctypes.c_int32
@@ -1239,5 +1241,7 @@ def evict_kv(scores, caches, keep: int, recent: int, seqlens_k, out):
         p.tensors[i] = EvictTensor(s.data_ptr(), d.data_ptr(), *(x * size for x in _strides3(s)),
                                    *(x * size for x in _strides3(d)), _row_elems(s) * size)
     with _on_device(dev):
-        _check(lib.fa_evict_kv(p, _stream(scores)), "evict_kv")
+        need = lib.fa_evict_kv_workspace_bytes(p)
+        workspace = torch.empty(need // 4, dtype=torch.float32, device=dev) if need else None
+        _check(lib.fa_evict_kv(p, workspace.data_ptr() if need else None, need, _stream(scores)), "evict_kv")
     return dst, kept, index, lens

@@ -323,7 +323,9 @@ typedef struct fa_evict_params {
   int32_t* seqlens_out; /* [batch] */
   fa_evict_tensor tensors[FA_MAX_EVICT_TENSORS];
 } fa_evict_params;
-fa_status fa_evict_kv(const fa_evict_params* p, void* stream);
+/* Bytes of workspace fa_evict_kv needs (16-byte aligned): 0 up to 8192 keys. */
+size_t fa_evict_kv_workspace_bytes(const fa_evict_params* p);
+fa_status fa_evict_kv(const fa_evict_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /* FA_ABI_VERSION of the loaded library. */
 int32_t fa_abi_version(void);

@@ -328,8 +328,23 @@ def test_evict_validation(lib, over, msg):
     p.batch, p.heads, p.seqlen, p.keep, p.recent = 1, 1, 8, 4, 0
     for k, v in over.items():
         setattr(p, k, v)
-    assert lib.fa_evict_kv(p, None) == _hip.FA_ERR_INVALID_ARGUMENT
+    assert lib.fa_evict_kv(p, None, 0, None) == _hip.FA_ERR_INVALID_ARGUMENT
     assert msg in lib.fa_last_error().decode()
+
+
+def test_evict_workspace(lib):
+    p = _hip.EvictParams()
+    p.scores = p.index = p.scores_out = p.seqlens_out = 0x10000
+    p.batch, p.heads, p.seqlen, p.keep, p.recent = 2, 3, 8192, 4, 0
+    assert lib.fa_evict_kv_workspace_bytes(p) == 0
+    for n, groups in ((8193, 2), (65536, 8), (16 * 8192, 16), (16 * 8192 + 1, 9), (33 * 8192, 11)):
+        p.seqlen = n  # the counts of 2048 digits a workgroup, and a list of every key
+        need = lib.fa_evict_kv_workspace_bytes(p)
+        assert need == 6 * (groups * 2048 + n) * 4
+        for ws, got in ((0x10000, need - 1), (None, need), (0x10008, need)):
+            assert lib.fa_evict_kv(p, ws, got, None) == _hip.FA_ERR_WORKSPACE
+    assert lib.fa_evict_kv(None, None, 0, None) == _hip.FA_ERR_INVALID_ARGUMENT
+    assert lib.fa_evict_kv_workspace_bytes(None) == 0
 
 
 @pytest.mark.parametrize("over,code,msg", [

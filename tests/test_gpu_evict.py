@@ -146,6 +146,24 @@ def test_evict_many_keys(kind, n, keep, recent):
     assert torch.equal(s2.cpu().view(torch.int32), scores.cpu().gather(-1, want).view(torch.int32))
 
 
+@pytest.mark.parametrize("lens", [[20000, 8191, 8193, 0, 16384], [16385, 20001, 101, 100, 99]])
+@pytest.mark.parametrize("kind", ["weights", "equal"])
+def test_evict_many_keys_of_other_lengths(kind, lens):
+    """Sequences whose candidates end in an early workgroup's range, beside ones that all stay."""
+    announce(f"evict many lengths {kind} {lens}")
+    b, n, keep, recent = len(lens), 20001, 100, 9
+    scores = _scores(b, 2, n, kind, 3)
+    k = torch.randn(b, 2, n, 64, device="cuda", generator=gen(4)).half()
+    (k2,), s2, index, left = fused_attn.evict_kv(scores, (k,), keep, recent, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    assert left.tolist() == [min(x, keep) for x in lens]
+    for i in range(b):
+        for j in range(2):
+            at = oracle.kept(scores[i, j].cpu().numpy(), lens[i], keep, recent)
+            assert index[i, j].tolist() == at + [-1] * (keep - len(at))
+            assert torch.equal(k2[i, j, :len(at)], k[i, j, at]) and not k2[i, j, len(at):].any()
+            assert torch.equal(s2[i, j, :len(at)], scores[i, j, at]) and not s2[i, j, len(at):].any()
+
+
 def test_evict_other_types():
     announce("evict types")
     scores = _scores(2, 2, 50, "weights")
@@ -260,6 +278,32 @@ def test_score_and_evict_together(int4):
     at = index.long()[..., None].expand(b, hkv, keep, d)
     k2, v2 = kv.gather(2, at), vv.gather(2, at)
     check(got, *oracle.attention(q, k2, v2, True), q, k2, v2, pairs)
+
+
+def test_evict_many_keys_in_a_graph_and_twice_at_once():
+    announce("evict many graph")
+    n, keep = 30000, 7000
+    scores = [_scores(1, 2, n, "weights", i) for i in range(2)]
+    want = [fused_attn.evict_kv(s, [], keep, 100)[2] for s in scores]
+    graphs, got = [], []
+    for s in scores:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(fused_attn.evict_kv(s, [], keep, 100)[2])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in scores]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for x in got:
+            x.zero_()
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, w in zip(got, want):
+            assert torch.equal(x, w)
+        torch.ones(1000, device="cuda").sum().item()
 
 
 def test_scored_and_evict_in_a_graph():
