@@ -73,9 +73,9 @@ __device__ __forceinline__ void row_ends(float& lo, float& hi) {
   if constexpr (LPR >= 32) lo = vmin(lo, __shfl_xor(lo, 16)), hi = vmax(hi, __shfl_xor(hi, 16));
 }
 
-// x / scale for a finite x and a positive scale, correctly rounded wherever the quotient is normal: the product
-// with y = RN(1 / scale) and one residual step (Markstein).  A quotient too small to be normal rounds to code 0
-// either way.
+// x / scale for 0 <= x <= 16 scale and a positive scale, correctly rounded wherever the quotient is normal: the product
+// with y = RN(1 / scale) and one residual step (Markstein).  A quotient too small to be normal rounds to code 0 either
+// way.  (A larger x could overflow the product, and the residual step make a NaN of it.)
 __device__ __forceinline__ float div_scale(float x, float scale, float y) {
   const float q = x * y;
   return __builtin_fmaf(__builtin_fmaf(-q, scale, x), y, q);
@@ -91,7 +91,6 @@ __device__ __forceinline__ uint32_t encode(const Chunk<T>& c, uint32_t& pair) {
 #pragma unroll
   for (int e = 1; e < 8; ++e) lo = vmin(lo, x[e]), hi = vmax(hi, x[e]);
   row_ends<LPR>(lo, hi);
-  const bool finite = lo > -__builtin_inff() && hi < __builtin_inff();  // the whole row: its ends are
   lo = vmin(vmax(lo, -kF16Max), kF16Max);
   hi = vmin(vmax(hi, -kF16Max), kF16Max);
   const f16x2 sz = {(_Float16)rounded((hi - lo) * (1.0f / 15.0f)), (_Float16)lo};
@@ -102,9 +101,9 @@ __device__ __forceinline__ uint32_t encode(const Chunk<T>& c, uint32_t& pair) {
     const float y = __fdiv_rn(1.0f, scale);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = x[e] - zero;
-      const float q = finite ? div_scale(d, scale, y) : __fdiv_rn(d, scale);
-      codes |= (uint32_t)__builtin_amdgcn_fmed3f(__builtin_rintf(q), 0.f, 15.f) << (4 * e);
+      // held to where the code already is 0 or 15, infinities among them (16 scale is exact)
+      const float d = __builtin_amdgcn_fmed3f(x[e] - zero, 0.f, 16.f * scale);
+      codes |= (uint32_t)fminf(__builtin_rintf(div_scale(d, scale, y)), 15.f) << (4 * e);
     }
   }
   return codes;

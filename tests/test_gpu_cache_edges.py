@@ -99,3 +99,35 @@ def test_calls_repeat_bit_for_bit():
                 call(q[1])
                 again = call(q[0])
                 assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_writer_with_one_channel_far_beyond_the_others(dtype, d):
+    """Finite values whose quotient by the row's scale leaves fp32: their code is 15 (or 0), as for any value past the ends."""
+    announce(f"int4 far values {dtype} d={d}")
+    x = torch.randn(1, 1, 12, d, device="cuda", generator=gen(1)) * 0.001
+    x[0, 0, 0] = 65503.0
+    x[0, 0, 0, 5] = 3e38
+    x[0, 0, 1] = 65504.0  # (no room above: the scale is 0)
+    x[0, 0, 1, 5] = 3e38
+    x[0, 0, 2] = 65000.0
+    x[0, 0, 2, 1::2] = 1e37
+    x[0, 0, 3] = 65503.99
+    x[0, 0, 3, 0] = 3.3e38
+    x[0, 0, 4] = -65503.0
+    x[0, 0, 4, 5] = -3e38
+    x[0, 0, 5, 5], x[0, 0, 5, 6] = 3e38, -3e38
+    x[0, 0, 6, 5] = 3e38
+    x[0, 0, 7, 5] = -3e38
+    x[0, 0, 8] = 65503.0
+    x[0, 0, 8, 5] = math.inf
+    x[0, 0, 9] = -65504.0
+    x[0, 0, 9, 5] = -65503.0
+    x[0, 0, 9, 6] = -math.inf
+    x = x.to(dtype)
+    _exactly(*fused_attn.quantize_kv_int4(x), x)
+    pool = [torch.zeros(1, 1, 12, w, dtype=t, device="cuda") for w, t in ((d // 2, torch.uint8), (2, torch.float16))]
+    twin = [t.clone() for t in pool]
+    fused_attn.append_kv_int4(x, x, *pool, *twin, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    _exactly(*pool, x), _exactly(*twin, x)
