@@ -1138,9 +1138,9 @@ def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split
             new = torch.zeros((b, hkv, nk), dtype=torch.float32, device=q.device) if scores is None else scores.clone()
         else:
             new = torch.empty((b, hkv, nk), dtype=torch.float32, device=q.device)
-        p.scores_out, p.scores_out_stride_b, p.scores_out_stride_h = new.data_ptr(), new.stride(0), new.stride(1)
-        if nk == 0:
-            p.scores_out = o.data_ptr()  # nothing is written: there are no keys
+        # a tensor without scores has no address; the library only looks whether it is asked for them, and writes none
+        p.scores_out = new.data_ptr() if new.numel() else 16
+        p.scores_out_stride_b, p.scores_out_stride_h = new.stride(0), new.stride(1)
         if scores is not None:
             p.scores_in, p.scores_in_stride_b, p.scores_in_stride_h = scores.data_ptr(), scores.stride(0), scores.stride(1)
     need = lib.fa_attention_cache_workspace_bytes(p, split_len)

@@ -131,3 +131,20 @@ def test_writer_with_one_channel_far_beyond_the_others(dtype, d):
     twin = [t.clone() for t in pool]
     fused_attn.append_kv_int4(x, x, *pool, *twin, torch.zeros(1, dtype=torch.int32, device="cuda"))
     _exactly(*pool, x), _exactly(*twin, x)
+
+
+@pytest.mark.parametrize("int4", [False, True])
+def test_scored_of_an_empty_batch(int4):
+    announce(f"scored empty batch int4={int4}")
+    q = torch.zeros(0, 4, 1, 64, device="cuda").half()
+    if int4:
+        k, extra = torch.zeros(0, 2, 9, 32, dtype=torch.uint8, device="cuda"), torch.zeros(0, 2, 9, 2, device="cuda").half()
+        extra = dict(k_scale=extra, v_scale=extra)
+    else:
+        k, extra = torch.zeros(0, 2, 9, 64, device="cuda").half(), {}
+    o, w = fused_attn.attention_scored(q, k, k, **extra)
+    assert o.shape == q.shape and w.shape == (0, 2, 9) and w.dtype == torch.float32
+    # no queries and no keys
+    o, w = fused_attn.attention_scored(torch.zeros(2, 4, 0, 64, device="cuda").half(), torch.zeros(2, 2, 0, 64, device="cuda").half(),
+                                       torch.zeros(2, 2, 0, 64, device="cuda").half())
+    assert o.shape == (2, 4, 0, 64) and w.shape == (2, 2, 0)
