@@ -1100,6 +1100,10 @@ def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split
     _require_gpu(q, k, v, *more)
     (b, hq, nq, d), hkv = q.shape, k.shape[1]
     nk = k.shape[2] if block_table is None else int(max_seqlen_k)
+    if block_table is not None:
+        check_block_table(block_table, b)
+        if nk > block_table.shape[1] * k.shape[2]:  # (a table without columns has no address that the library could see)
+            raise RuntimeError(f"block_table {tuple(block_table.shape)} has fewer pages per sequence than max_seqlen_k {nk} needs")
     if seqlens_k is not None:
         check_lengths(seqlens_k, b)
         seqlens_k = seqlens_k.contiguous()
@@ -1125,7 +1129,6 @@ def cache_attention(q, k, v, k_scale, v_scale, causal: bool, scale: float, split
                     *_strides3(o), b, hq, hkv, nq, nk, d, float(scale), int(bool(causal)), _DTYPE_CODE[q.dtype],
                     INT4 if int4 else _DTYPE_CODE[k.dtype], *pairs, None if seqlens_k is None else seqlens_k.data_ptr())
     if block_table is not None:
-        check_block_table(block_table, b)
         block_table = _plain_table(block_table)
         p.block_table, p.block_table_stride = block_table.data_ptr(), block_table.stride(0)
         p.block_table_cols, p.page_size, p.num_pages = block_table.shape[1], k.shape[2], k.shape[0]

@@ -26,3 +26,12 @@ def test_scored_calls_without_queries(host_only, int4, b, nq, nk):
     assert o.shape == q.shape and w.shape == (b, 2, nk) and not w.any()
     with pytest.raises(RuntimeError, match="split_len"):
         _hip.cache_attention(q, k, k, pairs, pairs, True, 0.1, 65, return_scores=True)
+
+
+@pytest.mark.parametrize("cols,nk", [(0, 1), (0, 640), (3, 49)])
+def test_paged_calls_need_their_pages(host_only, cols, nk):
+    """A table without columns has no address: the call must not become one over a dense cache."""
+    q, pool, pairs = torch.zeros(2, 4, 1, 64).half(), torch.zeros(5, 2, 16, 32, dtype=torch.uint8), torch.zeros(5, 2, 16, 2).half()
+    table, lens = torch.zeros(2, cols, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="fewer pages"):
+        _hip.cache_attention(q, pool, pool, pairs, pairs, True, 0.1, None, seqlens_k=lens, block_table=table, max_seqlen_k=nk)
