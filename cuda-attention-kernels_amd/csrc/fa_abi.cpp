@@ -191,6 +191,7 @@ fa_status validate_cache(const fa_cache_params* p, int32_t split_len) {
     if (p->k_stride_b < 0 || p->v_stride_b < 0) return fail(FA_ERR_INVALID_ARGUMENT, "negative page stride");
     if (!aligned(p->block_table, 4)) return fail(FA_ERR_INVALID_ARGUMENT, "block_table must be 4-byte aligned");
   }
+  if (const char* why = fa::cache_refusal(*p, split_len)) return fail(FA_ERR_UNSUPPORTED, why);
   return FA_OK;
 }
 

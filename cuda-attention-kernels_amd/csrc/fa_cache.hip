@@ -937,7 +937,28 @@ int splits(const fa_cache_params& p, int split_len) {
   return p.seqlen_k > 0 ? (p.seqlen_k + split_len - 1) / split_len : 1;
 }
 
+// Row blocks of 16 that a workgroup takes together.
+int row_tiles(const fa_cache_params& p) {
+  const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
+  return rows <= 16 ? 1 : rows <= 32 || p.head_dim == 256 ? 2 : 4;
+}
+
+// Workgroups of attn_cache_kernel.
+int64_t workgroups(const fa_cache_params& p, int n_split) {
+  const int64_t items = (int64_t)p.batch * p.heads_kv * n_split, rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
+  const int block = 16 * row_tiles(p);
+  return (p.seqlens_k != nullptr ? (items + 7) / 8 * 8 : items) * ((rows + block - 1) / block);
+}
+
 }  // namespace
+
+const char* cache_refusal(const fa_cache_params& p, int32_t split_len) {
+  if (p.block_table != nullptr && ((int64_t)split_len - 1) / p.page_size + 2 > kMaxSlots)
+    return "split_len too long for the page size: a partition may span at most 258 pages";
+  if ((int64_t)p.batch * p.heads_q * p.seqlen_q > INT32_MAX || workgroups(p, splits(p, split_len)) > INT32_MAX)
+    return "grid too large";
+  return nullptr;
+}
 
 size_t cache_workspace_bytes(const fa_cache_params& p, int32_t split_len) {
   size_t need = align16(fa_splitk_workspace_bytes(p.batch, p.heads_q, p.seqlen_q, p.head_dim, splits(p, split_len)));
@@ -970,19 +991,11 @@ fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace
     while ((int64_t{1} << lg) < (int64_t)p.page_size) ++lg;
     a.page_magic_shift = 31 + lg;
     a.page_magic = (uint32_t)(((uint64_t{1} << a.page_magic_shift) + (uint64_t)p.page_size - 1) / (uint64_t)p.page_size);
-    if (((int64_t)split_len - 1) / p.page_size + 2 > kMaxSlots) {
-      *err = "split_len too long for the page size: a partition may span at most 258 pages";
-      return FA_ERR_UNSUPPORTED;
-    }
   }
-  const int rows = a.group * p.seqlen_q, rt = rows <= 16 ? 1 : rows <= 32 || p.head_dim == 256 ? 2 : 4;
+  const int rows = a.group * p.seqlen_q, rt = row_tiles(p);
   a.n_rowblk = (rows + 16 * rt - 1) / (16 * rt);
   const int64_t items = (int64_t)p.batch * p.heads_kv * S, out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
-  const int64_t total = (p.seqlens_k != nullptr ? (items + 7) / 8 * 8 : items) * a.n_rowblk;
-  if (total > INT32_MAX || out_rows > INT32_MAX) {
-    *err = "grid too large";
-    return FA_ERR_UNSUPPORTED;
-  }
+  const int64_t total = workgroups(p, S);
   a.total = (int32_t)total;
   a.n_items = (int32_t)items;
   uint8_t* ws = (uint8_t*)workspace;

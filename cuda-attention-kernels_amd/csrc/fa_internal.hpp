@@ -191,6 +191,8 @@ fa_status run_combine(const CombineArgs& c, int d, bool bf16, int64_t rows, hipS
 // read: floats from codes; else codes from floats
 fa_status run_int4_rows(const fa_int4_params& p, bool read, hipStream_t stream, const char** err);
 fa_status run_append_int4(const fa_int4_append_params& p, hipStream_t stream, const char** err);
+// Why a call of valid parameters cannot be launched, or NULL.
+const char* cache_refusal(const fa_cache_params& p, int32_t split_len);
 size_t cache_workspace_bytes(const fa_cache_params& p, int32_t split_len);
 fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace, hipStream_t stream, const char** err);
 size_t evict_workspace_bytes(const fa_evict_params& p);

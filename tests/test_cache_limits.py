@@ -35,3 +35,42 @@ def test_paged_calls_need_their_pages(host_only, cols, nk):
     table, lens = torch.zeros(2, cols, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="fewer pages"):
         _hip.cache_attention(q, pool, pool, pairs, pairs, True, 0.1, None, seqlens_k=lens, block_table=table, max_seqlen_k=nk)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _hip.load_library()
+
+
+def _params(**over):
+    p = _hip.CacheParams()
+    p.q = p.k = p.v = p.o = p.k_scale = p.v_scale = 0x10000  # never dereferenced
+    p.batch, p.heads_q, p.heads_kv, p.seqlen_q, p.seqlen_k, p.head_dim = 1, 4, 2, 1, 64, 64
+    p.q_stride_b, p.q_stride_h, p.q_stride_n = 256, 64, 64
+    p.o_stride_b, p.o_stride_h, p.o_stride_n = 256, 64, 64
+    p.k_stride_b, p.k_stride_h, p.k_stride_n = 4096, 2048, 32
+    p.v_stride_b, p.v_stride_h, p.v_stride_n = 4096, 2048, 32
+    p.scale, p.dtype, p.kv_dtype = 0.125, _hip.BF16, _hip.INT4
+    for k, v in over.items():
+        setattr(p, k, v)
+    return p
+
+
+PAGED = dict(block_table=0x20000, seqlens_k=0x20000, block_table_cols=1024, block_table_stride=1024, page_size=16, num_pages=4,
+             seqlen_k=16384)
+
+
+@pytest.mark.parametrize("over,split,msg", [
+    (PAGED, 4160, "258 pages"),
+    (dict(batch=1 << 16, seqlen_q=1 << 13), 64, "grid too large"),  # 2^31 rows
+    (dict(batch=1 << 10, seqlen_k=1 << 26), 64, "grid too large"),  # 2^31 partitions
+])
+def test_workspace_query_refuses_what_the_call_refuses(lib, over, split, msg):
+    p = _params(**over)
+    assert lib.fa_attention_cache_workspace_bytes(p, split) == 0 and msg in lib.fa_last_error().decode()
+    assert lib.fa_attention_cache(p, split, 0x10000, 1 << 62, None) == _hip.FA_ERR_UNSUPPORTED
+    assert msg in lib.fa_last_error().decode()
+
+
+def test_workspace_query_at_the_longest_partition(lib):
+    assert lib.fa_attention_cache_workspace_bytes(_params(**PAGED), 4096) == 4 * 4 * (64 * 4 + 8)
