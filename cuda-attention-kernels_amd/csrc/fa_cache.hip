@@ -957,6 +957,9 @@ const char* cache_refusal(const fa_cache_params& p, int32_t split_len) {
     return "split_len too long for the page size: a partition may span at most 258 pages";
   if ((int64_t)p.batch * p.heads_q * p.seqlen_q > INT32_MAX || workgroups(p, splits(p, split_len)) > INT32_MAX)
     return "grid too large";
+  // (a tile's scores are addressed by 32-bit byte offsets: 128 a row)
+  if (p.scores_out != nullptr && (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q > (1 << 23))
+    return "scores are formed for at most 2^23 (q-head, query) rows a kv-head";
   return nullptr;
 }
 

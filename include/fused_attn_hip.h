@@ -286,7 +286,8 @@ typedef struct fa_cache_params {
   /* optional scores, fp32 [batch, heads_kv, seqlen_k] with unit key stride:
        scores_out[b, h, j] = scores_in[b, h, j] + the sum of key j's attention weights over the heads_q / heads_kv
        q-heads and the seqlen_q queries
-     (scores_in may be NULL for zeros, or scores_out itself).  Dense caches only. */
+     (scores_in may be NULL for zeros, or scores_out itself).  Dense caches, and at most 2^23 rows (q-heads x queries)
+     a kv-head. */
   const float* scores_in;
   int64_t scores_in_stride_b, scores_in_stride_h;
   float* scores_out;

@@ -64,6 +64,7 @@ PAGED = dict(block_table=0x20000, seqlens_k=0x20000, block_table_cols=1024, bloc
     (PAGED, 4160, "258 pages"),
     (dict(batch=1 << 16, seqlen_q=1 << 13), 64, "grid too large"),  # 2^31 rows
     (dict(batch=1 << 10, seqlen_k=1 << 26), 64, "grid too large"),  # 2^31 partitions
+    (dict(scores_out=0x10000, seqlen_q=(1 << 22) + 1), 64, "at most 2^23"),  # their scores' offsets pass 32 bits
 ])
 def test_workspace_query_refuses_what_the_call_refuses(lib, over, split, msg):
     p = _params(**over)
@@ -74,3 +75,9 @@ def test_workspace_query_refuses_what_the_call_refuses(lib, over, split, msg):
 
 def test_workspace_query_at_the_longest_partition(lib):
     assert lib.fa_attention_cache_workspace_bytes(_params(**PAGED), 4096) == 4 * 4 * (64 * 4 + 8)
+
+
+def test_most_rows_that_are_scored(lib):
+    need = lib.fa_attention_cache_workspace_bytes(_params(scores_out=0x10000, seqlen_q=1 << 22), 64)
+    rows = 4 << 22  # partials, the rows' LSE, 64 scores a row
+    assert need == rows * (64 + 2) * 4 + rows * 4 + rows * 64 * 4
