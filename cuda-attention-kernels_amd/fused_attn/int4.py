@@ -13,8 +13,8 @@ The pair belongs to the row, so that rows are appended one token at a time (``ap
 picked one at a time (``evict_kv``); the FP8 cache shares a scale among 64 keys and allows neither without re-coding.
 The minimum and maximum are held to +-65504; an infinity counts as the row's end, a NaN makes its row's pair NaN.
 
-On the GPU these are HIP kernels for D in {64, 128, 256}; the writer and the reader take the torch form at other D, and
-every function does for CPU tensors or ``FUSED_ATTN_BACKEND=reference``.  The reference package has no 4-bit cache.
+On the GPU these are HIP kernels for D in {64, 128, 256}; the writer, the reader and ``append_kv_int4`` take the torch form at
+other D, and every function does for CPU tensors or ``FUSED_ATTN_BACKEND=reference``.  The reference package has no 4-bit cache.
 """
 from __future__ import annotations
 
@@ -71,29 +71,29 @@ def dequantize_kv_int4(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dt
 def append_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
                    v_cache: torch.Tensor, v_scale: torch.Tensor, seqlens_k: torch.Tensor,
                    block_table: Optional[torch.Tensor] = None) -> None:
-    """Write new tokens k, v [B, Hkv, n, D] into a 4-bit cache in place (one launch).
+    """Write new tokens k, v [B, Hkv, n, D] into a 4-bit cache in place (one launch; the torch form waits for the device).
 
     Token i of sequence b goes to position ``seqlens_k[b] + i`` (int32 [B], the keys it holds before the call, which
     the call leaves as they are) of k_cache / v_cache uint8 [B, Hkv, capacity, D/2], or with ``block_table`` (int32
     [B, pages]) of pools [num_pages, Hkv, page_size, D/2]; k_scale / v_scale are their pairs [..., 2].  A token past
     the cache's end, or whose page is outside the pool, is not written.  No two sequences may share a written page."""
     args = (k, v, k_cache, k_scale, v_cache, v_scale, seqlens_k, block_table)
-    if k.is_cuda and _pick_backend(k) == "hip":
+    if k.is_cuda and _pick_backend(k) == "hip" and k.dim() == 4 and k.shape[-1] in _hip.INT4_HEAD_DIMS:
         return _hip.append_kv_int4(*args)
     _hip.check_append(*args)
-    cap = k_cache.shape[2] if block_table is None else block_table.shape[1] * k_cache.shape[2]
+    b, _, n, _ = k.shape
+    page = k_cache.shape[2]
+    cap = page if block_table is None else block_table.shape[1] * page
+    pos = seqlens_k.long()[:, None] + torch.arange(n, device=k.device)
+    seq, token = ((pos >= 0) & (pos < cap)).nonzero(as_tuple=True)
+    at, pos = seq, pos[seq, token]
+    if block_table is not None:
+        at, pos = block_table[seq, pos // page].long(), pos % page
+        ok = (at >= 0) & (at < k_cache.shape[0])
+        seq, token, at, pos = (t[ok] for t in (seq, token, at, pos))
     for x, codes, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
         c, s = _quantize_kv_int4_torch(x)
-        for b, n in enumerate(seqlens_k.tolist()):
-            for i in range(x.shape[2]):
-                at, pos = b, n + i
-                if not 0 <= pos < cap:
-                    continue
-                if block_table is not None:
-                    at, pos = int(block_table[b, pos // codes.shape[2]]), pos % codes.shape[2]
-                    if not 0 <= at < codes.shape[0]:
-                        continue
-                codes[at, :, pos], scale[at, :, pos] = c[b, :, i], s[b, :, i]
+        codes[at, :, pos], scale[at, :, pos] = c[seq, :, token], s[seq, :, token]
 
 
 def attention_lengths_reference(q, k, v, causal: bool, scale: float, seqlens_k=None):

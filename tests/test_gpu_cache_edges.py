@@ -148,3 +148,22 @@ def test_scored_of_an_empty_batch(int4):
     o, w = fused_attn.attention_scored(torch.zeros(2, 4, 0, 64, device="cuda").half(), torch.zeros(2, 2, 0, 64, device="cuda").half(),
                                        torch.zeros(2, 2, 0, 64, device="cuda").half())
     assert o.shape == (2, 4, 0, 64) and w.shape == (2, 2, 0)
+
+
+@pytest.mark.parametrize("d", [16, 32, 96])
+@pytest.mark.parametrize("paged", [False, True])
+def test_append_at_other_head_dims(d, paged):
+    """The torch form, as for the writer and the reader."""
+    announce(f"int4 append d={d} paged={paged}")
+    b, hkv, new, page = 4, 3, 2, 16
+    lens = torch.tensor([0, 15, 31, -1], dtype=torch.int32, device="cuda")
+    k, v = rows((b, hkv, new, d), torch.float16, 1), rows((b, hkv, new, d), torch.float16, 2)
+    shape = (9, hkv, page) if paged else (b, hkv, 2 * page)
+    caches = [torch.zeros(*shape, w, dtype=t, device="cuda") for w, t in
+              ((d // 2, torch.uint8), (2, torch.float16)) * 2]
+    bt = torch.tensor([[8, 1], [0, 2], [3, 4], [5, 6]], dtype=torch.int32, device="cuda") if paged else None
+    want = [t.cpu() for t in caches]
+    fused_attn.append_kv_int4(k.cpu(), v.cpu(), *want, lens.cpu(), block_table=None if bt is None else bt.cpu())
+    fused_attn.append_kv_int4(k, v, *caches, lens, block_table=bt)
+    for g, w in zip(caches, want):
+        assert torch.equal(g.cpu(), w) and g.any()
