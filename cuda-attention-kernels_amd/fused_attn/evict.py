@@ -47,7 +47,7 @@ def attention_scored(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scores: 
         _hip.check_scores(scores, (q.shape[0], k.shape[1], k.shape[2]))
     if seqlens_k is not None:
         _hip.check_lengths(seqlens_k, q.shape[0])
-    o, _, weights = attention_lengths_reference(q, k, v, causal, scale, seqlens_k)
+    o, _, weights = attention_lengths_reference(q, k, v, causal, scale, seqlens_k, scored=True)
     return o, weights if scores is None else scores + weights
 
 

@@ -25,7 +25,7 @@ import torch
 
 from . import _hip
 from .ops import _pick_backend
-from .reference import attention_reference, lse_reference
+from .reference import attention_reference, causal_mask, lse_reference
 
 FP16_MAX = 65504.0
 
@@ -96,23 +96,32 @@ def append_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, k_sc
         codes[at, :, pos], scale[at, :, pos] = c[seq, :, token], s[seq, :, token]
 
 
-def attention_lengths_reference(q, k, v, causal: bool, scale: float, seqlens_k=None):
-    """The unfused path over the first ``seqlens_k[b]`` keys of each sequence: (o, lse, weights [B, Hkv, Nk])."""
+def _weights_reference(q, k, causal: bool, scale: float) -> torch.Tensor:
+    """The probabilities of ``attention_reference`` [B, Hkv, Nk], summed over a kv-head's q-heads and the queries."""
+    b, hq, nq, d = q.shape
+    hkv, nk = k.shape[1], k.shape[2]
+    s = torch.matmul(q.float().reshape(b, hkv, hq // hkv * nq, d), k.float().transpose(-1, -2)) * scale
+    if causal:
+        s = s.masked_fill(~causal_mask(nq, nk, device=q.device).repeat(hq // hkv, 1), -math.inf)
+    return torch.nan_to_num(torch.softmax(s, dim=-1), nan=0.0).sum(2)  # (rows without a visible key: NaN)
+
+
+def attention_lengths_reference(q, k, v, causal: bool, scale: float, seqlens_k=None, scored: bool = False):
+    """The unfused path over the first ``seqlens_k[b]`` keys of each sequence: (o, lse, and if ``scored`` the weights
+    [B, Hkv, Nk])."""
     b, hq, nq, _ = q.shape
     hkv, nk = k.shape[1], k.shape[2]
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    weights = torch.zeros(b, hkv, nk, dtype=torch.float32, device=q.device)
+    weights = torch.zeros(b, hkv, nk, dtype=torch.float32, device=q.device) if scored else None
     lens = [nk] * b if seqlens_k is None else [min(max(n, 0), nk) for n in seqlens_k.tolist()]
     for i, n in enumerate(lens):
         at = i if k.shape[0] == b else 0
         ki, vi, qi = k[at:at + 1, :, :n], v[at:at + 1, :, :n], q[i:i + 1]
         o[i:i + 1] = attention_reference(qi, ki, vi, causal=causal, scale=scale)
         lse[i:i + 1] = lse_reference(qi, ki, causal=causal, scale=scale)
-        # the probabilities are the output for the unit values
-        eye = torch.eye(n, dtype=torch.float32, device=q.device).expand(1, hkv, n, n)
-        p = attention_reference(qi.float(), ki.float(), eye, causal=causal, scale=scale)
-        weights[i, :, :n] = p.view(hkv, hq // hkv * nq, n).sum(1)
+        if scored:
+            weights[i, :, :n] = _weights_reference(qi, ki, causal, scale)[0]
     return o, lse, weights
 
 

@@ -4,7 +4,9 @@ import contextlib
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
+import fused_attn
 from fused_attn import _hip
 
 
@@ -81,3 +83,28 @@ def test_most_rows_that_are_scored(lib):
     need = lib.fa_attention_cache_workspace_bytes(_params(scores_out=0x10000, seqlen_q=1 << 22), 64)
     rows = 4 << 22  # partials, the rows' LSE, 64 scores a row
     assert need == rows * (64 + 2) * 4 + rows * 4 + rows * 64 * 4
+
+
+class _Largest(TorchDispatchMode):
+    """The most elements of any tensor that an operator gives."""
+    numel = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        got = func(*args, **(kwargs or {}))
+        for t in got if isinstance(got, (tuple, list)) else (got,):
+            if isinstance(t, torch.Tensor):
+                self.numel = max(self.numel, t.numel())
+        return got
+
+
+@pytest.mark.parametrize("nq,causal", [(1, False), (3, True)])
+def test_torch_forms_grow_with_the_keys_not_their_square(nq, causal):
+    n, hq, hkv, d = 2000, 4, 2, 64
+    gen = torch.Generator().manual_seed(1)
+    q = torch.randn(1, hq, nq, d, generator=gen).half()
+    (k4, ks), (v4, vs) = (fused_attn.quantize_kv_int4(torch.randn(1, hkv, n, d, generator=gen)) for _ in "kv")
+    for call in (lambda: fused_attn.attention_int4(q, k4, ks, v4, vs, causal=causal),
+                 lambda: fused_attn.attention_scored(q, k4, v4, causal=causal, k_scale=ks, v_scale=vs)):
+        with _Largest() as largest:
+            call()
+        assert largest.numel <= hq * n * d  # a kv-head's rows for each of its q-heads
