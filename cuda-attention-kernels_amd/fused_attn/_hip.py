@@ -1167,9 +1167,31 @@ def _row_elems(t: torch.Tensor) -> int:
     return n
 
 
-def _extent(t: torch.Tensor) -> tuple[int, int]:
-    last = sum((t.size(i) - 1) * t.stride(i) for i in range(t.dim()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _repeated(t: torch.Tensor, cut: int) -> tuple[int, int]:
+    """Bytes: (common divisor of the strides of at least ``cut``, extent of what those dims repeat)."""
+    size, step, last = t.element_size(), 0, 0
+    for n, stride in zip(t.shape, t.stride()):
+        if n > 1 and stride * size >= cut:
+            step = math.gcd(step, stride * size)
+        elif n > 1:
+            last += (n - 1) * stride * size
+    return step, last + size
+
+
+def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether x and y are seen to share no byte: their whole extents are apart, or with the dims of the larger strides
+    taken as repetitions at multiples of a common step, what they repeat is (halves of one buffer's rows, or of its
+    positions)."""
+    a, b = x.data_ptr(), y.data_ptr()
+    ea, eb = _repeated(x, 1 << 62)[1], _repeated(y, 1 << 62)[1]
+    if a + ea <= b or b + eb <= a:
+        return True
+    for cut in {s * t.element_size() for t in (x, y) for n, s in zip(t.shape, t.stride()) if n > 1 and s > 0}:
+        (ga, ea), (gb, eb) = _repeated(x, cut), _repeated(y, cut)
+        step = math.gcd(ga, gb)
+        if step and (b - a) % step >= ea and (a - b) % step >= eb:
+            return True
+    return False
 
 
 def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
@@ -1200,10 +1222,9 @@ def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
                 raise RuntimeError("out needs contiguous rows and positive strides")
             if o.size(2) > 1 and o.stride(2) < _row_elems(o):
                 raise RuntimeError("rows of out overlap")
-        spans = [_extent(o) for o in out if o.numel()]
-        for i, (lo, hi) in enumerate(spans):
-            others = [_extent(t) for t in (scores, *caches) if t.numel()] + spans[:i]
-            if any(lo < b and a < hi for a, b in others):
+        written = [o for o in out if o.numel()]
+        for i, o in enumerate(written):
+            if not all(_apart(o, t) for t in (scores, *caches, *written[:i]) if t.numel()):
                 raise RuntimeError("out must not share memory with the caches, the scores or another out")
 
 

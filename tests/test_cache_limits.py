@@ -108,3 +108,50 @@ def test_torch_forms_grow_with_the_keys_not_their_square(nq, causal):
         with _Largest() as largest:
             call()
         assert largest.numel <= hq * n * d  # a kv-head's rows for each of its q-heads
+
+
+def _bytes_of(t):
+    """Every byte address of t."""
+    at = torch.zeros(t.shape, dtype=torch.int64) + t.data_ptr()
+    for i, (n, s) in enumerate(zip(t.shape, t.stride())):
+        at = at + (torch.arange(n) * s * t.element_size()).view(-1, *[1] * (t.dim() - 1 - i))
+    return {a + i for a in at.flatten().tolist() for i in range(t.element_size())}
+
+
+def test_evict_out_in_parts_of_one_buffer():
+    """Outputs between each other's or the caches' rows are taken; memory that is shared is not."""
+    scores, k, v = torch.rand(2, 3, 9), torch.randn(2, 3, 9, 4).half(), torch.randn(2, 3, 9, 4).half()
+    (wk, wv), _, _, _ = fused_attn.evict_kv(scores, (k, v), 5, 1)
+    rows, heads, keys = torch.zeros(2, 3, 6, 2, 4).half(), torch.zeros(2, 6, 5, 4).half(), torch.zeros(2, 3, 14, 4).half()
+    apart = [(rows[..., 0, :], rows[..., 1, :]), (heads[:, :3], heads[:, 3:]), (keys[:, :, :5], keys[:, :, 9:]),
+             (heads[:, ::2], heads[:, 1::2]), (rows[:, :, :5, 1], heads[:, 3:])]
+    for out in apart:
+        assert not _bytes_of(out[0]) & _bytes_of(out[1])
+        got = fused_attn.evict_kv(scores, (k, v), 5, 1, out=out)[0]
+        assert torch.equal(got[0][:, :, :5], wk) and torch.equal(got[1][:, :, :5], wv)
+    both = torch.zeros(2, 3, 14, 4).half()  # a cache and its output in one buffer
+    both[:, :, 5:] = k
+    got = fused_attn.evict_kv(scores, (both[:, :, 5:],), 5, 1, out=(both[:, :, :5],))[0][0]
+    assert torch.equal(got, wk) and torch.equal(both[:, :, 5:], k)
+    shared = [(rows[..., 0, :], rows[..., 0, :]), (heads[:, :3], heads[:, 2:5]), (keys[:, :, :5], keys[:, :, 4:9]),
+              (rows.view(2, 3, 6, 8)[..., :4], rows.view(2, 3, 6, 8)[..., 2:6])]
+    for out in shared:
+        assert _bytes_of(out[0]) & _bytes_of(out[1])
+        with pytest.raises(RuntimeError, match="share memory"):
+            fused_attn.evict_kv(scores, (k, v), 5, 1, out=out)
+
+
+def test_apart_never_misses_a_shared_byte():
+    gen = torch.Generator().manual_seed(3)
+    pick = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=gen))  # noqa: E731
+    buffer, seen = torch.zeros(4000, dtype=torch.uint8), 0
+    for _ in range(3000):
+        views = []
+        for _ in range(2):
+            shape = [pick(1, 4) for _ in range(4)]
+            stride = [pick(0, 5) * pick(1, 40) for _ in range(3)] + [1]
+            views.append(buffer.as_strided(shape, stride, pick(0, 200)))
+        if _hip._apart(*views):
+            seen += 1
+            assert not _bytes_of(views[0]) & _bytes_of(views[1])
+    assert seen > 300

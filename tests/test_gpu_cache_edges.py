@@ -167,3 +167,16 @@ def test_append_at_other_head_dims(d, paged):
     fused_attn.append_kv_int4(k, v, *caches, lens, block_table=bt)
     for g, w in zip(caches, want):
         assert torch.equal(g.cpu(), w) and g.any()
+
+
+def test_evict_into_two_halves_of_one_buffer():
+    announce("evict interleaved out")
+    b, h, n, keep = 2, 3, 200, 50
+    scores = torch.rand(b, h, n, device="cuda", generator=gen(1))
+    k, v = (torch.randn(b, h, n, 64, device="cuda", generator=gen(i)).half() for i in (2, 3))
+    both = torch.zeros(b, h, keep + 3, 2, 64, device="cuda").half()
+    want, _, index, _ = fused_attn.evict_kv(scores, (k, v), keep, 5)
+    got = fused_attn.evict_kv(scores, (k, v), keep, 5, out=(both[..., 0, :], both[..., 1, :]))
+    for i in range(2):
+        assert torch.equal(both[:, :, :keep, i], want[i])
+    assert not both[:, :, keep:].any() and torch.equal(got[2], index)
