@@ -1220,8 +1220,11 @@ def check_evict(scores, caches, keep: int, recent: int, seqlens_k, out) -> None:
                                    f"got {o.dtype} {tuple(o.shape)}")
             if not _rows_contiguous(o) or any(o.size(i) > 1 and o.stride(i) <= 0 for i in range(3)):
                 raise RuntimeError("out needs contiguous rows and positive strides")
-            if o.size(2) > 1 and o.stride(2) < _row_elems(o):
-                raise RuntimeError("rows of out overlap")
+            end = _row_elems(o)
+            for stride, size in sorted((o.stride(i), o.size(i)) for i in range(3) if o.size(i) > 1):
+                if stride < end:
+                    raise RuntimeError("rows of out overlap")
+                end += stride * (size - 1)
         written = [o for o in out if o.numel()]
         for i, o in enumerate(written):
             if not all(_apart(o, t) for t in (scores, *caches, *written[:i]) if t.numel()):

@@ -155,3 +155,17 @@ def test_apart_never_misses_a_shared_byte():
             seen += 1
             assert not _bytes_of(views[0]) & _bytes_of(views[1])
     assert seen > 300
+
+
+@pytest.mark.parametrize("stride", [(60, 20, 3, 1), (60, 16, 4, 1), (40, 20, 4, 1), (4, 6, 40, 1)])
+def test_evict_refuses_an_output_whose_rows_overlap(stride):
+    out = torch.zeros(400).as_strided((2, 3, 5, 4), stride)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused_attn.evict_kv(torch.rand(2, 3, 9), (torch.randn(2, 3, 9, 4),), 5, 1, out=(out,))
+
+
+@pytest.mark.parametrize("stride", [(60, 20, 4, 1), (12, 4, 24, 1), (4, 8, 24, 1), (4, 8, 40, 1), (100, 33, 6, 1)])
+def test_evict_takes_outputs_of_any_order(stride):
+    scores, k = torch.rand(2, 3, 9), torch.randn(2, 3, 9, 4)
+    out = torch.zeros(400).as_strided((2, 3, 5, 4), stride)
+    assert torch.equal(fused_attn.evict_kv(scores, (k,), 5, 1, out=(out,))[0][0], fused_attn.evict_kv(scores, (k,), 5, 1)[0][0])
