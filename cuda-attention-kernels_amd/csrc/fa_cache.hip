@@ -126,14 +126,16 @@ __device__ __forceinline__ void memory_words(const uint8_t* p, uint32_t* out) {
   }
 }
 
-// Waves a SIMD, which bound the registers: as many as fit without spilling.  One row block of D <= 128 holds three (32
-// x 8 heads x 32768 keys: 177 us, with two 188); more rows hold O in more registers.  D = 256 with 32 rows spills some
-// at two waves, and is faster so than with one (148 and 178 us).
+// Waves a SIMD, which bound the registers: as many as fit without spilling, but for the cases named.  One row block of 4
+// bits and D <= 128, or 16 bits and D = 64, holds three (4 bits, 32 x 8 heads x 32768 keys: 177 us, with two 188); 16 bits
+// at D = 128 two (16 x 8 heads x 4 rows, 16384 keys: 208 us, with three and 6 registers spilled 219); more rows hold O in
+// more registers.  D = 256 with 32 rows of 4 bits spills 30 to 47 registers at two waves, and is faster so than with one
+// (148 and 178 us); 64 scored rows of D = 64 and fp16 spill 5 at two.
 template <int D, bool I4, int RT>
 constexpr int waves_per_simd() {
   if (RT == 4) return I4 && D == 64 ? 2 : 1;
   if (RT == 2) return D == 256 && !I4 ? 1 : 2;
-  return D == 256 ? 1 : 3;
+  return D == 256 ? 1 : I4 || D == 64 ? 3 : 2;
 }
 
 template <int D, class E, bool I4, bool PAGED, bool SCORES, int RT>
