@@ -6,8 +6,9 @@
 //   score_j = sum_r p_rj / sum_j' p_rj'                                               (attention_scored)
 //
 // Decomposition.  Keys are cut into partitions of split_len; a workgroup of four waves takes one partition of one
-// (batch, kv-head) for up to 16 * RT rows, its waves every fourth 32-key tile each; the waves' (m, l, O) are merged
-// through LDS into one fp32 partial, and cache_finish_kernel or splitk_combine_kernel merges the partitions.  Bound by
+// (batch, kv-head) for up to 16 * RT rows, its waves every fourth 32-key tile each (scored calls of up to 16 rows: a run
+// of tiles each, whose scores are written together); the waves' (m, l, O) are merged through LDS into one fp32 partial,
+// and cache_finish_kernel or splitk_combine_kernel merges the partitions.  Bound by
 // the bytes of the cache (D + 8 a key at 4 bits, 4 D at 16) up to 16 rows of D=128: bf16, 32 x 8 heads x 32768 keys
 // (1.14 GB) 177 us = 6.4 TB/s.  Bound by the vector unit beyond that (codes, exponentials: 8 x 8 heads x 64 rows of
 // D=256, 20000 keys, 342 MB and 84 GFLOP: 146 us) and at D=64, where a key's few bytes need the same exponentials (48 x
@@ -32,10 +33,11 @@
 // so that P's rounding (2^-8 of itself) meets only (code - 7.5)/16, at most 0.47 of it.  For fp16 outputs, whose own
 // rounding is 2^-11, P' is the sum of two bf16 terms and takes two products.  Everything else is fp32.
 //
-// Scores.  p needs the row's final sum, which no partition has.  The s of a row and key are written as they are
-// (4 bytes: 3% of a 16-bit key's bytes at D=128 and four rows, 12% of a 4-bit one's), and cache_finish_kernel turns them
-// into weights once the partitions' sums are there.  They lie tile by tile, the rows of 32 keys together, so that a
-// workgroup writes one run of memory.  A second pass over K would read half the cache again.
+// Scores.  p needs the row's final sum, which no partition has.  The s of a row and key are written as they are, and
+// cache_finish_kernel reads them and turns them into weights once the partitions' sums are there: 8 bytes for every row of
+// a key, in all.  A second pass over K would read 2 D bytes of a key instead (4 bits: D/2 + 4), so this moves less up to
+// about D/4 rows (D/16), 32 and 8 at D=128; the 128 rows of 8 heads x 8191 keys write 42 MB and read them again beside 34 MB
+// of keys and values.  They lie tile by tile, the rows of 32 keys together, so that a workgroup writes one run of memory.
 #include <algorithm>
 
 #include "fa_device.hpp"
@@ -575,8 +577,8 @@ attn_cache_kernel(const CacheArgs a) {
       }
     }
   };
-  // Staged: 33 MB of scores beside 1 GB of keys cost 60 us of 219 when every tile wrote its 512 bytes, 50 so (what is
-  // left is the memory's turning between reads and writes: writes that stay in the L2 cost 10).
+  // Staged: 33 MB of scores beside 1 GB of keys cost 60 us when every tile wrote its 512 bytes, 50 so, of 219 in all (what
+  // is left is the memory's turning between reads and writes: writes that stay in the L2 cost 10; three waves a SIMD).
   // Direct: rows past R are beyond the descriptor's limit and dropped, without a branch around the stores (loads and
   // stores share one counter: a wait after stores that may have been skipped waits for too much).
   const int stage_tiles = STAGED ? kStageFloats / (R * kTile) : 1;

@@ -12,7 +12,8 @@
 //   * evict_select_kernel: up to 8192 keys, one workgroup a (sequence, kv-head), which holds them in registers.
 //   * evict_count_kernel, evict_list_kernel, evict_index_kernel: more keys, up to 16 workgroups a (sequence, kv-head), each
 //     with a range of them.  Bound by vector instructions (about 80 a key and wave), so the work is spread: 8 heads x
-//     65536 keys took one workgroup each 49 us, and take the three launches 27.
+//     65536 keys took one workgroup each 49 us, and take the three launches 25.  Every group reads the whole list of the
+//     keys that share the threshold's first digit, so where most do (all scores equal, or most of them 0) it takes 67.
 //   * gather_rows_kernel: the scores and the rows of up to eight tensors in one launch; a thread copies units of the widest
 //     power of two (16 bytes at most) that a tensor's rows, strides and addresses allow.  HBM-bound: 16 x 8 heads, 4096
 //     of 8192 keys with 4-bit rows of D=128, 33 us (161 MB moved: 4.9 TB/s); 8 heads, 16384 of 65536 with bf16 rows of

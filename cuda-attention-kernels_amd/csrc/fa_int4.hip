@@ -12,9 +12,10 @@
 // (scale, zero) pairs lie in a tensor of their own, one 4-byte word a row.  Scales per row (not per block of
 // keys) let rows be appended and picked one at a time.
 //
-// HBM-bound.  A lane holds 8 channels (16 bytes of 16-bit input, one 4-byte word of codes), so D/8 lanes hold a
-// row and its ends are a reduction over them; UNROLL rows a lane are loaded before any is worked on.  16 x 8 x 32768 rows
-// of D=128 bf16 (1.36 GB): written in 250 us, read back in 235, 5.4 and 5.8 TB/s.
+// A lane holds 8 channels (16 bytes of 16-bit input, one 4-byte word of codes), so D/8 lanes hold a row and its ends are a
+// reduction over them; UNROLL rows a lane are loaded before any is worked on.  16 x 8 x 32768 rows of D=128 bf16 (1.36 GB
+// each way): written in 251 us, read back in 223, 5.4 and 6.1 TB/s (265 and 234 under the profiler).  The reader is bound by
+// HBM; the writer by the vector unit as well, which its 154 instructions for 8 channels a lane keep busy nearly all the time.
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
 

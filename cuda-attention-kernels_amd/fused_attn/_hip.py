@@ -1080,8 +1080,13 @@ def default_cache_split_len(seqlen_q: int, seqlen_k: int, batch: int, heads_kv: 
     workgroups, in whole rounds of a workgroup's four waves of 32 keys.
 
     A workgroup costs about 4 us before and after its tiles, and more with 64 rows, whose merge moves 64 KiB through LDS
-    (8 heads, 128 rows each, 8191 keys, D=128 16-bit: 37 us at 512 keys, 72 at 128).  A lone long sequence is cut into 128
-    at most: the merge of more costs more than they save (2 x 54738 keys, D=256: 18 us at 512 keys, 34 at 128)."""
+    (8 heads, 128 rows each, 8191 keys, D=128 16-bit: 37 us at 512 keys, 72 at 128).  A lone sequence is cut into 128 at
+    most, as long as they are of 4096 keys or fewer: the merge of more costs more than they save (2 x 54738 keys, D=256: 18
+    us at 512 keys, 34 at 128).
+
+    The length is made from the longest sequence, so ragged batches and D=64, whose keys are few bytes, would often take
+    a shorter one: 48 x 8 heads of up to 8192 keys, D=64 paged, 49 us at the 4096 chosen here and 42 at 2048; 35 x 8 heads
+    of 32 rows, D=64, 12618 keys 96 and 84; 1 x 8 heads of 7735 keys, D=256, scored, takes 22 at 128 and 19 at 512."""
     rows = group * seqlen_q
     block = 16 if rows <= 16 else 32 if rows <= 32 or head_dim == 256 else 64  # rows of a workgroup
     items = max(1, batch * heads_kv * -(-rows // block))

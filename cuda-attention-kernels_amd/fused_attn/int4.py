@@ -134,7 +134,9 @@ def attention_int4(q: torch.Tensor, k4: torch.Tensor, k_scale: torch.Tensor, v4:
 
     ``seqlens_k`` (int32 [B], on the device): only the first seqlens_k[b] rows of sequence b are keys, and ``causal``
     aligns its queries to their end; the rows behind them are not read.  Any number of queries is accepted; the kernel
-    is made for decode (few queries)."""
+    is made for decode.  From about 64 (one sequence) to 128 queries (eight; 32 q-heads over 8, 8192 keys, D <= 128; twice
+    that at D=256) ``dequantize_kv_int4`` and ``attention`` are faster together: 8 x 128 queries of D=128 in 208 us, 271
+    here, 16 queries in 144 and 72."""
     if k4.dtype != torch.uint8:
         raise RuntimeError(f"attention_int4 needs 4-bit K/V (uint8), got {k4.dtype}")
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale

@@ -295,7 +295,8 @@ typedef struct fa_cache_params {
 } fa_cache_params;
 
 /* Bytes of workspace fa_attention_cache needs: fa_splitk_workspace_bytes, and with scores 4 bytes for every (q-head,
-   query, key).  0 for parameters that the call would refuse. */
+   query, key), keys rounded up to 32, and 4 for every (q-head, query).  0 for parameters that the call would refuse (a
+   split_len that spans more than 258 pages among them), and without a batch or queries. */
 size_t fa_attention_cache_workspace_bytes(const fa_cache_params* p, int32_t split_len);
 /* split_len: keys a partition, a positive multiple of 64; workspace 16-byte aligned. */
 fa_status fa_attention_cache(const fa_cache_params* p, int32_t split_len, void* workspace, size_t workspace_bytes,
