@@ -13,8 +13,8 @@ The pair belongs to the row, so that rows are appended one token at a time (``ap
 picked one at a time (``evict_kv``); the FP8 cache shares a scale among 64 keys and allows neither without re-coding.
 The minimum and maximum are held to +-65504; an infinity counts as the row's end, a NaN makes its row's pair NaN.
 
-On the GPU these are HIP kernels for D in {64, 128, 256}; the writer, the reader and ``append_kv_int4`` take the torch form at
-other D, and every function does for CPU tensors or ``FUSED_ATTN_BACKEND=reference``.  The reference package has no 4-bit cache.
+On the GPU these are HIP kernels for D in {64, 128, 256}; the writer, the reader and, at multiples of 8, ``append_kv_int4``
+take the torch form at other D, and every function does for CPU tensors or ``FUSED_ATTN_BACKEND=reference``.  The reference package has no 4-bit cache.
 """
 from __future__ import annotations
 
