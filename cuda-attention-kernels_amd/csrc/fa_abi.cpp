@@ -195,6 +195,32 @@ fa_status validate_cache(const fa_cache_params* p, int32_t split_len) {
   return FA_OK;
 }
 
+fa_status validate_pages(const fa_pages_params* p, bool allocate) {
+  if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->batch < 0 || p->block_table_cols < 0 || p->free_capacity < 0 || (allocate && p->num_tokens < 0))
+    return fail(FA_ERR_INVALID_ARGUMENT, "sizes must be non-negative");
+  if (p->free_capacity == INT32_MAX || (allocate && p->num_tokens == INT32_MAX))
+    return fail(FA_ERR_UNSUPPORTED, "free_pages and slots must have fewer than 2^31 - 1 entries");
+  if (p->page_size <= 0 || p->page_size > FA_MAX_PAGE_SIZE)
+    return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be positive, at most 2^24 keys");
+  if (p->batch > (1 << 24)) return fail(FA_ERR_UNSUPPORTED, "at most 2^24 requests");
+  if (p->batch > 1 && p->block_table_stride < p->block_table_cols)
+    return fail(FA_ERR_INVALID_ARGUMENT, "block_table rows overlap (stride below cols)");
+  if (p->batch > 0 && (p->seqlens == nullptr || p->seqlens_out == nullptr ||
+                       (allocate ? p->new_lens == nullptr : p->done == nullptr)))
+    return fail(FA_ERR_INVALID_ARGUMENT, "lengths must be non-NULL");
+  if (p->batch > 0 && p->block_table_cols > 0 && p->block_table == nullptr)
+    return fail(FA_ERR_INVALID_ARGUMENT, "block_table must be non-NULL");
+  if (p->num_free == nullptr || p->num_free_out == nullptr || (p->free_capacity > 0 && p->free_pages == nullptr) ||
+      (allocate && (p->cu_seqlens == nullptr || (p->num_tokens > 0 && p->slots == nullptr))))
+    return fail(FA_ERR_INVALID_ARGUMENT, "the list of free pages, its length and the outputs must be non-NULL");
+  if (!aligned(p->block_table, 4) || !aligned(p->seqlens, 4) || !aligned(p->new_lens, 4) || !aligned(p->keep_lens, 4) ||
+      !aligned(p->free_pages, 4) || !aligned(p->num_free, 4) || !aligned(p->cu_seqlens, 4) || !aligned(p->seqlens_out, 4) ||
+      !aligned(p->num_free_out, 4) || !aligned(p->slots, 8))
+    return fail(FA_ERR_INVALID_ARGUMENT, "slots must be 8-byte, all others 4-byte aligned");
+  return FA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -407,6 +433,50 @@ fa_status fa_quantize_kv_fp8(const fa_quant_params* p, void* stream) {
     return fail(FA_ERR_INVALID_ARGUMENT, "x and x8 must be 16-byte aligned, scale 4-byte aligned");
   const char* err = nullptr;
   const fa_status st = fa::run_quantize_fp8(*p, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+fa_status fa_allocate_pages(const fa_pages_params* p, void* stream) {
+  g_last_error.clear();
+  fa_status st = validate_pages(p, true);
+  if (st != FA_OK) return st;
+  const char* err = nullptr;
+  st = fa::run_allocate_pages(*p, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+fa_status fa_release_pages(const fa_pages_params* p, void* stream) {
+  g_last_error.clear();
+  fa_status st = validate_pages(p, false);
+  if (st != FA_OK) return st;
+  const char* err = nullptr;
+  st = fa::run_release_pages(*p, reinterpret_cast<hipStream_t>(stream), &err);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+fa_status fa_append_kv_paged(const fa_append_paged_params* p, void* stream) {
+  g_last_error.clear();
+  if (p == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->num_tokens < 0 || p->heads < 0 || p->head_dim < 0 || p->num_pages < 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "sizes must be non-negative");
+  if (p->head_dim % 8) return fail(FA_ERR_UNSUPPORTED, "head_dim must be a multiple of 8");
+  if (p->page_size <= 0 || p->page_size > FA_MAX_PAGE_SIZE)
+    return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be positive, at most 2^24 keys");
+  if ((int64_t)p->num_pages * p->page_size > INT32_MAX) return fail(FA_ERR_UNSUPPORTED, "a pool must have fewer than 2^31 slots");
+  if (p->num_tokens == 0 || p->heads == 0 || p->head_dim == 0 || p->num_pages == 0) return FA_OK;
+  if (p->k == nullptr || p->v == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->slots == nullptr)
+    return fail(FA_ERR_INVALID_ARGUMENT, "k, v, the pools and slots must be non-NULL");
+  if (!aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->k_cache, 16) || !aligned(p->v_cache, 16) || !aligned(p->slots, 8))
+    return fail(FA_ERR_INVALID_ARGUMENT, "k, v and the pools must be 16-byte, slots 8-byte aligned");
+  for (const int64_t s : {p->k_stride_t, p->k_stride_h, p->v_stride_t, p->v_stride_h, p->k_page_stride, p->k_cache_stride_h,
+                          p->k_cache_stride_n, p->v_page_stride, p->v_cache_stride_h, p->v_cache_stride_n}) {
+    if (s < 0 || s % 8) return fail(FA_ERR_INVALID_ARGUMENT, "strides must be non-negative multiples of 16 bytes");
+  }
+  const char* err = nullptr;
+  const fa_status st = fa::run_append_paged(*p, reinterpret_cast<hipStream_t>(stream), &err);
   if (st != FA_OK) return fail(st, err ? err : "launch failed");
   return FA_OK;
 }

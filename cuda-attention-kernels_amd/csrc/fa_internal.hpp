@@ -153,6 +153,28 @@ struct EvictArgs {
   EvictTensor tensors[FA_MAX_EVICT_TENSORS + 1];  // the scores first
 };
 
+// Pages (fa_pages.hip): fa_pages_params as the kernels read it.
+struct PagesArgs {
+  int32_t* block_table;
+  int64_t sbt;
+  const int32_t *seqlens, *new_lens, *keep_lens;
+  const uint8_t* done;
+  int32_t* free_pages;
+  const int32_t* num_free;
+  int64_t* slots;
+  int32_t *cu_seqlens, *seqlens_out, *num_free_out;
+  int32_t batch, cols, page_size, free_capacity, num_tokens;
+  uint32_t capacity;  // keys that a request may hold
+};
+struct AppendPagedArgs {
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  int64_t skt, skh, svt, svh, skp, skch, skcn, svp, svch, svcn;  // elements
+  const int64_t* slots;
+  int64_t num_slots;
+  int32_t heads, pieces, page_size, total;  // pieces: 16-byte pieces of a row; total: of all rows
+};
+
 // Number of rows (q-heads x queries) one split-K workgroup covers, and the
 // workgroup shape chosen for a given row count G*Nq.
 int splitk_waves_for_rows(int rows);
@@ -197,6 +219,9 @@ size_t cache_workspace_bytes(const fa_cache_params& p, int32_t split_len);
 fa_status run_cache(const fa_cache_params& p, int32_t split_len, void* workspace, hipStream_t stream, const char** err);
 size_t evict_workspace_bytes(const fa_evict_params& p);
 fa_status run_evict(const fa_evict_params& p, void* workspace, hipStream_t stream, const char** err);
+fa_status run_allocate_pages(const fa_pages_params& p, hipStream_t stream, const char** err);
+fa_status run_release_pages(const fa_pages_params& p, hipStream_t stream, const char** err);
+fa_status run_append_paged(const fa_append_paged_params& p, hipStream_t stream, const char** err);
 // kv: paged K/V (nullptr for a dense cache)
 fa_status run_splitk(const fa_fwd_params& p, int32_t split_len, void* workspace, hipStream_t stream,
                      const char** err, const fa_paged_kv* kv = nullptr);

@@ -10,6 +10,7 @@ from .evict import attention_scored, evict_kv
 from .fp8 import attention_fp8, attention_fp8_triton, dequantize_kv_fp8, quantize_kv_fp8
 from .int4 import append_kv_int4, attention_int4, dequantize_kv_int4, quantize_kv_int4
 from .ops import attention, attention_varlen, available_backends, pack_varlen
+from .pages import allocate_pages, append_kv_paged, release_pages
 from .paged import attention_paged, attention_paged_reference, paged_from_dense, paged_from_dense_fp8, \
     paged_from_dense_int4
 from .reference import attention_reference, attention_varlen_reference
@@ -34,6 +35,9 @@ __all__ = [
     "paged_from_dense",
     "paged_from_dense_fp8",
     "paged_from_dense_int4",
+    "allocate_pages",
+    "release_pages",
+    "append_kv_paged",
     "attention_int4",
     "quantize_kv_int4",
     "dequantize_kv_int4",

@@ -236,6 +236,52 @@ class EvictParams(ctypes.Structure):
     ]
 
 
+class PagesParams(ctypes.Structure):
+    """Mirror of ``fa_pages_params`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("block_table_cols", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("free_capacity", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("seqlens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("done", ctypes.c_void_p),
+        ("keep_lens", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("num_free", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p),
+        ("num_free_out", ctypes.c_void_p),
+    ]
+
+
+class AppendPagedParams(ctypes.Structure):
+    """Mirror of ``fa_append_paged_params`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        *_int64s("k_stride_t", "k_stride_h", "v_stride_t", "v_stride_h"),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        *_int64s("k_page_stride", "k_cache_stride_h", "k_cache_stride_n", "v_page_stride", "v_cache_stride_h",
+                 "v_cache_stride_n"),
+        ("slots", ctypes.c_void_p),
+        ("num_tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 _lib = None
 _lib_error: Optional[str] = None
 _lock = threading.Lock()
@@ -259,6 +305,18 @@ def _cache_library() -> ctypes.CDLL:
     lib = load_library()
     if not _has_int4(lib):
         raise RuntimeError(f"fused_attn HIP backend: {library_path()} is older than the 4-bit cache: build it again")
+    return lib
+
+
+def _has_pages(lib: ctypes.CDLL) -> bool:
+    return isinstance(getattr(lib, "fa_allocate_pages", None), lib._FuncPtr)
+
+
+def _pages_library() -> ctypes.CDLL:
+    """The library, if it has the functions of pages (added within this ABI version)."""
+    lib = load_library()
+    if not _has_pages(lib):
+        raise RuntimeError(f"fused_attn HIP backend: {library_path()} is older than allocate_pages: build it again")
     return lib
 
 
@@ -303,6 +361,11 @@ def _bind(lib: ctypes.CDLL) -> None:
         lib.fa_evict_kv_workspace_bytes.restype = ctypes.c_size_t
         lib.fa_evict_kv.argtypes = [ctypes.POINTER(EvictParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.fa_evict_kv.restype = ctypes.c_int
+    if _has_pages(lib):
+        for f in (lib.fa_allocate_pages, lib.fa_release_pages):
+            f.argtypes, f.restype = [ctypes.POINTER(PagesParams), ctypes.c_void_p], ctypes.c_int
+        lib.fa_append_kv_paged.argtypes = [ctypes.POINTER(AppendPagedParams), ctypes.c_void_p]
+        lib.fa_append_kv_paged.restype = ctypes.c_int
     lib.fa_device_supported.argtypes = [ctypes.c_int32]
     lib.fa_device_supported.restype = ctypes.c_int32
     lib.fa_last_error.argtypes = []
@@ -1277,3 +1340,126 @@ def evict_kv(scores, caches, keep: int, recent: int, seqlens_k, out):
         workspace = torch.empty(need // 4, dtype=torch.float32, device=dev) if need else None
         _check(lib.fa_evict_kv(p, workspace.data_ptr() if need else None, need, _stream(scores)), "evict_kv")
     return dst, kept, index, lens
+
+
+# ----------------------------------------------------------------------------------------------
+# pages
+# ----------------------------------------------------------------------------------------------
+
+MAX_PAGE_SIZE = 1 << 24  # FA_MAX_PAGE_SIZE
+
+
+def _check_int32(t: torch.Tensor, name: str, b: int) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != (b,):
+        raise RuntimeError(f"{name} must be int32 [{b}], got {t.dtype} {tuple(t.shape)}")
+
+
+def check_pages(block_table, seqlens_k, free_pages, num_free, page_size: int, new_lens=None, num_tokens: int = 0, done=None,
+                keep_lens=None) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise RuntimeError(f"block_table must be int32 [B, pages], got {block_table.dtype} {tuple(block_table.shape)}")
+    b = block_table.shape[0]
+    check_lengths(seqlens_k, b)
+    if new_lens is not None:
+        _check_int32(new_lens, "new_lens", b)
+    if keep_lens is not None:
+        _check_int32(keep_lens, "keep_lens", b)
+    if done is not None and (done.dtype not in (torch.bool, torch.uint8) or tuple(done.shape) != (b,)):
+        raise RuntimeError(f"done must be bool or uint8 [{b}], got {done.dtype} {tuple(done.shape)}")
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        raise RuntimeError(f"free_pages must be contiguous int32 [F], got {free_pages.dtype} {tuple(free_pages.shape)}")
+    if num_free.dtype != torch.int32 or num_free.numel() != 1:
+        raise RuntimeError(f"num_free must be int32 of one element, got {num_free.dtype} {tuple(num_free.shape)}")
+    if not 0 < page_size <= MAX_PAGE_SIZE:
+        raise RuntimeError(f"page_size must be positive, at most {MAX_PAGE_SIZE}, got {page_size}")
+    if not 0 <= num_tokens < 2 ** 31 - 1:
+        raise RuntimeError(f"num_tokens must be non-negative and below 2^31 - 1, got {num_tokens}")
+    for t in (seqlens_k, new_lens, done, keep_lens, free_pages, num_free):
+        if t is not None and t.device != block_table.device:
+            raise RuntimeError(f"all tensors must be on {block_table.device}, got {t.device}")
+
+
+def _pages_params(block_table, seqlens_k, free_pages, num_free, page_size: int, num_tokens: int = 0) -> PagesParams:
+    b, cols = block_table.shape
+    return PagesParams(block_table.data_ptr(), _stride(block_table, 0), b, cols, page_size, free_pages.numel(), num_tokens, 0,
+                       seqlens_k.data_ptr(), None, None, None, free_pages.data_ptr(), num_free.data_ptr())
+
+
+def allocate_pages(block_table, seqlens_k, new_lens, free_pages, num_free, page_size: int, num_tokens: int):
+    """Pages and slots for a batch's new tokens: (slots, cu_seqlens, seqlens, num_free), and block_table in place."""
+    check_pages(block_table, seqlens_k, free_pages, num_free, page_size, new_lens=new_lens, num_tokens=num_tokens)
+    b, cols = block_table.shape
+    if block_table.numel() and (cols > 1 and block_table.stride(1) != 1 or b > 1 and block_table.stride(0) < cols):
+        raise RuntimeError("block_table is written in place: it needs a unit last stride and rows that do not overlap")
+    _require_gpu(block_table, seqlens_k, new_lens, free_pages, num_free)
+    lib = _pages_library()
+    seqlens_k, new_lens = seqlens_k.contiguous(), new_lens.contiguous()
+    dev = block_table.device
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    small = torch.empty(2 * b + 2, dtype=torch.int32, device=dev)  # one allocation for the three small outputs
+    cu, lens, left = small[:b + 1], small[b + 1:2 * b + 1], small[2 * b + 1:].view(num_free.shape)
+    p = _pages_params(block_table, seqlens_k, free_pages, num_free, page_size, num_tokens)
+    p.new_lens, p.slots, p.cu_seqlens = new_lens.data_ptr(), slots.data_ptr(), cu.data_ptr()
+    p.seqlens_out, p.num_free_out = lens.data_ptr(), left.data_ptr()
+    with _on_device(dev):
+        _check(lib.fa_allocate_pages(p, _stream(block_table)), "allocate_pages")
+    return slots, cu, lens, left
+
+
+def release_pages(block_table, seqlens_k, done, free_pages, num_free, page_size: int, keep_lens=None):
+    """The pages of finished requests back onto free_pages, in place: (seqlens, num_free)."""
+    check_pages(block_table, seqlens_k, free_pages, num_free, page_size, done=done, keep_lens=keep_lens)
+    _require_gpu(block_table, seqlens_k, done, free_pages, num_free, *([] if keep_lens is None else [keep_lens]))
+    lib = _pages_library()
+    block_table, seqlens_k, done = _plain_table(block_table), seqlens_k.contiguous(), done.contiguous()
+    keep_lens = None if keep_lens is None else keep_lens.contiguous()
+    b, dev = block_table.shape[0], block_table.device
+    small = torch.empty(b + 1, dtype=torch.int32, device=dev)
+    lens, left = small[:b], small[b:].view(num_free.shape)
+    p = _pages_params(block_table, seqlens_k, free_pages, num_free, page_size)
+    p.done, p.keep_lens = done.data_ptr(), None if keep_lens is None else keep_lens.data_ptr()
+    p.seqlens_out, p.num_free_out = lens.data_ptr(), left.data_ptr()
+    with _on_device(dev):
+        _check(lib.fa_release_pages(p, _stream(block_table)), "release_pages")
+    return lens, left
+
+
+def check_append_paged(k, v, k_cache, v_cache, slots) -> None:
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
+        raise RuntimeError(f"k and v must both be [T, Hkv, D] of one type, got {k.dtype} {tuple(k.shape)} and "
+                           f"{v.dtype} {tuple(v.shape)}")
+    if k.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"k and v must be float16 or bfloat16, got {k.dtype}")
+    if k.shape[2] % 8:
+        raise RuntimeError(f"D must be a multiple of 8, got {k.shape[2]}")
+    for name, pool in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if pool.dim() != 4 or pool.dtype != k.dtype or (pool.shape[1], pool.shape[3]) != tuple(k.shape[1:]):
+            raise RuntimeError(f"{name} must be {k.dtype} [num_pages, {k.shape[1]}, page_size, {k.shape[2]}], got {pool.dtype} "
+                               f"{tuple(pool.shape)}")
+        # written in place: it cannot be copied into another layout first
+        if pool.numel() and (pool.stride(3) != 1 or pool.data_ptr() % 16
+                             or any(pool.size(i) > 1 and (pool.stride(i) <= 0 or pool.stride(i) % 8) for i in range(3))):
+            raise RuntimeError(f"{name} needs a unit D stride, a 16-byte aligned start and strides of whole 16 bytes")
+    if k_cache.shape != v_cache.shape:
+        raise RuntimeError(f"k_cache and v_cache must have the same shape, got {tuple(k_cache.shape)} and "
+                           f"{tuple(v_cache.shape)}")
+    if slots.dtype != torch.int64 or tuple(slots.shape) != (k.shape[0],):
+        raise RuntimeError(f"slots must be int64 [{k.shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
+    for t in (v, k_cache, v_cache, slots):
+        if t.device != k.device:
+            raise RuntimeError(f"all tensors must be on {k.device}, got {t.device}")
+
+
+def append_kv_paged(k, v, k_cache, v_cache, slots) -> None:
+    """Packed rows k, v [T,Hkv,D] to their slots of 16-bit pools, in place."""
+    check_append_paged(k, v, k_cache, v_cache, slots)
+    _require_gpu(k, v, k_cache, v_cache, slots)
+    lib = _pages_library()
+    if k.numel() == 0 or k_cache.numel() == 0:
+        return
+    k, v, slots = _aligned_rows(k, 8), _aligned_rows(v, 8), slots.contiguous()
+    p = AppendPagedParams(k.data_ptr(), v.data_ptr(), _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1),
+                          k_cache.data_ptr(), v_cache.data_ptr(), *_strides3(k_cache), *_strides3(v_cache), slots.data_ptr(),
+                          *k.shape, k_cache.shape[0], k_cache.shape[2])
+    with _on_device(k.device):
+        _check(lib.fa_append_kv_paged(p, _stream(k)), "append_kv_paged")

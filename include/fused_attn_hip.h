@@ -29,8 +29,8 @@ extern "C" {
 #endif
 
 /* Raised by changes that an older caller or library does not survive; added functions keep it
-   (fa_attention_fwd_ws and its size query came within 6, and so did the functions of the 4-bit cache and of
-   eviction: look them up before use). */
+   (fa_attention_fwd_ws and its size query came within 6, and so did the functions of the 4-bit cache, of
+   eviction and of pages: look them up before use). */
 #define FA_ABI_VERSION 6
 
 /* Element types (reference: DType, csrc/flash_attn.h:7). */
@@ -328,6 +328,55 @@ typedef struct fa_evict_params {
 /* Bytes of workspace fa_evict_kv needs (16-byte aligned): 0 up to 8192 keys. */
 size_t fa_evict_kv_workspace_bytes(const fa_evict_params* p);
 fa_status fa_evict_kv(const fa_evict_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages of a K/V cache (the reference has none).  Request b holds n = max(seqlens[b], 0) keys in the pages
+   block_table[b, 0 .. ceil(n / page_size) - 1]; free_pages[0 .. num_free[0] - 1] are the pages nobody holds.  num_free is
+   read as one of [0, free_capacity]. */
+typedef struct fa_pages_params {
+  int32_t* block_table; /* [batch, block_table_cols], rows block_table_stride elements apart */
+  int64_t block_table_stride;
+  int32_t batch, block_table_cols, page_size; /* page_size in [1, FA_MAX_PAGE_SIZE] */
+  int32_t free_capacity;                      /* entries of free_pages, below 2^31 - 1 */
+  int32_t num_tokens;                         /* allocate: entries of slots, below 2^31 - 1 */
+  int32_t reserved;
+  const int32_t* seqlens;   /* [batch] */
+  const int32_t* new_lens;  /* [batch], allocate: new tokens (negative: none) */
+  const uint8_t* done;      /* [batch], release: not 0 for requests that give their pages back */
+  const int32_t* keep_lens; /* [batch] or NULL, release: keys whose whole pages stay with others */
+  int32_t* free_pages;
+  const int32_t* num_free;
+  int64_t* slots;        /* [num_tokens], allocate */
+  int32_t* cu_seqlens;   /* [batch + 1], allocate */
+  int32_t* seqlens_out;  /* [batch] */
+  int32_t* num_free_out; /* [1] */
+} fa_pages_params;
+
+/* New tokens get their pages.  They are packed: request b's m = max(new_lens[b], 0) are tokens cu_seqlens[b] to
+   cu_seqlens[b + 1] - 1 (cu_seqlens held to num_tokens).  A request's further pages are taken from the end of the list,
+   requests in order, and entered in its row of block_table; slots[t] = page * page_size + offset of token t.  A request is
+   refused if its keys exceed block_table_cols * page_size, its tokens num_tokens, or it needs pages and the list has too
+   few for it and all before it: its tokens get slot -1 and it keeps its length and row.  Tokens of no request get -1, and
+   so do those whose page in block_table is negative.  The outputs must not overlap the inputs; free_pages is not changed. */
+fa_status fa_allocate_pages(const fa_pages_params* p, void* stream);
+/* Requests with done[b] give the pages behind their first floor(keep_lens[b] / page_size) back, in order, onto the end of the
+   list, and their length becomes 0.  Requests whose pages the list has no room for keep both.  block_table is not changed. */
+fa_status fa_release_pages(const fa_pages_params* p, void* stream);
+
+/* K/V rows of packed tokens to their slots of 16-bit pools, in place.  A slot outside [0, num_pages * page_size) is not
+   written; two tokens must not have the same one. */
+typedef struct fa_append_paged_params {
+  const void* k; /* [num_tokens, heads, head_dim], 16-bit, unit head_dim stride */
+  const void* v;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h; /* elements; everything 16-byte aligned */
+  void* k_cache; /* pools [num_pages, heads, page_size, head_dim] */
+  void* v_cache;
+  int64_t k_page_stride, k_cache_stride_h, k_cache_stride_n, v_page_stride, v_cache_stride_h, v_cache_stride_n;
+  const int64_t* slots; /* [num_tokens] */
+  int32_t num_tokens, heads, head_dim; /* head_dim a multiple of 8 */
+  int32_t num_pages, page_size;        /* num_pages * page_size below 2^31 */
+  int32_t reserved;
+} fa_append_paged_params;
+fa_status fa_append_kv_paged(const fa_append_paged_params* p, void* stream);
 
 /* FA_ABI_VERSION of the loaded library. */
 int32_t fa_abi_version(void);
