@@ -221,6 +221,64 @@ fa_status validate_pages(const fa_pages_params* p, bool allocate) {
   return FA_OK;
 }
 
+// Validation shared by the calls over 16-bit and FP8 pools; clears q's K/V batch strides.  table_keys: keys that a row of
+// the table must have room for.
+fa_status validate_paged(fa_fwd_params* q, const fa_paged_kv* kv, int32_t split_len, int32_t table_keys) {
+  q->k_stride_b = q->v_stride_b = 0;  // keys are found through the block table
+  fa_status st = validate(q, /*varlen=*/false, /*fp8_ok=*/true, /*generic_ok=*/false);
+  if (st != FA_OK) return st;
+  if (q->lse != nullptr && (q->lse_stride_b < 0 || q->lse_stride_h < 0))
+    return fail(FA_ERR_INVALID_ARGUMENT, "negative LSE stride");
+  if (split_len <= 0 || split_len % 64 != 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "split_len must be a positive multiple of 64");
+  if (kv->page_size <= 0 || kv->page_size % 16 != 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 16");
+  if (kv->page_size > FA_MAX_PAGE_SIZE)
+    return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be at most 2^24 keys");
+  const bool fp8 = q->kv_dtype == FA_DTYPE_FP8_E4M3;
+  if (fp8 && kv->page_size % 64 != 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "FP8 pools need page_size a multiple of 64 (64-key scale blocks)");
+  if (fp8 && (q->scale_stride_b < 0 || q->scale_stride_h < 0))
+    return fail(FA_ERR_INVALID_ARGUMENT, "negative FP8 scale stride");
+  if (kv->num_pages < 0 || kv->block_table_cols < 0) return fail(FA_ERR_INVALID_ARGUMENT, "negative page count");
+  if (q->batch == 0 || q->seqlen_q == 0) return FA_OK;
+  if (kv->block_table == nullptr || kv->seqlens_k == nullptr)
+    return fail(FA_ERR_INVALID_ARGUMENT, "block_table and seqlens_k must be non-NULL");
+  if (!aligned(kv->block_table, 4) || !aligned(kv->seqlens_k, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "block_table and seqlens_k must be 4-byte aligned");
+  if (q->batch > 1 && kv->block_table_stride < kv->block_table_cols)
+    return fail(FA_ERR_INVALID_ARGUMENT, "block_table rows overlap (stride below cols)");
+  if ((int64_t)kv->block_table_cols * kv->page_size < table_keys)
+    return fail(FA_ERR_INVALID_ARGUMENT, "block_table has fewer pages per sequence than seqlen_k needs");
+  const int64_t kvvec = 16 / (int64_t)dtype_bytes(q->kv_dtype);
+  if (kv->k_page_stride < 0 || kv->v_page_stride < 0 || kv->k_page_stride % kvvec || kv->v_page_stride % kvvec)
+    return fail(FA_ERR_INVALID_ARGUMENT, "page strides must be non-negative multiples of 16 bytes");
+  return FA_OK;
+}
+
+fa_status validate_shared(const fa_fwd_params* p, const fa_paged_kv* kv, const fa_shared_prefix* s, fa_fwd_params* q) {
+  if (p == nullptr || kv == nullptr || s == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (s->max_prefix_len < 0 || s->max_suffix_len < 0 || s->num_groups < 0)
+    return fail(FA_ERR_INVALID_ARGUMENT, "sizes must be non-negative");
+  // (positions of keys, and of the end of a last partition behind them, stay below 2^31)
+  if (s->max_prefix_len > (1 << 29) || s->max_suffix_len > (1 << 29))
+    return fail(FA_ERR_UNSUPPORTED, "max_prefix_len and max_suffix_len must be at most 2^29");
+  if (s->split_len < 0 || s->split_len % 64 != 0 || s->split_len > (1 << 29))
+    return fail(FA_ERR_INVALID_ARGUMENT, "split_len must be a positive multiple of 64, at most 2^29 (or 0)");
+  if (s->cu_groups != nullptr && s->num_groups == 0) return fail(FA_ERR_INVALID_ARGUMENT, "cu_groups needs a group");
+  if (s->cu_groups == nullptr && s->num_groups > 1) return fail(FA_ERR_INVALID_ARGUMENT, "several groups need cu_groups");
+  if (!aligned(s->prefix_lens, 4) || !aligned(s->cu_groups, 4))
+    return fail(FA_ERR_INVALID_ARGUMENT, "prefix_lens and cu_groups must be 4-byte aligned");
+  *q = *p;
+  q->seqlen_k = kv->num_pages > 0 ? 1 : 0;  // (whether the pools' pointers have to be there)
+  fa_status st = validate_paged(q, kv, 64, 0);
+  if (st != FA_OK) return st;
+  if (q->batch == 0 || q->seqlen_q == 0) return FA_OK;
+  if (s->num_groups > q->batch && s->cu_groups != nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "more groups than requests");
+  if (const char* why = fa::shared_refusal(*q, *kv, *s)) return fail(FA_ERR_UNSUPPORTED, why);
+  return FA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -348,35 +406,8 @@ fa_status fa_attention_paged_decode(const fa_fwd_params* p, const fa_paged_kv* k
   g_last_error.clear();
   if (p == nullptr || kv == nullptr) return fail(FA_ERR_INVALID_ARGUMENT, "params is NULL");
   fa_fwd_params q = *p;
-  q.k_stride_b = q.v_stride_b = 0;  // keys are found through the block table
-  fa_status st = validate(&q, /*varlen=*/false, /*fp8_ok=*/true, /*generic_ok=*/false);
-  if (st != FA_OK) return st;
-  if (q.lse != nullptr && (q.lse_stride_b < 0 || q.lse_stride_h < 0))
-    return fail(FA_ERR_INVALID_ARGUMENT, "negative LSE stride");
-  if (split_len <= 0 || split_len % 64 != 0)
-    return fail(FA_ERR_INVALID_ARGUMENT, "split_len must be a positive multiple of 64");
-  if (kv->page_size <= 0 || kv->page_size % 16 != 0)
-    return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be a positive multiple of 16");
-  if (kv->page_size > FA_MAX_PAGE_SIZE)
-    return fail(FA_ERR_INVALID_ARGUMENT, "page_size must be at most 2^24 keys");
-  const bool fp8 = q.kv_dtype == FA_DTYPE_FP8_E4M3;
-  if (fp8 && kv->page_size % 64 != 0)
-    return fail(FA_ERR_INVALID_ARGUMENT, "FP8 pools need page_size a multiple of 64 (64-key scale blocks)");
-  if (fp8 && (q.scale_stride_b < 0 || q.scale_stride_h < 0))
-    return fail(FA_ERR_INVALID_ARGUMENT, "negative FP8 scale stride");
-  if (kv->num_pages < 0 || kv->block_table_cols < 0) return fail(FA_ERR_INVALID_ARGUMENT, "negative page count");
-  if (q.batch == 0 || q.seqlen_q == 0) return FA_OK;
-  if (kv->block_table == nullptr || kv->seqlens_k == nullptr)
-    return fail(FA_ERR_INVALID_ARGUMENT, "block_table and seqlens_k must be non-NULL");
-  if (!aligned(kv->block_table, 4) || !aligned(kv->seqlens_k, 4))
-    return fail(FA_ERR_INVALID_ARGUMENT, "block_table and seqlens_k must be 4-byte aligned");
-  if (q.batch > 1 && kv->block_table_stride < kv->block_table_cols)
-    return fail(FA_ERR_INVALID_ARGUMENT, "block_table rows overlap (stride below cols)");
-  if ((int64_t)kv->block_table_cols * kv->page_size < q.seqlen_k)
-    return fail(FA_ERR_INVALID_ARGUMENT, "block_table has fewer pages per sequence than seqlen_k needs");
-  const int64_t kvvec = 16 / (int64_t)dtype_bytes(q.kv_dtype);
-  if (kv->k_page_stride < 0 || kv->v_page_stride < 0 || kv->k_page_stride % kvvec || kv->v_page_stride % kvvec)
-    return fail(FA_ERR_INVALID_ARGUMENT, "page strides must be non-negative multiples of 16 bytes");
+  fa_status st = validate_paged(&q, kv, split_len, q.seqlen_k);
+  if (st != FA_OK || q.batch == 0 || q.seqlen_q == 0) return st;
   const int32_t splits = q.seqlen_k > 0 ? (q.seqlen_k + split_len - 1) / split_len : 1;
   const size_t need = fa_splitk_workspace_bytes(q.batch, q.heads_q, q.seqlen_q, q.head_dim, splits);
   if (workspace == nullptr || workspace_bytes < need) {
@@ -388,6 +419,32 @@ fa_status fa_attention_paged_decode(const fa_fwd_params* p, const fa_paged_kv* k
   if (!aligned(workspace, 16)) return fail(FA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   const char* err = nullptr;
   st = fa::run_splitk(q, split_len, workspace, reinterpret_cast<hipStream_t>(stream), &err, kv);
+  if (st != FA_OK) return fail(st, err ? err : "launch failed");
+  return FA_OK;
+}
+
+size_t fa_shared_prefix_workspace_bytes(const fa_fwd_params* p, const fa_paged_kv* kv, const fa_shared_prefix* s) {
+  g_last_error.clear();
+  fa_fwd_params q;
+  if (validate_shared(p, kv, s, &q) != FA_OK || q.batch == 0 || q.seqlen_q == 0) return 0;
+  return fa::shared_workspace_bytes(q, *kv, *s);
+}
+
+fa_status fa_attention_shared_prefix(const fa_fwd_params* p, const fa_paged_kv* kv, const fa_shared_prefix* s,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  fa_fwd_params q;
+  fa_status st = validate_shared(p, kv, s, &q);
+  if (st != FA_OK || q.batch == 0 || q.seqlen_q == 0) return st;
+  const size_t need = fa::shared_workspace_bytes(q, *kv, *s);
+  if (workspace == nullptr || workspace_bytes < need) {
+    char buf[160];
+    snprintf(buf, sizeof(buf), "workspace too small: need %zu bytes, got %zu", need, workspace == nullptr ? (size_t)0 : workspace_bytes);
+    return fail(FA_ERR_WORKSPACE, buf);
+  }
+  if (!aligned(workspace, 16)) return fail(FA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  const char* err = nullptr;
+  st = fa::run_shared(q, *kv, *s, workspace, reinterpret_cast<hipStream_t>(stream), &err);
   if (st != FA_OK) return fail(st, err ? err : "launch failed");
   return FA_OK;
 }

@@ -1,0 +1,107 @@
+// Requests in groups that share the start of their keys: which keys of a request are read once for its group.
+//
+// The kernels split a group's prefix at a multiple of kPrefixUnit keys: the keys below it (the "shared" ones) are read
+// for all rows of the group at once, those from it on through each request's own block-table row.  64 keys are a whole
+// tile, a whole FP8 scale block and whole page groups of every page size, so both parts address memory as an unsplit
+// sequence would.
+#pragma once
+
+#include "fa_device.hpp"
+
+namespace fa {
+
+constexpr int kPrefixUnit = 64;
+
+struct SharedArgs {
+  const int32_t* prefix_lens;  // [groups], or NULL: max_prefix for every group
+  const int32_t* cu_groups;    // [groups + 1], or NULL: one group of the whole batch
+  int32_t groups, batch;
+  int32_t max_prefix, max_suffix;  // bounds of the shared keys, and of a request's keys behind them
+  int32_t table_keys;              // keys that a block-table row can name
+  int32_t part_base, part_stride;  // a row's partials: part_stride of them, these ones from part_base on
+};
+
+// Shared keys of group g (in range).
+__device__ __forceinline__ int shared_keys(const SharedArgs& s, int g) {
+  const int p = s.prefix_lens != nullptr ? min(max(s.prefix_lens[g], 0), s.max_prefix) : s.max_prefix;
+  return min(p, s.table_keys) / kPrefixUnit * kPrefixUnit;
+}
+
+// Requests [b0, b1) of group g (in range), within the batch whatever cu_groups holds.
+__device__ __forceinline__ void group_range(const SharedArgs& s, int g, int& b0, int& b1) {
+  b0 = 0;
+  b1 = s.batch;
+  if (s.cu_groups != nullptr) {
+    b0 = min(max(s.cu_groups[g], 0), s.batch);
+    b1 = min(max(s.cu_groups[g + 1], b0), s.batch);
+  }
+}
+
+// Shared keys of request b (uniform over the wave; every lane calls it).  A request of no group has none.
+__device__ __forceinline__ int shared_keys_of(const SharedArgs& s, int b) {
+  if (s.cu_groups == nullptr) return __builtin_amdgcn_readfirstlane(shared_keys(s, 0));
+  const int lane = (int)threadIdx.x & 63;
+  for (int base = 0; base < s.groups; base += 64) {
+    const int g = base + lane;
+    int b0 = 0, b1 = 0;
+    if (g < s.groups) group_range(s, g, b0, b1);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(b0 <= b && b < b1);
+    if (in != 0) return __builtin_amdgcn_readfirstlane(shared_keys(s, base + __builtin_ctzll(in)));
+  }
+  return 0;
+}
+
+// The group of row block `rb` and the block within it, when a group of n requests has ceil(n * rows_each / rows) blocks
+// (uniform; every lane calls it).  False past the last block.
+__device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_each, int rows, int& rb, int& g, int& b0, int& b1) {
+  const int lane = (int)threadIdx.x & 63;
+  if (s.cu_groups == nullptr) {
+    g = b0 = 0;
+    b1 = s.batch;
+    return rb < (s.batch * rows_each + rows - 1) / rows;
+  }
+  for (int base = 0; base < s.groups; base += 64) {
+    int lo = 0, hi = 0;
+    if (base + lane < s.groups) group_range(s, base + lane, lo, hi);
+    const int blocks = ((hi - lo) * rows_each + rows - 1) / rows;
+    int end = blocks;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int left = __shfl_up(end, d);
+      end += lane >= d ? left : 0;
+    }
+    const uint64_t in = __builtin_amdgcn_ballot_w64(end > rb);
+    if (in != 0) {
+      const int at = __builtin_ctzll(in);
+      g = base + at;
+      b0 = __builtin_amdgcn_readlane(lo, at);
+      b1 = __builtin_amdgcn_readlane(hi, at);
+      rb -= __builtin_amdgcn_readlane(end - blocks, at);
+      return true;
+    }
+    rb -= __builtin_amdgcn_readlane(end, 63);
+  }
+  return false;
+}
+
+// The request of [b0, b1) whose block-table row names the group's shared keys: the first that holds them all, or else
+// (no row sees more) the first of the longest (uniform; every lane calls it).
+__device__ __forceinline__ int prefix_holder(const int32_t* seqlens, int b0, int b1, int keys) {
+  const int lane = (int)threadIdx.x & 63;
+  int best = b0, most = -1;
+  for (int base = b0; base < b1; base += 64) {
+    int n = base + lane < b1 ? min(seqlens[base + lane], keys) : -1;
+    int top = n;
+#pragma unroll
+    for (int d = 32; d >= 1; d /= 2) top = max(top, __shfl_xor(top, d));
+    top = __builtin_amdgcn_readfirstlane(top);
+    if (top > most) {
+      most = top;
+      best = base + __builtin_ctzll(__builtin_amdgcn_ballot_w64(n == top));
+      if (most >= keys) break;
+    }
+  }
+  return best;
+}
+
+}  // namespace fa

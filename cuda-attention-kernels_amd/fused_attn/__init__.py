@@ -14,6 +14,7 @@ from .pages import allocate_pages, append_kv_paged, release_pages
 from .paged import attention_paged, attention_paged_reference, paged_from_dense, paged_from_dense_fp8, \
     paged_from_dense_int4
 from .reference import attention_reference, attention_varlen_reference
+from .shared_prefix import attention_shared_prefix
 from .splitk import attention_splitk, attention_splitk_triton, choose_num_splits
 
 __all__ = [
@@ -35,6 +36,7 @@ __all__ = [
     "paged_from_dense",
     "paged_from_dense_fp8",
     "paged_from_dense_int4",
+    "attention_shared_prefix",
     "allocate_pages",
     "release_pages",
     "append_kv_paged",

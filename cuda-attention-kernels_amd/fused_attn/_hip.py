@@ -122,6 +122,19 @@ class PagedKV(ctypes.Structure):
     ]
 
 
+class SharedPrefix(ctypes.Structure):
+    """Mirror of ``fa_shared_prefix`` (include/fused_attn_hip.h)."""
+
+    _fields_ = [
+        ("prefix_lens", ctypes.c_void_p),
+        ("cu_groups", ctypes.c_void_p),
+        ("num_groups", ctypes.c_int32),
+        ("max_prefix_len", ctypes.c_int32),
+        ("max_suffix_len", ctypes.c_int32),
+        ("split_len", ctypes.c_int32),
+    ]
+
+
 def _int64s(*names: str) -> list:
     return [(n, ctypes.c_int64) for n in names]
 
@@ -366,6 +379,11 @@ def _bind(lib: ctypes.CDLL) -> None:
             f.argtypes, f.restype = [ctypes.POINTER(PagesParams), ctypes.c_void_p], ctypes.c_int
         lib.fa_append_kv_paged.argtypes = [ctypes.POINTER(AppendPagedParams), ctypes.c_void_p]
         lib.fa_append_kv_paged.restype = ctypes.c_int
+        shared = [P, ctypes.POINTER(PagedKV), ctypes.POINTER(SharedPrefix)]
+        lib.fa_shared_prefix_workspace_bytes.argtypes = shared
+        lib.fa_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
+        lib.fa_attention_shared_prefix.argtypes = [*shared, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.fa_attention_shared_prefix.restype = ctypes.c_int
     lib.fa_device_supported.argtypes = [ctypes.c_int32]
     lib.fa_device_supported.restype = ctypes.c_int32
     lib.fa_last_error.argtypes = []
@@ -909,6 +927,65 @@ def paged_decode(q, k_cache, v_cache, block_table, seqlens_k, max_seqlen_k: int,
                                              ctypes.c_void_p(workspace.data_ptr()),
                                              workspace.numel() * workspace.element_size(),
                                              ctypes.c_void_p(_stream(q))), "attention_paged_decode")
+    return (o, lse) if return_lse else o
+
+
+def check_shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups) -> None:
+    if k_cache.dtype == torch.uint8:
+        raise RuntimeError("attention_shared_prefix takes 16-bit and FP8 pools, not 4-bit ones")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    _check_qkv(q, k_cache, v_cache, "paged", kv_fp8=k_cache.dtype == _FP8)
+    b = q.shape[0]
+    check_block_table(block_table, b)
+    check_lengths(seqlens_k, b)
+    groups = 1
+    if cu_groups is not None:
+        if cu_groups.dtype != torch.int32 or cu_groups.dim() != 1 or not 2 <= cu_groups.numel() <= max(b, 1) + 1:
+            raise RuntimeError(f"cu_groups must be int32 [G + 1] of 1 to {b} groups, got {cu_groups.dtype} {tuple(cu_groups.shape)}")
+        groups = cu_groups.numel() - 1
+    if isinstance(prefix_lens, torch.Tensor):
+        if prefix_lens.dtype != torch.int32 or tuple(prefix_lens.shape) != (groups,):
+            raise RuntimeError(f"prefix_lens must be a number or int32 [{groups}], got {prefix_lens.dtype} {tuple(prefix_lens.shape)}")
+    for t in (k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups):
+        if isinstance(t, torch.Tensor) and t.device != q.device:
+            raise RuntimeError(f"all tensors must be on {q.device}, got {t.device}")
+
+
+def shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups, max_prefix_len: int,
+                  max_suffix_len: int, causal: bool = False, scale: Optional[float] = None, split_len: Optional[int] = None,
+                  return_lse: bool = False, k_scale=None, v_scale=None):
+    """Attention over a paged cache whose requests share prefixes; operands checked by ``check_shared_prefix``."""
+    fp8 = k_cache.dtype == _FP8
+    if fp8:
+        _check_paged_fp8_scales(k_cache, k_scale, v_scale)
+    if split_len is not None and int(split_len) <= 0:
+        raise RuntimeError(f"split_len must be a positive multiple of 64, got {split_len}")
+    _require_gpu(q, k_cache, v_cache, block_table, seqlens_k)
+    lib = _pages_library()
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    q, k_cache, v_cache = _prep_qkv(q, k_cache, v_cache, kv_fp8=fp8)
+    if fp8:
+        k_scale, v_scale = _prep_fp8_scales(k_cache, k_scale, v_scale)
+    bt, sl = _plain_table(block_table), seqlens_k.contiguous()
+    o = _new_output(q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+    p = make_params(q, k_cache, v_cache, o, causal, scale, lse=lse, k_scale=k_scale if fp8 else None,
+                    v_scale=v_scale if fp8 else None)
+    p.k_stride_b = p.v_stride_b = 0
+    kv = PagedKV(bt.data_ptr(), bt.stride(0), bt.shape[1], k_cache.shape[2], sl.data_ptr(), k_cache.shape[0], 0,
+                 _stride(k_cache, 0), _stride(v_cache, 0))
+    if prefix_lens is not None:
+        prefix_lens = prefix_lens.contiguous()
+    if cu_groups is not None:
+        cu_groups = cu_groups.contiguous()
+    s = SharedPrefix(None if prefix_lens is None else prefix_lens.data_ptr(), None if cu_groups is None else cu_groups.data_ptr(),
+                     1 if cu_groups is None else cu_groups.numel() - 1, max_prefix_len, max_suffix_len,
+                     0 if split_len is None else int(split_len))
+    need = lib.fa_shared_prefix_workspace_bytes(p, kv, s)
+    ws = torch.empty(need // 4 + 4, dtype=torch.float32, device=q.device)
+    with _on_device(q.device):
+        _check(lib.fa_attention_shared_prefix(p, kv, s, ws.data_ptr(), need, _stream(q)), "attention_shared_prefix")
     return (o, lse) if return_lse else o
 
 

@@ -1,0 +1,70 @@
+"""Decode attention for requests that share the start of their context.
+
+Requests behind one system prompt, or parallel answers to one document, hold the same pages at the start of their
+block-table rows.  ``attention_paged`` reads those keys once per request; here a group's rows (requests x q-heads of a
+kv-head x queries) meet them together, as the rows of one matrix product, and each request's own keys behind them as in
+``attention_paged``.  Both parts' partials are merged by their log-sum-exps, so the result is that of
+
+    attention_paged(q, k_cache, v_cache, block_table, seqlens_k, ...)
+
+up to the rounding of another order of sums.  The reference package has no paged cache.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Union
+
+import torch
+
+from . import _hip
+from .ops import _pick_backend
+from .paged import attention_paged
+
+
+def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                            seqlens_k: torch.Tensor, prefix_lens: Union[int, torch.Tensor],
+                            cu_groups: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None,
+                            max_prefix_len: Optional[int] = None, max_suffix_len: Optional[int] = None,
+                            split_len: Optional[int] = None, return_lse: bool = False,
+                            k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+    """Attention of q [B, Hq, Nq, D] (fp16/bf16, D in {64, 128, 256}) over a paged cache, 16-bit or FP8, whose requests
+    share prefixes.  ``block_table``, ``seqlens_k`` (all keys of a request, the shared ones among them), ``causal``,
+    ``scale``, ``return_lse`` and the FP8 pools' ``k_scale`` / ``v_scale`` are those of ``attention_paged``.
+
+    Group g is the requests ``cu_groups[g]`` to ``cu_groups[g + 1] - 1`` (int32 [G + 1] from 0 to B; None: one group, the
+    whole batch), whose rows name the same keys in their first ``prefix_lens[g]`` positions (int32 [G], or one number for
+    every group).  A prefix may be 0, need not fill whole pages, and a request may be shorter than it (a padded batch's
+    empty ones among them).
+
+    ``max_prefix_len`` and ``max_suffix_len`` size the grid: the largest of prefix_lens, and of a request's keys behind
+    its group's prefix.  When omitted they are read from the device, which waits for it; as numbers, they let the call be
+    captured into a graph.  Longer prefixes than max_prefix_len are shared up to it; keys past max_suffix_len of their
+    own are not read.  ``split_len``: keys per partition, a multiple of 64."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    number = not isinstance(prefix_lens, torch.Tensor)
+    _hip.check_shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups)
+    if not q.is_cuda or _pick_backend(q) != "hip":
+        return attention_paged(q, k_cache, v_cache, block_table, seqlens_k, causal=causal, scale=scale, return_lse=return_lse,
+                               k_scale=k_scale, v_scale=v_scale)
+    if max_prefix_len is None:
+        max_prefix_len = prefix_lens if number else int(prefix_lens.max().item()) if prefix_lens.numel() else 0
+    if max_suffix_len is None:
+        max_suffix_len = _longest_suffix(seqlens_k, prefix_lens, cu_groups)
+    if number:  # (the kernels hold every group's prefix to max_prefix_len)
+        max_prefix_len, prefix_lens = min(int(max_prefix_len), int(prefix_lens)), None
+    return _hip.shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups, max(0, int(max_prefix_len)),
+                              max(0, int(max_suffix_len)), causal=causal, scale=scale, split_len=split_len,
+                              return_lse=return_lse, k_scale=k_scale, v_scale=v_scale)
+
+
+def _longest_suffix(seqlens_k: torch.Tensor, prefix_lens, cu_groups: Optional[torch.Tensor]) -> int:
+    if seqlens_k.numel() == 0:
+        return 0
+    if isinstance(prefix_lens, torch.Tensor):
+        p = prefix_lens.long().clamp(min=0)
+        if cu_groups is not None:
+            request = torch.arange(seqlens_k.numel(), device=seqlens_k.device)
+            p = p[torch.searchsorted(cu_groups[1:].long().contiguous(), request, right=True).clamp(max=p.numel() - 1)]
+    else:
+        p = max(0, int(prefix_lens))
+    return max(0, int((seqlens_k.long() - p).max().item()))

@@ -186,6 +186,24 @@ typedef struct fa_paged_kv {
 fa_status fa_attention_paged_decode(const fa_fwd_params* p, const fa_paged_kv* kv, int32_t split_len,
                                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention over a paged cache for requests that share the start of their keys: fa_attention_paged_decode's result, with
+   a group's shared keys read once for all its rows.  Group g is requests cu_groups[g] to cu_groups[g + 1] - 1, and their
+   block-table rows name the same keys in the first prefix_lens[g] positions.  p->seqlen_k is unused: the grid is laid out
+   for max_prefix_len shared keys and max_suffix_len keys behind them, which bound prefix_lens[g] and
+   seqlens_k[b] - prefix_lens[g] (larger values are read as these bounds allow).  A request may be shorter than its group's
+   prefix, and then sees the keys that it has. */
+typedef struct fa_shared_prefix {
+  const int32_t* prefix_lens; /* [num_groups] on the device, or NULL: max_prefix_len for every group */
+  const int32_t* cu_groups;   /* [num_groups + 1] on the device, from 0 to batch, ascending; NULL: one group, the batch */
+  int32_t num_groups;
+  int32_t max_prefix_len, max_suffix_len;
+  int32_t split_len; /* keys per partition, a positive multiple of 64, or 0 for the library's choice */
+} fa_shared_prefix;
+/* Bytes of workspace (16-byte aligned).  0 for parameters that the call would refuse, and without a batch or queries. */
+size_t fa_shared_prefix_workspace_bytes(const fa_fwd_params* p, const fa_paged_kv* kv, const fa_shared_prefix* s);
+fa_status fa_attention_shared_prefix(const fa_fwd_params* p, const fa_paged_kv* kv, const fa_shared_prefix* s,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* Reference split heuristic (fused_attn/triton_splitk.py:130-137):
    min(2*num_cus / (batch*heads), seqlen_k / 256, 64), 1 for seqlen_q > 64. */
 int32_t fa_choose_num_splits(int32_t batch, int32_t heads, int32_t seqlen_k, int32_t seqlen_q, int32_t num_cus);
