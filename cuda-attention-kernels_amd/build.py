@@ -22,7 +22,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB_OUT = os.path.join(HERE, "fused_attn", "libfused_attn_hip.so")
 SOURCES = ["fa_prefill.hip", "fa_prefill_f32.hip", "fa_splitk.hip", "fa_generic.hip", "fa_quant.hip", "fa_int4.hip",
-           "fa_cache.hip", "fa_evict.hip", "fa_pages.hip", "fa_abi.cpp"]
+           "fa_cache.hip", "fa_evict.hip", "fa_pages.hip", "fa_shared.hip",
+           "fa_abi.cpp"]
 # the matrix-core ceiling probe bench.py times beside the prefill workload: a library of its own
 PROBE_SOURCES = ["fa_ceiling.hip"]
 PROBE_OUT = os.path.join(HERE, "fused_attn", "libfa_probe.so")

@@ -181,6 +181,8 @@ int splitk_waves_for_rows(int rows);
 
 // TileArgs fields that prefill and split-K share (pointers, strides, heads, scale).
 TileArgs common_args(const fa_fwd_params& p);
+// and those of paged K/V.
+void paged_args(TileArgs& a, const fa_paged_kv& kv);
 
 inline fa_status hip_status(hipError_t e, const char** err) {
   if (e == hipSuccess) return FA_OK;
@@ -226,13 +228,14 @@ fa_status run_append_paged(const fa_append_paged_params& p, hipStream_t stream, 
 fa_status run_splitk(const fa_fwd_params& p, int32_t split_len, void* workspace, hipStream_t stream,
                      const char** err, const fa_paged_kv* kv = nullptr);
 
-// Attention behind shared prefixes (fa_splitk.hip): how a call is cut up.
+// Attention behind shared prefixes (fa_shared.hip): how a call is cut up.
 struct SharedPlan {
   int32_t max_prefix, max_suffix;      // bounds of the shared keys, and of a request's keys behind them
   int32_t prefix_split, suffix_split;  // keys per partition
   int32_t prefix_parts, suffix_parts;  // partitions
   int32_t prefix_waves, suffix_waves;  // waves (of 32 rows) per workgroup
   int64_t prefix_blocks;               // row blocks of all groups, at most
+  bool fused;                          // both parts in one launch
 };
 SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int page_size);
 // Why a call of valid parameters cannot be launched, or NULL.

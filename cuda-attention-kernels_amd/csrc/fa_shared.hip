@@ -1,0 +1,276 @@
+// Attention of requests that share the start of their keys (gfx950).
+//
+// A group's shared keys meet the rows of all its requests (requests x q-heads of a kv-head x queries) as one product: the
+// pipelined prefill kernel over pages (attn_fwd_kernel, SHARED), 128 rows a workgroup, the keys cut into partitions.  The
+// requests' own keys go through the split-K kernel, a partition of one request's a workgroup.  Every (row, partition) of
+// either part leaves a partial, normalised by its own row sum, with its (max, sum); one kernel merges a row's:
+//   m = max_s m_s;  w_s = 2^(m_s - m) l_s;  O = sum_s w_s O_s / sum_s w_s   (0 when the sum is 0)
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "fa_prefill_kernel.hpp"
+#include "fa_shared.hpp"
+
+namespace fa {
+
+struct MergeArgs {
+  const float* part;  // [batch, hq, nq, part_stride] partials, then their (m, l) in ml
+  const float* ml;
+  void* o;
+  float* lse;  // optional natural-log LSE
+  int64_t sob, soh, son, slb, slh;
+  const int32_t* seqlens;
+  int32_t hq, nq, chunks;  // chunks: workgroups a request
+  SharedArgs shared;
+};
+
+// A thread merges 4 values of a row over every WAYS-th of its partials, CH of them in flight together; WAYS threads meet
+// in LDS.  A workgroup's rows are one request's, so that its group and its partitions are found once, uniformly.
+template <int D, class E, int WAYS>
+__global__ void __launch_bounds__(256) shared_merge_kernel(const MergeArgs a) {
+  constexpr int TPR = D / 4, ROWS = 256 / (TPR * WAYS), CH = 8;
+  static_assert(ROWS >= 1, "a row per workgroup at least");
+  constexpr float NEG_INF = -__builtin_inff();
+  __shared__ f32x4 s_acc[WAYS > 1 ? 256 : 1];
+  __shared__ f32x2 s_ml[WAYS > 1 ? ROWS * WAYS : 1];
+  const int b = (int)(blockIdx.x / (uint32_t)a.chunks), chunk = (int)(blockIdx.x - (uint32_t)b * (uint32_t)a.chunks);
+  const int tid = (int)threadIdx.x, dq = tid % TPR, way = tid / TPR % WAYS, sub = tid / (TPR * WAYS);
+  const int rows = a.hq * a.nq, r = chunk * ROWS + sub;  // (q-head, query) of the request
+  const int shared = shared_keys_of(a.shared, b);
+  const int keys = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens[b]), shared);
+  const int first = (shared + a.shared.prefix_split - 1) / a.shared.prefix_split;
+  const int count = r < rows ? first + (keys > shared ? (keys - shared + a.shared.suffix_split - 1) / a.shared.suffix_split : 0) : 0;
+  const int skip = a.shared.part_base - first;  // places between the two runs of a row's partials
+  const int64_t base = ((int64_t)b * rows + min(r, rows - 1)) * a.shared.part_stride;
+  const float* ml = a.ml + base * 2;
+  const float* op = a.part + base * D + 4 * dq;
+  float m = NEG_INF, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = way; s0 < count; s0 += CH * WAYS) {
+    f32x2 st[CH];
+    f32x4 pv[CH];
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      int s = s0 + u * WAYS;
+      st[u] = f32x2{NEG_INF, 0.f};
+      pv[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s < count) {
+        s += s >= first ? skip : 0;
+        st[u] = __builtin_bit_cast(f32x2, ld8(ml + 2 * s));
+        pv[u] = __builtin_bit_cast(f32x4, ld16(op + (int64_t)s * D));
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) mn = fmaxf(mn, st[u][0]);
+    const float m_ref = (mn == NEG_INF) ? 0.f : mn;
+    const float alpha = fast_exp2(m - m_ref);  // 0 while m = -inf
+    l *= alpha;
+    acc *= alpha;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const float w = fast_exp2(st[u][0] - m_ref) * st[u][1];
+      l += w;
+      acc += w * pv[u];
+    }
+    m = mn;
+  }
+  if constexpr (WAYS > 1) {
+    s_acc[tid] = acc;
+    if (dq == 0) s_ml[sub * WAYS + way] = f32x2{m, l};
+    __syncthreads();
+    if (way > 0) return;
+    float mn = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < WAYS; ++w) mn = fmaxf(mn, s_ml[sub * WAYS + w][0]);
+    const float m_ref = (mn == NEG_INF) ? 0.f : mn;
+    m = mn;
+    l = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAYS; ++w) {
+      const float f = fast_exp2(s_ml[sub * WAYS + w][0] - m_ref);
+      l += f * s_ml[sub * WAYS + w][1];
+      acc += f * s_acc[(sub * WAYS + w) * TPR + dq];
+    }
+  }
+  if (r >= rows) return;
+  const float l_safe = (l == 0.f) ? 1.f : l, inv = 1.f / l_safe;
+  const int h = r / a.nq, n = r - h * a.nq;
+  if (a.lse != nullptr && dq == 0) a.lse[b * a.slb + (int64_t)h * a.slh + n] = (m + __log2f(l_safe)) * kLn2;
+  uint16_t* o = (uint16_t*)a.o + b * a.sob + (int64_t)h * a.soh + (int64_t)n * a.son + 4 * dq;
+  st8(o, u32x2{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv)});
+}
+
+// ------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------
+
+namespace {
+
+constexpr int prefix_tile_keys(int d) { return d == 256 ? 32 : 64; }
+
+template <int D, class E>
+hipError_t launch_tiles(const SharedTileArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((attn_fwd_kernel<D, E, 4, prefix_tile_keys(D), false, true>), dim3((unsigned)a.total), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int D, class E, int WAYS>
+hipError_t launch_merge_ways(MergeArgs a, int batch, hipStream_t stream) {
+  constexpr int ROWS = 256 / (D / 4 * WAYS);
+  a.chunks = (a.hq * a.nq + ROWS - 1) / ROWS;
+  hipLaunchKernelGGL((shared_merge_kernel<D, E, WAYS>), dim3((unsigned)a.chunks * (unsigned)batch), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int D, class E>
+hipError_t launch_merge(const MergeArgs& a, int batch, int parts, hipStream_t stream) {
+  if (parts <= 8) return launch_merge_ways<D, E, 1>(a, batch, stream);
+  return launch_merge_ways<D, E, 4>(a, batch, stream);
+}
+
+}  // namespace
+
+SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int page_size) {
+  const int group = p.heads_q / p.heads_kv, rows = group * p.seqlen_q;
+  SharedPlan plan{};
+  plan.max_prefix = s.max_prefix_len / kPrefixUnit * kPrefixUnit;
+  // (a prefix is cut at whole units: up to 63 of its keys go with each request's own)
+  plan.max_suffix = s.max_suffix_len + kPrefixUnit - 1;
+  const int64_t all_rows = (int64_t)p.batch * rows;
+  const bool fp8 = p.kv_dtype == FA_DTYPE_FP8_E4M3;
+  plan.fused = !fp8;
+  plan.prefix_waves = fp8 ? splitk_waves_for_rows((int)std::min<int64_t>(all_rows, 1024)) : 4;
+  plan.suffix_waves = splitk_waves_for_rows(rows);
+  // (one group: exactly; several: each may leave a block unfilled, and the workgroups past the last block return)
+  const int64_t block = plan.prefix_waves * 32;
+  const int64_t group_blocks = s.num_groups > 1 ? all_rows / block + s.num_groups : (all_rows + block - 1) / block;
+  plan.prefix_blocks = group_blocks;
+  // Partitions.  A workgroup of the shared keys costs about 8 us before and after its tiles (64 keys in about 1 us at
+  // D = 128, alone on its CU or one of two) and leaves 128 rows of partials; one a CU leaves the CU's other place to the
+  // requests' own keys.  So: as many as there are CUs, half as many where those would have fewer than 1024 keys each (64
+  // requests of 4 rows, 8 kv-heads, 8192 keys: the call takes 42 us at 512 keys, 37 at 1024; 32 of 16 rows, 16384 keys, 66
+  // at 2048 and 86 at 4096).  Own keys: 1024 waves, four a CU, but no more than kLongest keys each, for the last to start
+  // not to run on alone (256 requests of up to 1000 keys, D = 64: 95 us whole, 91 in two).
+  constexpr int64_t kWgs = 256, kLong = 1024, kWaves = 1024, kLongest = 576;
+  auto whole = [](int64_t keys, int64_t parts) { return ((keys + parts - 1) / parts + kPrefixUnit - 1) / kPrefixUnit * kPrefixUnit; };
+  auto fits = [&](int64_t len, int64_t pages) {  // a partition spans a limited number of pages
+    return (int32_t)std::max<int64_t>(kPrefixUnit, std::min(len, (pages - 2) * page_size / kPrefixUnit * kPrefixUnit));
+  };
+  const int64_t prefix_items = p.heads_kv * ((all_rows + block - 1) / block);
+  int64_t len = whole(plan.max_prefix, std::max<int64_t>(1, (plan.fused ? kWgs : 2 * kWgs) / prefix_items));
+  if (plan.fused && len < kLong) len = std::min(kLong, whole(plan.max_prefix, std::max<int64_t>(1, kWgs / 2 / prefix_items)));
+  plan.prefix_split = s.split_len > 0 ? s.split_len : fits(len, plan.fused ? kPrefixPages : 256);
+  const int64_t suffix_items = (int64_t)p.batch * p.heads_kv * ((rows + 31) / 32);
+  len = std::min(kLongest, whole(plan.max_suffix, std::max<int64_t>(1, kWaves / suffix_items)));
+  plan.suffix_split = s.split_len > 0 ? s.split_len : fits(len, 256);
+  plan.prefix_parts = (plan.max_prefix + plan.prefix_split - 1) / plan.prefix_split;
+  plan.suffix_parts = (plan.max_suffix + plan.suffix_split - 1) / plan.suffix_split;
+  return plan;
+}
+
+const char* shared_refusal(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_shared_prefix& s) {
+  const SharedPlan plan = plan_shared(p, s, kv.page_size);
+  const int64_t rows = (int64_t)p.heads_q / p.heads_kv * p.seqlen_q;
+  auto slots = [&](int64_t len) { return (len - 1) / kv.page_size + 2; };
+  if (slots(plan.prefix_split) > (plan.fused ? kPrefixPages : 256) || slots(plan.suffix_split) > 256)
+    return "split_len too long for the page size: a partition may span at most 128 pages of 16-bit rows, 256 of FP8 ones";
+  const int64_t out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
+  const int64_t row_blocks = (rows + plan.suffix_waves * 32 - 1) / (plan.suffix_waves * 32);
+  if (out_rows > INT32_MAX / 2 || plan.prefix_blocks * p.heads_kv * plan.prefix_parts > INT32_MAX ||
+      ((int64_t)p.batch * p.heads_kv * plan.suffix_parts + 8) * row_blocks > INT32_MAX)
+    return "grid too large";
+  return nullptr;
+}
+
+size_t shared_workspace_bytes(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_shared_prefix& s) {
+  const SharedPlan plan = plan_shared(p, s, kv.page_size);
+  return (size_t)p.batch * p.heads_q * p.seqlen_q * (size_t)(plan.prefix_parts + plan.suffix_parts) *
+         ((size_t)p.head_dim + 2) * sizeof(float);
+}
+
+fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_shared_prefix& s, void* workspace,
+                     hipStream_t stream, const char** err) {
+  const SharedPlan plan = plan_shared(p, s, kv.page_size);
+  const bool fp8 = p.kv_dtype == FA_DTYPE_FP8_E4M3, bf = p.dtype == FA_DTYPE_BF16;
+  const int64_t out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
+  const int stride = plan.prefix_parts + plan.suffix_parts;
+  SharedTileArgs a{};
+  static_cast<TileArgs&>(a) = common_args(p);
+  paged_args(a, kv);
+  a.o = workspace;
+  a.ml = (float*)workspace + out_rows * stride * p.head_dim;
+  a.batch = p.batch;
+  a.ppw = 1;
+  a.shared.prefix_lens = s.prefix_lens;
+  a.shared.cu_groups = s.cu_groups;
+  a.shared.groups = s.cu_groups != nullptr ? s.num_groups : 1;
+  a.shared.batch = p.batch;
+  a.shared.max_prefix = plan.max_prefix;
+  a.shared.max_suffix = plan.max_suffix;
+  a.shared.table_keys = (int32_t)std::min<int64_t>((int64_t)kv.block_table_cols * kv.page_size, INT32_MAX);
+  a.shared.part_stride = stride;
+  a.shared.part_base = plan.prefix_parts;
+  a.shared.prefix_split = plan.prefix_split;
+  a.shared.suffix_split = plan.suffix_split;
+  const int rows = a.group * p.seqlen_q;
+  const int64_t prefix_wgs = plan.prefix_blocks * p.heads_kv * plan.prefix_parts;
+  hipError_t e = hipSuccess;
+  if (plan.fused) {
+    a.shared.prefix_wgs = (int32_t)prefix_wgs;
+    a.n_rowblk = (int32_t)plan.prefix_blocks;
+    a.shared.suffix_blocks = (rows + 31) / 32;
+    a.shared.by_page = FastDiv::by(kv.page_size);
+    a.shared.by_hkv = FastDiv::by(p.heads_kv);
+    a.shared.by_group = FastDiv::by(a.group);
+    a.shared.by_nq = FastDiv::by(p.seqlen_q);
+    a.shared.by_batch = FastDiv::by(p.batch);
+    a.shared.by_prefix_blocks = FastDiv::by(a.n_rowblk);
+    a.shared.by_suffix_blocks = FastDiv::by(a.shared.suffix_blocks);
+    a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts * a.shared.suffix_blocks);
+    a.total = (int32_t)(a.shared.prefix_wgs + ((int64_t)a.n_items + 3) / 4);
+    e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) { return launch_tiles<decltype(d)::value, decltype(t)>(a, stream); });
+    if (e != hipSuccess) return hip_status(e, err);
+  } else {
+    if (plan.prefix_parts > 0) {
+      a.split_len = plan.prefix_split;
+      a.n_split = a.n_chunk = plan.prefix_parts;
+      a.nk = plan.max_prefix;
+      a.n_rowblk = (int32_t)plan.prefix_blocks;
+      a.total = (int32_t)prefix_wgs;
+      e = launch_shared_split(a, p.head_dim, bf, fp8, true, plan.prefix_waves, stream);
+      if (e != hipSuccess) return hip_status(e, err);
+    }
+    a.split_len = plan.suffix_split;
+    a.n_split = a.n_chunk = plan.suffix_parts;
+    a.nk = plan.max_suffix;
+    a.n_rowblk = (rows + plan.suffix_waves * 32 - 1) / (plan.suffix_waves * 32);
+    a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts);
+    a.total = (int32_t)(((int64_t)a.n_items + 7) / 8 * 8 * a.n_rowblk);
+    e = launch_shared_split(a, p.head_dim, bf, fp8, false, plan.suffix_waves, stream);
+    if (e != hipSuccess) return hip_status(e, err);
+  }
+
+  MergeArgs m{};
+  m.part = (const float*)a.o;
+  m.ml = a.ml;
+  m.o = p.o;
+  m.lse = p.lse;
+  m.sob = p.o_stride_b;
+  m.soh = p.o_stride_h;
+  m.son = p.o_stride_n;
+  m.slb = p.lse_stride_b;
+  m.slh = p.lse_stride_h;
+  m.seqlens = kv.seqlens_k;
+  m.hq = p.heads_q;
+  m.nq = p.seqlen_q;
+  m.shared = a.shared;
+  e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) {
+    return launch_merge<decltype(d)::value, decltype(t)>(m, p.batch, stride, stream);
+  });
+  return hip_status(e, err);
+}
+
+}  // namespace fa

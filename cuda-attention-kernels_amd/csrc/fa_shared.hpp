@@ -7,10 +7,24 @@
 #pragma once
 
 #include "fa_device.hpp"
+#include "fa_internal.hpp"
 
 namespace fa {
 
 constexpr int kPrefixUnit = 64;
+constexpr int kPrefixPages = 128;  // pages that a partition of the shared keys may span
+
+// Division of 0 <= n < 2^31 by a number that the host knows: (n * mul) >> shift.
+struct FastDiv {
+  uint32_t mul;
+  int32_t shift;
+  __host__ static FastDiv by(int32_t d) {
+    int lg = 0;
+    while ((int64_t{1} << lg) < (int64_t)d) ++lg;
+    return {(uint32_t)(((uint64_t{1} << (31 + lg)) + (uint64_t)d - 1) / (uint64_t)d), 31 + lg};
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
 
 struct SharedArgs {
   const int32_t* prefix_lens;  // [groups], or NULL: max_prefix for every group
@@ -18,13 +32,26 @@ struct SharedArgs {
   int32_t groups, batch;
   int32_t max_prefix, max_suffix;  // bounds of the shared keys, and of a request's keys behind them
   int32_t table_keys;              // keys that a block-table row can name
-  int32_t part_base, part_stride;  // a row's partials: part_stride of them, these ones from part_base on
+  int32_t part_base, part_stride;  // a row's partials: part_stride of them, those of its own keys from part_base on
+  int32_t prefix_split, suffix_split;  // keys per partition
+  int32_t suffix_blocks;               // blocks of 32 rows of a request
+  FastDiv by_page, by_hkv, by_group, by_nq, by_batch, by_prefix_blocks, by_suffix_blocks;
+  int32_t prefix_wgs;                  // workgroups of the shared keys; the ones behind them read the requests' own
+};
+
+struct SharedTileArgs : TileArgs {
+  SharedArgs shared;
 };
 
 // Shared keys of group g (in range).
 __device__ __forceinline__ int shared_keys(const SharedArgs& s, int g) {
   const int p = s.prefix_lens != nullptr ? min(max(s.prefix_lens[g], 0), s.max_prefix) : s.max_prefix;
   return min(p, s.table_keys) / kPrefixUnit * kPrefixUnit;
+}
+
+// Keys that request b is read to have, behind `shared` shared ones.
+__device__ __forceinline__ int keys_of(const SharedArgs& s, int seqlen, int shared) {
+  return min(max(seqlen, 0), min(shared + s.max_suffix, s.table_keys));
 }
 
 // Requests [b0, b1) of group g (in range), within the batch whatever cu_groups holds.
@@ -43,26 +70,33 @@ __device__ __forceinline__ int shared_keys_of(const SharedArgs& s, int b) {
   const int lane = (int)threadIdx.x & 63;
   for (int base = 0; base < s.groups; base += 64) {
     const int g = base + lane;
-    int b0 = 0, b1 = 0;
-    if (g < s.groups) group_range(s, g, b0, b1);
+    int b0 = 0, b1 = 0, keys = 0;
+    if (g < s.groups) {
+      group_range(s, g, b0, b1);
+      keys = shared_keys(s, g);  // (every lane its group's: the loads are in flight together)
+    }
     const uint64_t in = __builtin_amdgcn_ballot_w64(b0 <= b && b < b1);
-    if (in != 0) return __builtin_amdgcn_readfirstlane(shared_keys(s, base + __builtin_ctzll(in)));
+    if (in != 0) return __builtin_amdgcn_readlane(keys, __builtin_ctzll(in));
   }
   return 0;
 }
 
-// The group of row block `rb` and the block within it, when a group of n requests has ceil(n * rows_each / rows) blocks
-// (uniform; every lane calls it).  False past the last block.
-__device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_each, int rows, int& rb, int& g, int& b0, int& b1) {
+// The requests [b0, b1) and shared keys of the group that row block `rb` belongs to, and the block within it, when a group
+// of n requests has ceil(n * rows_each / rows) blocks (uniform; every lane calls it).  False past the last block.
+__device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_each, int rows, int& rb, int& b0, int& b1, int& keys) {
   const int lane = (int)threadIdx.x & 63;
   if (s.cu_groups == nullptr) {
-    g = b0 = 0;
+    b0 = 0;
     b1 = s.batch;
+    keys = __builtin_amdgcn_readfirstlane(shared_keys(s, 0));
     return rb < (s.batch * rows_each + rows - 1) / rows;
   }
   for (int base = 0; base < s.groups; base += 64) {
-    int lo = 0, hi = 0;
-    if (base + lane < s.groups) group_range(s, base + lane, lo, hi);
+    int lo = 0, hi = 0, k = 0;
+    if (base + lane < s.groups) {
+      group_range(s, base + lane, lo, hi);
+      k = shared_keys(s, base + lane);
+    }
     const int blocks = ((hi - lo) * rows_each + rows - 1) / rows;
     int end = blocks;
 #pragma unroll
@@ -73,7 +107,7 @@ __device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_eac
     const uint64_t in = __builtin_amdgcn_ballot_w64(end > rb);
     if (in != 0) {
       const int at = __builtin_ctzll(in);
-      g = base + at;
+      keys = __builtin_amdgcn_readlane(k, at);
       b0 = __builtin_amdgcn_readlane(lo, at);
       b1 = __builtin_amdgcn_readlane(hi, at);
       rb -= __builtin_amdgcn_readlane(end - blocks, at);
@@ -90,7 +124,9 @@ __device__ __forceinline__ int prefix_holder(const int32_t* seqlens, int b0, int
   const int lane = (int)threadIdx.x & 63;
   int best = b0, most = -1;
   for (int base = b0; base < b1; base += 64) {
-    int n = base + lane < b1 ? min(seqlens[base + lane], keys) : -1;
+    const int n = base + lane < b1 ? min(seqlens[base + lane], keys) : -1;
+    const uint64_t whole = __builtin_amdgcn_ballot_w64(n == keys);
+    if (whole != 0) return base + __builtin_ctzll(whole);
     int top = n;
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) top = max(top, __shfl_xor(top, d));
@@ -98,10 +134,20 @@ __device__ __forceinline__ int prefix_holder(const int32_t* seqlens, int b0, int
     if (top > most) {
       most = top;
       best = base + __builtin_ctzll(__builtin_amdgcn_ballot_w64(n == top));
-      if (most >= keys) break;
     }
   }
   return best;
+}
+
+// The split-K kernels over the shared keys (prefix) or the requests' own (fa_splitk.hip); nw: waves per workgroup.
+hipError_t launch_shared_split(const SharedTileArgs& a, int d, bool bf, bool fp8, bool prefix, int nw, hipStream_t stream);
+
+template <class F>
+hipError_t by_dim_and_type(int d, bool bf, F&& f) {
+  auto type = [&](auto dim) { return bf ? f(dim, BF16{}) : f(dim, F16{}); };
+  if (d == 64) return type(std::integral_constant<int, 64>{});
+  if (d == 128) return type(std::integral_constant<int, 128>{});
+  return type(std::integral_constant<int, 256>{});
 }
 
 }  // namespace fa

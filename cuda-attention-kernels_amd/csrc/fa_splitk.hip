@@ -88,9 +88,6 @@ constexpr bool paged_dealt(int head_dim, bool fp8) { return !fp8 || head_dim == 
 // shares, or the shared ones, for the rows of all requests of a group.
 enum Keys { kOwn = 0, kSuffix = 1, kPrefix = 2 };
 
-struct SharedTileArgs : TileArgs {
-  SharedArgs shared;
-};
 template <int KEYS>
 struct SplitkArgs {
   using type = typename std::conditional<KEYS == kOwn, TileArgs, SharedTileArgs>::type;
@@ -141,13 +138,12 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   if constexpr (KEYS == kPrefix) {
     // kv-head innermost (8 of them: one to an XCD, whose L2 then holds its keys), then the row blocks, which read the
     // same keys at about the same time
-    int item = (int)blockIdx.x, group;
+    int item = (int)blockIdx.x;
     kvh = item % a.hkv;
     item /= a.hkv;
     rb = item % a.n_rowblk;
     chunk = item / a.n_rowblk;
-    if (!group_of_block(a.shared, a.group * a.nq, NW * 32, rb, group, b0, b1)) return;  // uniform over the workgroup
-    seq_k = __builtin_amdgcn_readfirstlane(shared_keys(a.shared, group));
+    if (!group_of_block(a.shared, a.group * a.nq, NW * 32, rb, b0, b1, seq_k)) return;  // uniform over the workgroup
     if (chunk * a.ppw * a.split_len >= seq_k) return;
     b = prefix_holder(a.seqlens_k, b0, b1, seq_k);
   } else if constexpr (PAGED && (paged_dealt(D, IS_FP8) || KEYS == kSuffix)) {
@@ -190,7 +186,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   if constexpr (PAGED && KEYS == kOwn) seq_k = min(max(__builtin_amdgcn_readfirstlane(a.seqlens_k[b]), 0), a.nk);
   if constexpr (KEYS == kSuffix) {
     start = shared_keys_of(a.shared, b);
-    seq_k = min(max(__builtin_amdgcn_readfirstlane(a.seqlens_k[b]), 0), min(start + a.nk, a.shared.table_keys));
+    seq_k = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens_k[b]), start);
   }
   // rows: (q-head in group, query); kPrefix: of every request of the group
   const int R = (KEYS == kPrefix ? b1 - b0 : 1) * a.group * seq_q;
@@ -217,7 +213,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
     const int in_group = row_ok ? row / seq_q : 0, member = in_group / a.group;
     bq = b0 + member;
     hq = kvh * a.group + (in_group - member * a.group);
-    const int n = max(a.seqlens_k[bq], 0);
+    const int n = keys_of(a.shared, a.seqlens_k[bq], seq_k);
     row_keys = max(min(a.causal ? n - seq_q + qi + 1 : n, seq_k), 0);
   }
 
@@ -512,7 +508,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
     } else if (wave_active && row_ok) {
       int64_t prow = a.part_major ? prow0 + j : ((int64_t)(b * a.hq + hq) * seq_q + qi) * a.n_split + part;
       if constexpr (KEYS != kOwn)
-        prow = ((int64_t)(bq * a.hq + hq) * seq_q + qi) * a.shared.part_stride + a.shared.part_base + part;
+        prow = ((int64_t)(bq * a.hq + hq) * seq_q + qi) * a.shared.part_stride + (KEYS == kSuffix ? a.shared.part_base : 0) + part;
       float* op = (float*)a.o + prow * D;
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
@@ -926,92 +922,6 @@ __global__ void __launch_bounds__(256) splitk_combine_kernel(const CombineArgs c
   }
 }
 
-// The merge of a row's partials of the shared keys (the first of its part_stride places) and of its own (from part_base
-// on): splitk_combine_kernel's sums over those that its length and its group's prefix have.
-struct SharedCombineArgs {
-  CombineArgs c;
-  SharedArgs shared;
-  int32_t prefix_split, suffix_split;  // keys per partition
-};
-
-template <int D, class E>
-__global__ void __launch_bounds__(256) shared_combine_kernel(const SharedCombineArgs a) {
-  constexpr int TPS = D / 8;
-  constexpr int SPB = 256 / TPS;
-  constexpr float NEG_INF = -__builtin_inff();
-  __shared__ f32x4 part[SPB][TPS][2];
-  __shared__ f32x2 mlpart[SPB];
-  const CombineArgs& c = a.c;
-  const uint32_t row = blockIdx.x, nq = (uint32_t)c.nq;
-  const uint32_t bh = row / nq, qi = row - bh * nq, b = bh / (uint32_t)c.hq, hq = bh - b * (uint32_t)c.hq;
-  const int shared = shared_keys_of(a.shared, (int)b);
-  const int keys = min(max(__builtin_amdgcn_readfirstlane(c.seqlens_k[b]), 0), min(shared + a.shared.max_suffix, a.shared.table_keys));
-  const int first = (shared + a.prefix_split - 1) / a.prefix_split;
-  const int count = first + (keys > shared ? (keys - shared + a.suffix_split - 1) / a.suffix_split : 0);
-  const int64_t base = (int64_t)row * a.shared.part_stride;
-  const int skip = a.shared.part_base - first;  // places between the two runs
-  const float* ml = c.ml + base * 2;
-  const float* op = c.opart + base * D;
-  const int tid = (int)threadIdx.x;
-  const int sg = tid / TPS, dq = tid % TPS;
-  constexpr int CH = 4;  // partials a thread loads before it merges any
-  float m = NEG_INF, l = 0.f;
-  f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = sg; s0 < count; s0 += CH * SPB) {
-    f32x2 st[CH];
-    f32x4 pv0[CH], pv1[CH];
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      int s = s0 + u * SPB;
-      if (s < count) {
-        s += s >= first ? skip : 0;
-        st[u] = __builtin_bit_cast(f32x2, ld8(ml + 2 * s));
-        pv0[u] = __builtin_bit_cast(f32x4, ld16(op + (int64_t)s * D + 8 * dq));
-        pv1[u] = __builtin_bit_cast(f32x4, ld16(op + (int64_t)s * D + 8 * dq + 4));
-      } else {
-        st[u] = f32x2{NEG_INF, 0.f};
-        pv0[u] = pv1[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const float m_new = fmaxf(m, st[u][0]);
-      const float m_ref = (m_new == NEG_INF) ? 0.f : m_new;
-      const float alpha = fast_exp2(m - m_ref);
-      const float w = fast_exp2(st[u][0] - m_ref) * st[u][1];
-      l = l * alpha + w;
-      acc0 = acc0 * alpha + w * pv0[u];
-      acc1 = acc1 * alpha + w * pv1[u];
-      m = m_new;
-    }
-  }
-  part[sg][dq][0] = acc0;
-  part[sg][dq][1] = acc1;
-  if (dq == 0) mlpart[sg] = f32x2{m, l};
-  __syncthreads();
-  if (tid < TPS) {
-    float mx = NEG_INF;
-#pragma unroll
-    for (int k = 0; k < SPB; ++k) mx = fmaxf(mx, mlpart[k][0]);
-    const float m_ref = (mx == NEG_INF) ? 0.f : mx;
-    f32x4 t0 = {0.f, 0.f, 0.f, 0.f}, t1 = {0.f, 0.f, 0.f, 0.f};
-    float lt = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < SPB; ++k) {
-      const float w = fast_exp2(mlpart[k][0] - m_ref);
-      lt += w * mlpart[k][1];
-      t0 += w * part[k][tid][0];
-      t1 += w * part[k][tid][1];
-    }
-    const float l_safe = (lt == 0.f) ? 1.f : lt;
-    const float inv = 1.f / l_safe;
-    if (c.lse != nullptr && tid == 0) c.lse[b * c.slb + (int64_t)hq * c.slh + qi] = (mx + __log2f(l_safe)) * kLn2;
-    uint16_t* o = (uint16_t*)c.o + b * c.sob + (int64_t)hq * c.soh + (int64_t)qi * c.son + 8 * tid;
-    st8(o, u32x2{pack2<E>(t0[0] * inv, t0[1] * inv), pack2<E>(t0[2] * inv, t0[3] * inv)});
-    st8(o + 4, u32x2{pack2<E>(t1[0] * inv, t1[1] * inv), pack2<E>(t1[2] * inv, t1[3] * inv)});
-  }
-}
-
 // ------------------------------------------------------------------------------------
 // Host-side launchers
 // ------------------------------------------------------------------------------------
@@ -1160,7 +1070,7 @@ fa_status splitk_scratch(void** ptr, const char** err) {
   return FA_OK;
 }
 
-static void paged_args(TileArgs& a, const fa_paged_kv& kv) {
+void paged_args(TileArgs& a, const fa_paged_kv& kv) {
   a.skb = a.svb = 0;
   a.block_table = kv.block_table;
   a.seqlens_k = kv.seqlens_k;
@@ -1287,133 +1197,10 @@ static hipError_t launch_shared(const SharedTileArgs& a, bool fp8, bool prefix, 
   return prefix ? launch_shared_nw<D, E, E, kPrefix>(a, nw, stream) : launch_shared_nw<D, E, E, kSuffix>(a, nw, stream);
 }
 
-template <int D, class E>
-static hipError_t launch_shared_combine(const SharedCombineArgs& a, int64_t rows, hipStream_t stream) {
-  hipLaunchKernelGGL((shared_combine_kernel<D, E>), dim3((unsigned)rows), dim3(256), 0, stream, a);
-  return hipGetLastError();
-}
-
-template <class F>
-static hipError_t by_dim_and_type(int d, bool bf, F&& f) {
-  auto type = [&](auto dim) { return bf ? f(dim, BF16{}) : f(dim, F16{}); };
-  if (d == 64) return type(std::integral_constant<int, 64>{});
-  if (d == 128) return type(std::integral_constant<int, 128>{});
-  return type(std::integral_constant<int, 256>{});
-}
-
-SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int page_size) {
-  constexpr int kWgs = 1024;
-  const int group = p.heads_q / p.heads_kv, rows = group * p.seqlen_q;
-  SharedPlan plan{};
-  plan.max_prefix = s.max_prefix_len / kPrefixUnit * kPrefixUnit;
-  // (a prefix is cut at whole units: up to 63 of its keys go with each request's own)
-  plan.max_suffix = s.max_suffix_len + kPrefixUnit - 1;
-  const int64_t all_rows = (int64_t)p.batch * rows;
-  plan.prefix_waves = splitk_waves_for_rows((int)std::min<int64_t>(all_rows, 1024));
-  plan.suffix_waves = splitk_waves_for_rows(rows);
-  const int64_t group_blocks = all_rows / (plan.prefix_waves * 32) + std::max(1, s.num_groups);
-  plan.prefix_blocks = group_blocks;
-  const int64_t cap = (int64_t)254 * page_size / 64 * 64;  // a partition spans at most 256 pages of the table
-  auto cut = [&](int64_t keys, int64_t items, int64_t shortest) {
-    const int64_t parts = std::max<int64_t>(1, kWgs / std::max<int64_t>(items, 1));
-    const int64_t len = ((keys + parts - 1) / parts + 63) / 64 * 64;
-    return (int32_t)std::min(std::max<int64_t>(std::min<int64_t>(len, 4096), shortest), std::max<int64_t>(cap, 64));
-  };
-  plan.prefix_split = s.split_len > 0 ? s.split_len : cut(plan.max_prefix, p.heads_kv * group_blocks, 256);
-  plan.suffix_split = s.split_len > 0 ? s.split_len
-                                      : cut(plan.max_suffix, (int64_t)p.batch * p.heads_kv * ((rows + 127) / 128), 128);
-  plan.prefix_parts = (plan.max_prefix + plan.prefix_split - 1) / plan.prefix_split;
-  plan.suffix_parts = (plan.max_suffix + plan.suffix_split - 1) / plan.suffix_split;
-  return plan;
-}
-
-const char* shared_refusal(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_shared_prefix& s) {
-  const SharedPlan plan = plan_shared(p, s, kv.page_size);
-  const int64_t rows = (int64_t)p.heads_q / p.heads_kv * p.seqlen_q;
-  auto slots = [&](int64_t len) { return (len - 1) / kv.page_size + 2; };
-  if (slots(plan.prefix_split) > 256 || slots(plan.suffix_split) > 256)
-    return "split_len too long for the page size: a partition may span at most 256 pages";
-  const int64_t out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
-  const int64_t row_blocks = (rows + plan.suffix_waves * 32 - 1) / (plan.suffix_waves * 32);
-  if (out_rows > INT32_MAX / 2 || plan.prefix_blocks * p.heads_kv * plan.prefix_parts > INT32_MAX ||
-      ((int64_t)p.batch * p.heads_kv * plan.suffix_parts + 8) * row_blocks > INT32_MAX)
-    return "grid too large";
-  return nullptr;
-}
-
-size_t shared_workspace_bytes(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_shared_prefix& s) {
-  const SharedPlan plan = plan_shared(p, s, kv.page_size);
-  return (size_t)p.batch * p.heads_q * p.seqlen_q * (size_t)(plan.prefix_parts + plan.suffix_parts) *
-         ((size_t)p.head_dim + 2) * sizeof(float);
-}
-
-fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_shared_prefix& s, void* workspace,
-                     hipStream_t stream, const char** err) {
-  const SharedPlan plan = plan_shared(p, s, kv.page_size);
-  const bool fp8 = p.kv_dtype == FA_DTYPE_FP8_E4M3, bf = p.dtype == FA_DTYPE_BF16;
-  const int64_t out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
-  const int stride = plan.prefix_parts + plan.suffix_parts;
-  SharedTileArgs a{};
-  static_cast<TileArgs&>(a) = common_args(p);
-  paged_args(a, kv);
-  a.o = workspace;
-  a.ml = (float*)workspace + out_rows * stride * p.head_dim;
-  a.batch = p.batch;
-  a.ppw = 1;
-  a.shared.prefix_lens = s.prefix_lens;
-  a.shared.cu_groups = s.cu_groups;
-  a.shared.groups = s.cu_groups != nullptr ? s.num_groups : 1;
-  a.shared.batch = p.batch;
-  a.shared.max_prefix = plan.max_prefix;
-  a.shared.max_suffix = plan.max_suffix;
-  a.shared.table_keys = (int32_t)std::min<int64_t>((int64_t)kv.block_table_cols * kv.page_size, INT32_MAX);
-  a.shared.part_stride = stride;
-  hipError_t e = hipSuccess;
-  if (plan.prefix_parts > 0) {
-    a.split_len = plan.prefix_split;
-    a.n_split = a.n_chunk = plan.prefix_parts;
-    a.nk = plan.max_prefix;
-    a.n_rowblk = (int32_t)plan.prefix_blocks;
-    a.total = (int32_t)(plan.prefix_blocks * p.heads_kv * plan.prefix_parts);
-    a.shared.part_base = 0;
-    e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) {
-      return launch_shared<decltype(d)::value, decltype(t)>(a, fp8, true, plan.prefix_waves, stream);
-    });
-    if (e != hipSuccess) return hip_status(e, err);
-  }
-  a.split_len = plan.suffix_split;
-  a.n_split = a.n_chunk = plan.suffix_parts;
-  a.nk = plan.max_suffix;
-  const int rows = a.group * p.seqlen_q;
-  a.n_rowblk = (rows + plan.suffix_waves * 32 - 1) / (plan.suffix_waves * 32);
-  a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts);
-  a.total = (int32_t)(((int64_t)a.n_items + 7) / 8 * 8 * a.n_rowblk);
-  a.shared.part_base = plan.prefix_parts;
-  e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) {
-    return launch_shared<decltype(d)::value, decltype(t)>(a, fp8, false, plan.suffix_waves, stream);
+hipError_t launch_shared_split(const SharedTileArgs& a, int d, bool bf, bool fp8, bool prefix, int nw, hipStream_t stream) {
+  return by_dim_and_type(d, bf, [&](auto dim, auto type) {
+    return launch_shared<decltype(dim)::value, decltype(type)>(a, fp8, prefix, nw, stream);
   });
-  if (e != hipSuccess) return hip_status(e, err);
-
-  SharedCombineArgs c{};
-  c.c.opart = (const float*)a.o;
-  c.c.ml = a.ml;
-  c.c.o = p.o;
-  c.c.sob = p.o_stride_b;
-  c.c.soh = p.o_stride_h;
-  c.c.son = p.o_stride_n;
-  c.c.hq = p.heads_q;
-  c.c.nq = p.seqlen_q;
-  c.c.seqlens_k = kv.seqlens_k;
-  c.c.lse = p.lse;
-  c.c.slb = p.lse_stride_b;
-  c.c.slh = p.lse_stride_h;
-  c.shared = a.shared;
-  c.prefix_split = plan.prefix_split;
-  c.suffix_split = plan.suffix_split;
-  e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) {
-    return launch_shared_combine<decltype(d)::value, decltype(t)>(c, out_rows, stream);
-  });
-  return hip_status(e, err);
 }
 
 }  // namespace fa
