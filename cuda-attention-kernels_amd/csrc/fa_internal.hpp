@@ -233,9 +233,7 @@ struct SharedPlan {
   int32_t max_prefix, max_suffix;      // bounds of the shared keys, and of a request's keys behind them
   int32_t prefix_split, suffix_split;  // keys per partition
   int32_t prefix_parts, suffix_parts;  // partitions
-  int32_t prefix_waves, suffix_waves;  // waves (of 32 rows) per workgroup
   int64_t prefix_blocks;               // row blocks of all groups, at most
-  bool fused;                          // both parts in one launch
 };
 SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int page_size);
 // Why a call of valid parameters cannot be launched, or NULL.

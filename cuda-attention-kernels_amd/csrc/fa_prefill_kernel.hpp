@@ -39,9 +39,9 @@ struct FwdArgs {
 // At D=256 the fp32 output accumulator alone takes 128 registers per lane, so the kernel runs one wave per
 // SIMD there.  D=64 and D=32 also come with 64-key tiles, which leave registers and LDS for three
 // workgroups per CU in place of two (kFwdShortTile; plan_fwd says when).
-template <int D, class E, int NW, int BN, bool SPLIT, bool SHARED = false>
+template <int D, class E, int NW, int BN, bool SPLIT, bool SHARED = false, class KV = E>
 __global__ void __launch_bounds__(NW * 64)
-    __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : (D < 128 && BN == 64 ? 3 : 2))))
+    __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : (D < 128 && BN == 64 && KV::bytes == 2 ? 3 : 2))))
 attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   static_assert(NW == 4 || (NW == 8 && D != 256), "4 or 8 waves (two per SIMD) per workgroup");
   // V tiles are at least 32 columns wide, since O^T += V^T P^T works in 32-wide d blocks.  At
@@ -60,6 +60,10 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   static_assert((TILE * 2) % (1024 * NW) == 0 && (VTILE * 2) % (1024 * NW) == 0,
                 "direct loads must split evenly over the waves");
   constexpr float NEG_INF = -__builtin_inff();
+  // FP8 K/V (SHARED): widened on their way into LDS, so that the loop below finds 16-bit tiles
+  constexpr bool IS8 = KV::bytes == 1;
+  constexpr int KVB = KV::bytes;
+  static_assert(!IS8 || SHARED, "FP8 K/V: shared keys only");
   // At D=16 the loop is bound by its vector work (the two products cost 12 MFMAs per 128-key
   // tile against about 200 VALU instructions), so the row sums of P move to the matrix core: one
   // 16x16x32 MFMA per 16-key half-block against a 0/1 operand (rowsum_ones) replaces eight
@@ -83,9 +87,9 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
       if (item >= a.n_items) return;
       // (arrays named at compile time, as above)
       if (w < 2) {
-        suffix_rows<D, E>(a, item, k_buf0 + half, v_buf0 + half);
+        suffix_rows<D, E, KV>(a, item, k_buf0 + half, v_buf0 + half);
       } else {
-        suffix_rows<D, E>(a, item, k_buf1 + half, v_buf1 + half);
+        suffix_rows<D, E, KV>(a, item, k_buf1 + half, v_buf1 + half);
       }
       return;
     }
@@ -196,9 +200,9 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     row_len = a.seqlens_k[bq];
   }
 
-  const uint8_t* kbase = (const uint8_t*)a.k + ((int64_t)b * a.skb + (int64_t)kvh * a.skh + ktok0 * a.skn) * 2;
-  const uint8_t* vbase = (const uint8_t*)a.v + ((int64_t)b * a.svb + (int64_t)kvh * a.svh + ktok0 * a.svn) * 2;
-  const int64_t krow_bytes = a.skn * 2, vrow_bytes = a.svn * 2;
+  const uint8_t* kbase = (const uint8_t*)a.k + ((int64_t)b * a.skb + (int64_t)kvh * a.skh + ktok0 * a.skn) * KVB;
+  const uint8_t* vbase = (const uint8_t*)a.v + ((int64_t)b * a.svb + (int64_t)kvh * a.svh + ktok0 * a.svn) * KVB;
+  const int64_t krow_bytes = a.skn * KVB, vrow_bytes = a.svn * KVB;
 
   // A negative softmax scale is applied by negating Q (exact for 16-bit floats), so
   // the kernel works with c = |scale| * log2(e) > 0 and max(c*s) = c*max(s).  c is
@@ -238,7 +242,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   int pg[PG_REGS] = {};
   const int unit = wave * (BN / NW) / 16 * 16;  // the first of the 16 keys of a tile that hold the wave's rows
   int pslot = 0, poff = 0;                      // their table slot (from the workgroup's first) and offset in the page
-  int first_slot = 0;
+  int first_slot = 0, table_row = b;
   if constexpr (SHARED) {
     first_slot = a.shared.by_page.of(klo);
     const int slot_end = a.shared.by_page.of(khi - 1) + 1;
@@ -257,6 +261,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   // padded batch): the entries are then loaded again from one that does.  (Both loads start together.)
   if constexpr (SHARED) {
     const int holder = prefix_holder(a.seqlens_k, b0, b1, shared);
+    table_row = holder;
     if (holder != b) {
       const int slot_end = a.shared.by_page.of(khi - 1) + 1;
       const int32_t* bt = a.block_table + (int64_t)holder * a.sbt;
@@ -298,20 +303,64 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
       valid_new = ok ? valid_new : 0;
       page_new = ok ? page : 0;
     } else if (step == 1) {
-      knew.base = kbase + (int64_t)page_new * (a.spk * 2);
-      knew.limit = valid_new > 0 ? (uint32_t)(valid_new - 1) * (uint32_t)krow_bytes + (uint32_t)(D * 2) : 0u;
+      knew.base = kbase + (int64_t)page_new * (a.spk * KVB);
+      knew.limit = valid_new > 0 ? (uint32_t)(valid_new - 1) * (uint32_t)krow_bytes + (uint32_t)(D * KVB) : 0u;
     } else if (step == 2) {
       knew.base += (int64_t)off_new * krow_bytes;
-      vsrc[2].base = vbase + (int64_t)page_new * (a.spv * 2);
+      vsrc[2].base = vbase + (int64_t)page_new * (a.spv * KVB);
     } else {
       vsrc[2].base += (int64_t)off_new * vrow_bytes;
-      vsrc[2].limit = valid_new > 0 ? (uint32_t)(valid_new - 1) * (uint32_t)vrow_bytes + (uint32_t)(D * 2) : 0u;
+      vsrc[2].limit = valid_new > 0 ? (uint32_t)(valid_new - 1) * (uint32_t)vrow_bytes + (uint32_t)(D * KVB) : 0u;
     }
   };
   auto source_next = [&]() __attribute__((always_inline)) {
     ksrc = knew;
     vsrc[0] = vsrc[1];
     vsrc[1] = vsrc[2];
+  };
+  // FP8: a wave's rows of a tile come through registers, NP pieces of 16 values a lane, one iteration before they are
+  // widened and written to LDS.  The block scales lie in lanes: lane i holds those of the partition's 64-key block i.
+  constexpr int NP = IS8 ? BN / NW * D / 1024 : 1;
+  u32x4 kreg[NP], vreg[NP];
+  float k_scales = 0.f, v_scales = 0.f;
+  if constexpr (IS8) {
+    const int n = klo + 64 * lane;
+    if (n < khi) {
+      const int slot = a.shared.by_page.of(n);
+      const int page = a.block_table[(int64_t)table_row * a.sbt + slot];
+      if ((uint32_t)page < (uint32_t)a.num_pages) {  // (keys outside the pool are zeros, with scale 0)
+        const int64_t at = (int64_t)page * a.ssb + (int64_t)kvh * a.ssh + (n - slot * a.page_size) / 64;
+        k_scales = a.k_scale[at];
+        v_scales = a.v_scale[at];
+      }
+    }
+  }
+  auto scale_of = [&](float scales, int t) __attribute__((always_inline)) {
+    return lane_value(scales, t * BN / 64);
+  };
+  // what tile t's products are multiplied with to be scores in log2 units
+  auto score_scale = [&](int t) __attribute__((always_inline)) { return IS8 ? fmaxf(c * scale_of(k_scales, t), kMinScale) : c; };
+  // Lane's row of piece 0, and where piece i lies from there: a uniform distance in memory (the pieces' rows are PR apart,
+  // PR a power of two, and kperm moves that bit as a whole), and in LDS a distance and a flip of chunk bits.  The lane's
+  // places are formed anew from three registers each time: as registers of their own they would be spilled, and a spill's
+  // reload waits for the rows in flight.
+  constexpr int PR = IS8 ? 1024 / D : 1;
+  const int row0 = IS8 ? wave * (BN / NW) + lane * 16 / D : 0, col0 = IS8 ? lane * 16 % D : 0;
+  int k_at = (kperm(row0) & 15) * (int)krow_bytes + col0, v_at = (row0 & 15) * (int)vrow_bytes + col0;
+  uint32_t k_put = (uint32_t)(row0 * D + (((col0 / 8) ^ Shape::swz_k(row0)) * 8)) * 2u;
+  uint32_t v_put = (uint32_t)(row0 * D + (((col0 / 8) ^ VShape::swz_v(row0)) * 8)) * 2u;
+  auto fetch = [&](const PageRows& src, int64_t row_bytes, bool keys, int i) __attribute__((always_inline)) {
+    // (the rows of a partition's tiles are all there, or none of them: its ends are whole 64 keys)
+    return __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(src.base, src.limit), keys ? k_at : v_at,
+                                                 i * (keys ? kperm(PR) : PR) * (int)row_bytes, 0);
+  };
+  // half h (8 values) of piece i to its place in a tile
+  auto widen = [&](const u32x4& piece, uint16_t* dst, bool keys, int i, int h) __attribute__((always_inline)) {
+    const u32x2 lo = fp8x4_to_e<E>(piece[2 * h]), hi = fp8x4_to_e<E>(piece[2 * h + 1]);
+    const uint32_t flip = (uint32_t)(h ^ (keys ? Shape::swz_k(i * PR) ^ Shape::swz_k(0) : VShape::swz_v(i * PR) ^ VShape::swz_v(0))) * 16u;
+    uint32_t& put = keys ? k_put : v_put;
+    __asm__ volatile("" : "+v"(put));
+    st16((uint8_t*)dst + ((put ^ flip) + (uint32_t)(i * PR * D * 2)), u32x4{lo[0], lo[1], hi[0], hi[1]});
   };
   auto k_rsrc = [&](int n0) __attribute__((always_inline)) {
     if constexpr (SHARED) {
@@ -369,12 +418,35 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
       source_next();
     };
     source(0);
-    load_k(key0(0), k_buf0);
-    vsrc[0] = vsrc[1];
-    load_v(key0(0), v_buf0);
-    source(1);
-    load_k(key0(1), k_buf1);
-    source(2);  // (in iteration 0: K of tile 2, V of tile 1)
+    if constexpr (IS8) {
+      u32x4 first[NP], second[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) first[i] = fetch(ksrc, krow_bytes, true, i);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) vreg[i] = fetch(vsrc[1], vrow_bytes, false, i);
+      source(1);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) second[i] = fetch(ksrc, krow_bytes, true, i);
+      source(2);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) kreg[i] = fetch(ksrc, krow_bytes, true, i);
+#pragma unroll
+      for (int i = 0; i < 2 * NP; ++i) {
+        widen(first[i / 2], k_buf0, true, i / 2, i % 2);
+        widen(vreg[i / 2], v_buf0, false, i / 2, i % 2);
+        widen(second[i / 2], k_buf1, true, i / 2, i % 2);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) vreg[i] = fetch(vsrc[0], vrow_bytes, false, i);
+      source(3);  // (in iteration 0, K of tile 2 and V of tile 1 go to LDS, and K of tile 3 and V of tile 2 are fetched)
+    } else {
+      load_k(key0(0), k_buf0);
+      vsrc[0] = vsrc[1];
+      load_v(key0(0), v_buf0);
+      source(1);
+      load_k(key0(1), k_buf1);
+      source(2);  // (in iteration 0: K of tile 2, V of tile 1)
+    }
   } else if (n_tiles > 0) {
     load_k(key0(0), k_buf0);
     load_v(key0(0), v_buf0);
@@ -420,6 +492,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   for (int d = 0; d < DB; ++d) oacc[d] = f32x16{};
   // running max m_run (log2 domain, scaled) and this lane's share of the row sum
   float m_run = NEG_INF, l_run = 0.f;
+  float v_cur = 0.f;  // FP8: O's unit
   f32x4 l_acc = f32x4{};  // MFMA_ROWSUM: every lane's registers hold its own row's full sum
   const u32x4 ones = rowsum_ones<E>(lane);
   // S^T of two consecutive tiles (the loop below is unrolled by 2)
@@ -444,7 +517,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     }
   };
   // row max of c*S over the tile (both lanes of the row agree)
-  auto tile_max = [&](const f32x16(&sc)[KB]) __attribute__((always_inline)) {
+  auto tile_max = [&](const f32x16(&sc)[KB], float c) __attribute__((always_inline)) {
     float mx = sc[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -511,7 +584,24 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     static_assert(NDMA <= NM, "one DMA instruction per slot");
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) nxt[kb] = f32x16{};
-    const float m_safe = (m_run == NEG_INF) ? 0.f : m_run;
+    float m_safe = (m_run == NEG_INF) ? 0.f : m_run;
+    // FP8: O is held in units of v_cur, the V block scale of a recent tile.  A tile whose scale vb is within a factor 2 of
+    // it takes vb / v_cur into its exponents, and out of its row sum again; any other first brings O to its own scale.
+    const float c_this = score_scale(t), c_next = score_scale(t + 1);
+    float unfold = 1.f;
+    if constexpr (IS8) {
+      const float vb = scale_of(v_scales, t);
+      if (vb > 0.f && !(vb <= 2.f * v_cur && v_cur <= 2.f * vb)) {
+        const float ratio = v_cur / vb;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) oacc[d] *= ratio;
+        v_cur = vb;
+      }
+      if (vb > 0.f) {
+        unfold = v_cur / vb;
+        m_safe += __log2f(unfold);
+      }
+    }
     u32x4 pf[KB][2];
     u32x4 opnd[PD + 1];
     float rs = 0.f;
@@ -532,8 +622,8 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     // exp micro-step u: scores 2e and 2e+1 of chunk (kb, h) of S_t
     auto exp_step = [&](int u) __attribute__((always_inline)) {
       const int kb = u / 8, h = (u / 4) % 2, e = u % 4;
-      const float p0 = fast_exp2(__builtin_fmaf(cur[kb][8 * h + 2 * e], c, -m_safe));
-      const float p1 = fast_exp2(__builtin_fmaf(cur[kb][8 * h + 2 * e + 1], c, -m_safe));
+      const float p0 = fast_exp2(__builtin_fmaf(cur[kb][8 * h + 2 * e], c_this, -m_safe));
+      const float p1 = fast_exp2(__builtin_fmaf(cur[kb][8 * h + 2 * e + 1], c_this, -m_safe));
       const uint32_t pk = pack2<E>(p0, p1);
       pf[kb][h][e] = pk;
       // the row sum of the rounded P that the MFMA consumes (so O/l is a convex combination)
@@ -551,7 +641,20 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     static_for<0, NM>([&](auto mc) __attribute__((always_inline)) {
       constexpr int m = decltype(mc)::value;
       if constexpr (m + PD < NM) read(m + PD);
-      if constexpr (m < NDMA) {
+      if constexpr (IS8) {
+        // a half of a piece every few slots; the piece's registers then take their next rows
+        constexpr int every = NM / (4 * NP);
+        if constexpr (m % every == 0 && m / every < 4 * NP) {
+          constexpr int u = m / every, i = u / 2 % NP;
+          if constexpr (u < 2 * NP) {
+            widen(kreg[i], kd, true, i, u % 2);
+            if constexpr (u % 2 == 1) kreg[i] = fetch(ksrc, krow_bytes, true, i);
+          } else {
+            widen(vreg[i], vd, false, i, u % 2);
+            if constexpr (u % 2 == 1) vreg[i] = fetch(vsrc[0], vrow_bytes, false, i);
+          }
+        }
+      } else if constexpr (m < NDMA) {
         if constexpr (m < QPW) {
           dma_k(rk, kd, m);
         } else {
@@ -584,13 +687,13 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
       }
       if constexpr (SHARED) {
         constexpr int first = NDMA, every = (NM - NDMA) / 4;  // behind this iteration's own loads
-        if constexpr (m >= first && (m - first) % every == 0 && (m - first) / every < 4) source_step((m - first) / every, t + 3);
+        if constexpr (m >= first && (m - first) % every == 0 && (m - first) / every < 4) source_step((m - first) / every, t + (IS8 ? 4 : 3));
       }
       __builtin_amdgcn_sched_barrier(0);
     });
     if constexpr (SHARED) source_next();
-    l_run += rs;
-    float mt = max_xor32(mx * c);
+    l_run += IS8 ? rs * unfold : rs;
+    float mt = max_xor32(mx * c_next);
     if (t + 1 >= n_fast) {
       const int n1 = key0(t + 1);
       if (t + 1 < n_tiles) {
@@ -600,7 +703,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
           // (measured: ~150 extra VALU/SALU instructions per tile)
           __asm__ volatile("");
           mask(nxt, n1);
-          mt = tile_max(nxt);
+          mt = tile_max(nxt, c_next);
         }
       } else {
         mt = NEG_INF;  // past the last tile: nxt holds stale LDS data and is discarded
@@ -623,7 +726,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) qk(k_buf0, s_a, s);
     if (key0(0) + BN > mask_from) mask(s_a, key0(0));
-    update_max(tile_max(s_a));
+    update_max(tile_max(s_a, score_scale(0)));
     __syncthreads();  // every wave has read K_0: its buffer takes K_2
   }
 
@@ -646,8 +749,13 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
 #pragma unroll
       for (int i = 0; i < VQPW; ++i) dma_v(rv, v_next, i);
     }
-    lds_dma_wait();
-    __syncthreads();
+    if constexpr (IS8) {
+      // what is in flight goes to registers: only the writes to LDS, and the reads of it, have to be done
+      __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    } else {
+      lds_dma_wait();
+      __syncthreads();
+    }
   };
   for (int t = 0; t < n_tiles; t += 2) {
     step(std::integral_constant<int, 0>{}, t);
@@ -668,7 +776,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     // here) and (m, l), [S][B, Hq, Nq][D]
     const int64_t rows = (int64_t)a.kv_groups * a.group * seq_q;
     const int64_t row0 = sp * rows + ((int64_t)b * a.hq + hq) * seq_q + wr0;
-    const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
+    const float inv = l_tot > 0.f ? (IS8 ? v_cur : 1.f) / l_tot : 0.f;
     if (row_ok && g == 0) st8(a.ml + (SHARED ? (int64_t)out_row * part_stride + sp : row0 + j) * 2, __builtin_bit_cast(u32x2, f32x2{m_run, l_tot}));
     if constexpr (NW * 32 * D * 4 <= 4 * TILE * 2) {
       // through LDS, as the output below: whole rows per store instruction

@@ -112,8 +112,10 @@ namespace {
 constexpr int prefix_tile_keys(int d) { return d == 256 ? 32 : 64; }
 
 template <int D, class E>
-hipError_t launch_tiles(const SharedTileArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((attn_fwd_kernel<D, E, 4, prefix_tile_keys(D), false, true>), dim3((unsigned)a.total), dim3(256), 0, stream, a);
+hipError_t launch_tiles(const SharedTileArgs& a, bool fp8, hipStream_t stream) {
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)a.total), dim3(256), 0, stream, a); };
+  fp8 ? launch(attn_fwd_kernel<D, E, 4, prefix_tile_keys(D), false, true, FP8>)
+      : launch(attn_fwd_kernel<D, E, 4, prefix_tile_keys(D), false, true>);
   return hipGetLastError();
 }
 
@@ -141,11 +143,8 @@ SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int pa
   plan.max_suffix = s.max_suffix_len + kPrefixUnit - 1;
   const int64_t all_rows = (int64_t)p.batch * rows;
   const bool fp8 = p.kv_dtype == FA_DTYPE_FP8_E4M3;
-  plan.fused = !fp8;
-  plan.prefix_waves = fp8 ? splitk_waves_for_rows((int)std::min<int64_t>(all_rows, 1024)) : 4;
-  plan.suffix_waves = splitk_waves_for_rows(rows);
   // (one group: exactly; several: each may leave a block unfilled, and the workgroups past the last block return)
-  const int64_t block = plan.prefix_waves * 32;
+  constexpr int block = 128;  // rows of a workgroup
   const int64_t group_blocks = s.num_groups > 1 ? all_rows / block + s.num_groups : (all_rows + block - 1) / block;
   plan.prefix_blocks = group_blocks;
   // Partitions.  A workgroup of the shared keys costs about 8 us before and after its tiles (64 keys in about 1 us at
@@ -156,16 +155,17 @@ SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int pa
   // not to run on alone (256 requests of up to 1000 keys, D = 64: 95 us whole, 91 in two).
   constexpr int64_t kWgs = 256, kLong = 1024, kWaves = 1024, kLongest = 576;
   auto whole = [](int64_t keys, int64_t parts) { return ((keys + parts - 1) / parts + kPrefixUnit - 1) / kPrefixUnit * kPrefixUnit; };
-  auto fits = [&](int64_t len, int64_t pages) {  // a partition spans a limited number of pages
-    return (int32_t)std::max<int64_t>(kPrefixUnit, std::min(len, (pages - 2) * page_size / kPrefixUnit * kPrefixUnit));
+  auto fits = [&](int64_t len, int64_t pages) {  // a partition spans a limited number of pages, and of FP8 scale blocks
+    len = std::min(len, (pages - 2) * page_size / kPrefixUnit * kPrefixUnit);
+    return (int32_t)std::max<int64_t>(kPrefixUnit, fp8 ? std::min<int64_t>(len, kFp8Keys) : len);
   };
   const int64_t prefix_items = p.heads_kv * ((all_rows + block - 1) / block);
-  int64_t len = whole(plan.max_prefix, std::max<int64_t>(1, (plan.fused ? kWgs : 2 * kWgs) / prefix_items));
-  if (plan.fused && len < kLong) len = std::min(kLong, whole(plan.max_prefix, std::max<int64_t>(1, kWgs / 2 / prefix_items)));
-  plan.prefix_split = s.split_len > 0 ? s.split_len : fits(len, plan.fused ? kPrefixPages : 256);
+  int64_t len = whole(plan.max_prefix, std::max<int64_t>(1, kWgs / prefix_items));
+  if (len < kLong) len = std::min(kLong, whole(plan.max_prefix, std::max<int64_t>(1, kWgs / 2 / prefix_items)));
+  plan.prefix_split = s.split_len > 0 ? s.split_len : fits(len, kPrefixPages);
   const int64_t suffix_items = (int64_t)p.batch * p.heads_kv * ((rows + 31) / 32);
   len = std::min(kLongest, whole(plan.max_suffix, std::max<int64_t>(1, kWaves / suffix_items)));
-  plan.suffix_split = s.split_len > 0 ? s.split_len : fits(len, 256);
+  plan.suffix_split = s.split_len > 0 ? s.split_len : fits(len, kSuffixPages);
   plan.prefix_parts = (plan.max_prefix + plan.prefix_split - 1) / plan.prefix_split;
   plan.suffix_parts = (plan.max_suffix + plan.suffix_split - 1) / plan.suffix_split;
   return plan;
@@ -175,12 +175,12 @@ const char* shared_refusal(const fa_fwd_params& p, const fa_paged_kv& kv, const 
   const SharedPlan plan = plan_shared(p, s, kv.page_size);
   const int64_t rows = (int64_t)p.heads_q / p.heads_kv * p.seqlen_q;
   auto slots = [&](int64_t len) { return (len - 1) / kv.page_size + 2; };
-  if (slots(plan.prefix_split) > (plan.fused ? kPrefixPages : 256) || slots(plan.suffix_split) > 256)
-    return "split_len too long for the page size: a partition may span at most 128 pages of 16-bit rows, 256 of FP8 ones";
+  if (slots(plan.prefix_split) > kPrefixPages || slots(plan.suffix_split) > kSuffixPages)
+    return "split_len too long for the page size: a partition may span at most 128 pages";
+  if (p.kv_dtype == FA_DTYPE_FP8_E4M3 && s.split_len > kFp8Keys) return "split_len must be at most 4096 keys of FP8 pools";
   const int64_t out_rows = (int64_t)p.batch * p.heads_q * p.seqlen_q;
-  const int64_t row_blocks = (rows + plan.suffix_waves * 32 - 1) / (plan.suffix_waves * 32);
-  if (out_rows > INT32_MAX / 2 || plan.prefix_blocks * p.heads_kv * plan.prefix_parts > INT32_MAX ||
-      ((int64_t)p.batch * p.heads_kv * plan.suffix_parts + 8) * row_blocks > INT32_MAX)
+  if (out_rows > INT32_MAX / 2 || plan.prefix_blocks * p.heads_kv * plan.prefix_parts > INT32_MAX / 2 ||
+      (int64_t)p.batch * p.heads_kv * plan.suffix_parts * ((rows + 31) / 32) > INT32_MAX / 2)
     return "grid too large";
   return nullptr;
 }
@@ -218,40 +218,20 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   const int rows = a.group * p.seqlen_q;
   const int64_t prefix_wgs = plan.prefix_blocks * p.heads_kv * plan.prefix_parts;
   hipError_t e = hipSuccess;
-  if (plan.fused) {
-    a.shared.prefix_wgs = (int32_t)prefix_wgs;
-    a.n_rowblk = (int32_t)plan.prefix_blocks;
-    a.shared.suffix_blocks = (rows + 31) / 32;
-    a.shared.by_page = FastDiv::by(kv.page_size);
-    a.shared.by_hkv = FastDiv::by(p.heads_kv);
-    a.shared.by_group = FastDiv::by(a.group);
-    a.shared.by_nq = FastDiv::by(p.seqlen_q);
-    a.shared.by_batch = FastDiv::by(p.batch);
-    a.shared.by_prefix_blocks = FastDiv::by(a.n_rowblk);
-    a.shared.by_suffix_blocks = FastDiv::by(a.shared.suffix_blocks);
-    a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts * a.shared.suffix_blocks);
-    a.total = (int32_t)(a.shared.prefix_wgs + ((int64_t)a.n_items + 3) / 4);
-    e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) { return launch_tiles<decltype(d)::value, decltype(t)>(a, stream); });
-    if (e != hipSuccess) return hip_status(e, err);
-  } else {
-    if (plan.prefix_parts > 0) {
-      a.split_len = plan.prefix_split;
-      a.n_split = a.n_chunk = plan.prefix_parts;
-      a.nk = plan.max_prefix;
-      a.n_rowblk = (int32_t)plan.prefix_blocks;
-      a.total = (int32_t)prefix_wgs;
-      e = launch_shared_split(a, p.head_dim, bf, fp8, true, plan.prefix_waves, stream);
-      if (e != hipSuccess) return hip_status(e, err);
-    }
-    a.split_len = plan.suffix_split;
-    a.n_split = a.n_chunk = plan.suffix_parts;
-    a.nk = plan.max_suffix;
-    a.n_rowblk = (rows + plan.suffix_waves * 32 - 1) / (plan.suffix_waves * 32);
-    a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts);
-    a.total = (int32_t)(((int64_t)a.n_items + 7) / 8 * 8 * a.n_rowblk);
-    e = launch_shared_split(a, p.head_dim, bf, fp8, false, plan.suffix_waves, stream);
-    if (e != hipSuccess) return hip_status(e, err);
-  }
+  a.shared.prefix_wgs = (int32_t)prefix_wgs;
+  a.n_rowblk = (int32_t)plan.prefix_blocks;
+  a.shared.suffix_blocks = (rows + 31) / 32;
+  a.shared.by_page = FastDiv::by(kv.page_size);
+  a.shared.by_hkv = FastDiv::by(p.heads_kv);
+  a.shared.by_group = FastDiv::by(a.group);
+  a.shared.by_nq = FastDiv::by(p.seqlen_q);
+  a.shared.by_batch = FastDiv::by(p.batch);
+  a.shared.by_prefix_blocks = FastDiv::by(a.n_rowblk);
+  a.shared.by_suffix_blocks = FastDiv::by(a.shared.suffix_blocks);
+  a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts * a.shared.suffix_blocks);
+  a.total = (int32_t)(a.shared.prefix_wgs + ((int64_t)a.n_items + 3) / 4);
+  e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) { return launch_tiles<decltype(d)::value, decltype(t)>(a, fp8, stream); });
+  if (e != hipSuccess) return hip_status(e, err);
 
   MergeArgs m{};
   m.part = (const float*)a.o;

@@ -12,7 +12,9 @@
 namespace fa {
 
 constexpr int kPrefixUnit = 64;
-constexpr int kPrefixPages = 128;  // pages that a partition of the shared keys may span
+constexpr int kPrefixPages = 128;  // pages that a partition of the shared keys may span,
+constexpr int kSuffixPages = 256;  // and one of a request's own
+constexpr int kFp8Keys = 64 * 64;  // keys of an FP8 partition: a lane holds a 64-key block's scales
 
 // Division of 0 <= n < 2^31 by a number that the host knows: (n * mul) >> shift.
 struct FastDiv {
@@ -138,9 +140,6 @@ __device__ __forceinline__ int prefix_holder(const int32_t* seqlens, int b0, int
   }
   return best;
 }
-
-// The split-K kernels over the shared keys (prefix) or the requests' own (fa_splitk.hip); nw: waves per workgroup.
-hipError_t launch_shared_split(const SharedTileArgs& a, int d, bool bf, bool fp8, bool prefix, int nw, hipStream_t stream);
 
 template <class F>
 hipError_t by_dim_and_type(int d, bool bf, F&& f) {

@@ -53,7 +53,6 @@
 
 #include "fa_device.hpp"
 #include "fa_internal.hpp"
-#include "fa_shared.hpp"
 #include "fa_tile.hpp"
 
 namespace fa {
@@ -84,19 +83,9 @@ __device__ __forceinline__ void wg_barrier() {
 // queries, 24 sequences of 4000 keys 164 -> 180 us; D=64, 4 queries, 16 up to 30000 114 -> 128).
 constexpr bool paged_dealt(int head_dim, bool fp8) { return !fp8 || head_dim == 256; }
 
-// Which keys a paged call's workgroups read (fa_shared.hpp): each request's own, those behind the ones that its group
-// shares, or the shared ones, for the rows of all requests of a group.
-enum Keys { kOwn = 0, kSuffix = 1, kPrefix = 2 };
-
-template <int KEYS>
-struct SplitkArgs {
-  using type = typename std::conditional<KEYS == kOwn, TileArgs, SharedTileArgs>::type;
-};
-
-template <int D, class E, class KV, int NW, int BN, bool PAGED, bool ONE_STAGE, int PGS, int KEYS = kOwn>
+template <int D, class E, class KV, int NW, int BN, bool PAGED, bool ONE_STAGE, int PGS>
 __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
-attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
-  static_assert(PAGED || KEYS == kOwn, "shared keys live in pages");
+attn_splitk_kernel(const TileArgs a) {
   using Shape = TileShape<D, BN>;    // 16-bit tiles
   using Shape8 = TileShape8<D, BN>;  // FP8 tiles
   constexpr bool IS_FP8 = KV::bytes == 1;
@@ -132,21 +121,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   // ---- work item: (batch, kv-head, chunk of ppw partitions, row block) -------------
   int rb, chunk, kvh, b;
   bool idle = false;  // grid padding: exits below, with the workgroups past a sequence's end
-  int b0 = 0, b1 = 0;  // kPrefix: the group's requests
-  int start = 0;       // the part's first key: kSuffix, the keys that the group shares
-  int seq_k = a.nk;
-  if constexpr (KEYS == kPrefix) {
-    // kv-head innermost (8 of them: one to an XCD, whose L2 then holds its keys), then the row blocks, which read the
-    // same keys at about the same time
-    int item = (int)blockIdx.x;
-    kvh = item % a.hkv;
-    item /= a.hkv;
-    rb = item % a.n_rowblk;
-    chunk = item / a.n_rowblk;
-    if (!group_of_block(a.shared, a.group * a.nq, NW * 32, rb, b0, b1, seq_k)) return;  // uniform over the workgroup
-    if (chunk * a.ppw * a.split_len >= seq_k) return;
-    b = prefix_holder(a.seqlens_k, b0, b1, seq_k);
-  } else if constexpr (PAGED && (paged_dealt(D, IS_FP8) || KEYS == kSuffix)) {
+  if constexpr (PAGED && paged_dealt(D, IS_FP8)) {
     // Sequences differ in length, so the items are dealt to the XCDs one by one (a contiguous range
     // each, as below, gives an XCD whole sequences, and the one with the longest runs on alone), chunk
     // outermost: the chunks past a short sequence's end, which have nothing to do, come last.  kv-head
@@ -182,19 +157,15 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   }
 
   const int seq_q = a.nq;
+  int seq_k = a.nk;
   // paged: this sequence's own length, clamped to the grid's [0, max length]
-  if constexpr (PAGED && KEYS == kOwn) seq_k = min(max(__builtin_amdgcn_readfirstlane(a.seqlens_k[b]), 0), a.nk);
-  if constexpr (KEYS == kSuffix) {
-    start = shared_keys_of(a.shared, b);
-    seq_k = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens_k[b]), start);
-  }
-  // rows: (q-head in group, query); kPrefix: of every request of the group
-  const int R = (KEYS == kPrefix ? b1 - b0 : 1) * a.group * seq_q;
+  if constexpr (PAGED) seq_k = min(max(__builtin_amdgcn_readfirstlane(a.seqlens_k[b]), 0), a.nk);
+  const int R = a.group * seq_q;  // rows: (q-head in group, query)
   const int r0 = rb * NW * 32;    // < R: the grid has ceil(R / (NW * 32)) row blocks
 
   const int part0 = chunk * a.ppw;
   const int part_end = min(part0 + a.ppw, a.n_split);
-  const int klo = start + part0 * a.split_len;
+  const int klo = part0 * a.split_len;
 
   // ---- lane roles ------------------------------------------------------------------
   const int tid = (int)threadIdx.x;
@@ -205,39 +176,16 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   const int row = wr0 + j;
   const bool row_ok = row < R;
   const bool wave_active = wr0 < R;
-  int hq = kvh * a.group + (row_ok ? row / seq_q : 0);
+  const int hq = kvh * a.group + (row_ok ? row / seq_q : 0);
   const int qi = row_ok ? row % seq_q : 0;
-  int bq = b;      // the row's request
-  int row_keys = 0;  // kPrefix: the shared keys that it sees
-  if constexpr (KEYS == kPrefix) {
-    const int in_group = row_ok ? row / seq_q : 0, member = in_group / a.group;
-    bq = b0 + member;
-    hq = kvh * a.group + (in_group - member * a.group);
-    const int n = keys_of(a.shared, a.seqlens_k[bq], seq_k);
-    row_keys = max(min(a.causal ? n - seq_q + qi + 1 : n, seq_k), 0);
-  }
 
   // The keys this workgroup and this wave see.  Paged: after the loads below, since it waits for the
   // sequence's length; a dense call has it ready and needs no such wait (there, late, it cost up to 3%).
   const int tiles_per_part = a.split_len / BN;  // split_len is a multiple of 64 (C ABI)
   int offset, khi, n_tiles, wave_khi, mask_from;
   auto visible_keys = [&]() __attribute__((always_inline)) {
-    if constexpr (KEYS == kPrefix) {
-      offset = 0;
-      khi = min(seq_k, part_end * a.split_len);
-      n_tiles = khi > klo ? (khi - klo + BN - 1) / BN : 0;
-      int most = row_ok ? row_keys : 0, least = row_ok ? row_keys : khi;
-#pragma unroll
-      for (int d = 32; d >= 1; d /= 2) {
-        most = max(most, __shfl_xor(most, d));
-        least = min(least, __shfl_xor(least, d));
-      }
-      wave_khi = min(khi, __builtin_amdgcn_readfirstlane(most));
-      mask_from = min(khi, __builtin_amdgcn_readfirstlane(least));
-      return;
-    }
     offset = seq_k - seq_q;  // bottom-right causal alignment (reference.py:24-33)
-    khi = min(seq_k, start + part_end * a.split_len);
+    khi = min(seq_k, part_end * a.split_len);
     if (a.causal) {
       // last query of the block (rows wrap around the queries once per q-head)
       const int re = min(r0 + NW * 32, R);
@@ -308,9 +256,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
     // length first cost every call 0.4 us); <= block_table_cols.
     // Issued before the Q loads: waiting for the entries then leaves Q in flight.
     first_slot = klo / a.page_size;
-    int kgrid = min(a.nk, part_end * a.split_len);
-    if constexpr (KEYS == kSuffix) kgrid = min(start + kgrid, a.shared.table_keys);
-    if constexpr (KEYS == kPrefix) kgrid = min(seq_k, part_end * a.split_len);
+    const int kgrid = min(a.nk, part_end * a.split_len);
     const int slot_end = kgrid > klo ? (kgrid - 1) / a.page_size + 1 : first_slot;
     const int32_t* bt = a.block_table + (int64_t)b * a.sbt;
 #pragma unroll
@@ -329,7 +275,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   // the loads stay unconditional and are all in flight together)
   u32x4 qf[KS];
   {
-    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)bq * a.sqb + (int64_t)hq * a.sqh + (int64_t)qi * a.sqn + 8 * g;
+    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)b * a.sqb + (int64_t)hq * a.sqh + (int64_t)qi * a.sqn + 8 * g;
     const uint32_t keep = row_ok ? 0xffffffffu : 0u;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = (ld16(qp + 16 * s) ^ qsign) & keep;
@@ -472,7 +418,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) voffs8[d] = r8 * D + (((2 * d + (grp & 1)) ^ Shape8::swz_v(r8)) * 16) + 8 * (lane & 1);
   }
-  const int qlim = KEYS == kPrefix ? row_keys - 1 : qi + offset;  // last key this lane's row may see (causal)
+  const int qlim = qi + offset;  // last key this lane's row may see (causal)
 
   // Partial of partition `part` in fp32, normalised by its row sum, plus its log2-domain
   // statistics (triton_splitk.py:90-96); then the state restarts for the next partition.
@@ -506,9 +452,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
       for (int c = lane; c < n16; c += 64) st16(op0 + 4 * c, ld16(sp + 4 * c));
       if (row_ok && g == 0) st8(a.ml + (prow0 + j) * 2, __builtin_bit_cast(u32x2, f32x2{m_run, l_tot}));
     } else if (wave_active && row_ok) {
-      int64_t prow = a.part_major ? prow0 + j : ((int64_t)(b * a.hq + hq) * seq_q + qi) * a.n_split + part;
-      if constexpr (KEYS != kOwn)
-        prow = ((int64_t)(bq * a.hq + hq) * seq_q + qi) * a.shared.part_stride + (KEYS == kSuffix ? a.shared.part_base : 0) + part;
+      const int64_t prow = a.part_major ? prow0 + j : ((int64_t)(b * a.hq + hq) * seq_q + qi) * a.n_split + part;
       float* op = (float*)a.o + prow * D;
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
@@ -622,7 +566,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int n = n0 + kb * 32 + 16 * (r >> 3) + 8 * g + (r & 7);
-          const bool ok = (n < khi) & (((KEYS != kPrefix) & (a.causal == 0)) | (n <= qlim));
+          const bool ok = (n < khi) & ((a.causal == 0) | (n <= qlim));
           sacc[kb][r] = ok ? sacc[kb][r] : NEG_INF;
         }
       }
@@ -808,7 +752,7 @@ attn_splitk_kernel(const typename SplitkArgs<KEYS>::type a) {
   // partitions past the visible keys (causal; dense: or past the sequence end): empty
   // partials, m = -inf and l = 0, which the combine weighs by zero
   for (int part = part0 + (n_tiles + tiles_per_part - 1) / tiles_per_part; part < part_end; ++part) {
-    if (PAGED && start + part * a.split_len >= seq_k) break;
+    if (PAGED && part * a.split_len >= seq_k) break;
     emit_partial(part);
   }
 }
@@ -1165,42 +1109,6 @@ fa_status run_splitk(const fa_fwd_params& p, int32_t split_len, void* workspace,
   c.slb = p.lse_stride_b;
   c.slh = p.lse_stride_h;
   return run_combine(c, p.head_dim, bf, out_rows, stream, err);
-}
-
-// ------------------------------------------------------------------------------------
-// Attention of requests that share the start of their keys
-// ------------------------------------------------------------------------------------
-
-template <int D, class E, class KV, int NW, int BN, bool ONE_STAGE, int KEYS>
-static hipError_t launch_shared_tiles(const SharedTileArgs& a, hipStream_t stream) {
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)a.total), dim3(NW * 64), 0, stream, a); };
-  if constexpr (KV::bytes == 2) {
-    if (a.page_size % 32 != 0) {
-      launch(attn_splitk_kernel<D, E, KV, NW, BN, true, ONE_STAGE, 16, KEYS>);
-      return hipGetLastError();
-    }
-  }
-  launch(attn_splitk_kernel<D, E, KV, NW, BN, true, ONE_STAGE, 32, KEYS>);
-  return hipGetLastError();
-}
-
-template <int D, class E, class KV, int KEYS>
-static hipError_t launch_shared_nw(const SharedTileArgs& a, int nw, hipStream_t stream) {
-  if (nw == 4) return launch_shared_tiles<D, E, KV, 4, (D == 256 ? 32 : 64), false, KEYS>(a, stream);
-  if (nw == 2) return launch_shared_tiles<D, E, KV, 2, 32, false, KEYS>(a, stream);
-  return launch_shared_tiles<D, E, KV, 1, 32, KV::bytes == 2, KEYS>(a, stream);
-}
-
-template <int D, class E>
-static hipError_t launch_shared(const SharedTileArgs& a, bool fp8, bool prefix, int nw, hipStream_t stream) {
-  if (fp8) return prefix ? launch_shared_nw<D, E, FP8, kPrefix>(a, nw, stream) : launch_shared_nw<D, E, FP8, kSuffix>(a, nw, stream);
-  return prefix ? launch_shared_nw<D, E, E, kPrefix>(a, nw, stream) : launch_shared_nw<D, E, E, kSuffix>(a, nw, stream);
-}
-
-hipError_t launch_shared_split(const SharedTileArgs& a, int d, bool bf, bool fp8, bool prefix, int nw, hipStream_t stream) {
-  return by_dim_and_type(d, bf, [&](auto dim, auto type) {
-    return launch_shared<decltype(dim)::value, decltype(type)>(a, fp8, prefix, nw, stream);
-  });
 }
 
 }  // namespace fa
