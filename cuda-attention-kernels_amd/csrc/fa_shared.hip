@@ -151,20 +151,24 @@ SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int pa
   // D = 128, alone on its CU or one of two) and leaves 128 rows of partials; one a CU leaves the CU's other place to the
   // requests' own keys.  So: as many as there are CUs, half as many where those would have fewer than 1024 keys each (64
   // requests of 4 rows, 8 kv-heads, 8192 keys: the call takes 42 us at 512 keys, 37 at 1024; 32 of 16 rows, 16384 keys, 66
-  // at 2048 and 86 at 4096).  Own keys: 1024 waves, four a CU, but no more than kLongest keys each, for the last to start
-  // not to run on alone (256 requests of up to 1000 keys, D = 64: 95 us whole, 91 in two).
-  constexpr int64_t kWgs = 256, kLong = 1024, kWaves = 1024, kLongest = 576;
+  // at 2048 and 86 at 4096).  A group has a block at least; which ones have more, and how long their prefixes are, is not
+  // known here.  Own keys: 1024 waves, four a CU (512 at D = 256: 49 requests of up to 700 keys, 4 kv-heads, 55 us at 192
+  // keys, 47 at 320), but no more than 576 keys each, for the last to start not to run on alone, and 320 where there are
+  // many (256 requests of up to 1000 keys, 8 kv-heads, D = 64: 95 us whole, 91 at 576, 88 at 320; 32 of up to 2000: 66 at
+  // 576, 72 at 320).
+  constexpr int64_t kWgs = 256, kLong = 1024, kWaves = 1024;
   auto whole = [](int64_t keys, int64_t parts) { return ((keys + parts - 1) / parts + kPrefixUnit - 1) / kPrefixUnit * kPrefixUnit; };
   auto fits = [&](int64_t len, int64_t pages) {  // a partition spans a limited number of pages, and of FP8 scale blocks
     len = std::min(len, (pages - 2) * page_size / kPrefixUnit * kPrefixUnit);
     return (int32_t)std::max<int64_t>(kPrefixUnit, fp8 ? std::min<int64_t>(len, kFp8Keys) : len);
   };
-  const int64_t prefix_items = p.heads_kv * ((all_rows + block - 1) / block);
+  const int64_t prefix_items = p.heads_kv * std::max<int64_t>((all_rows + block - 1) / block, s.num_groups);
   int64_t len = whole(plan.max_prefix, std::max<int64_t>(1, kWgs / prefix_items));
   if (len < kLong) len = std::min(kLong, whole(plan.max_prefix, std::max<int64_t>(1, kWgs / 2 / prefix_items)));
   plan.prefix_split = s.split_len > 0 ? s.split_len : fits(len, kPrefixPages);
   const int64_t suffix_items = (int64_t)p.batch * p.heads_kv * ((rows + 31) / 32);
-  len = std::min(kLongest, whole(plan.max_suffix, std::max<int64_t>(1, kWaves / suffix_items)));
+  len = whole(plan.max_suffix, std::max<int64_t>(1, (p.head_dim == 256 ? kWaves / 2 : kWaves) / suffix_items));
+  len = std::min<int64_t>(len, suffix_items <= kWaves / 4 ? 576 : 320);
   plan.suffix_split = s.split_len > 0 ? s.split_len : fits(len, kSuffixPages);
   plan.prefix_parts = (plan.max_prefix + plan.prefix_split - 1) / plan.prefix_split;
   plan.suffix_parts = (plan.max_suffix + plan.suffix_split - 1) / plan.suffix_split;

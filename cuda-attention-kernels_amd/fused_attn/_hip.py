@@ -1473,8 +1473,7 @@ def allocate_pages(block_table, seqlens_k, new_lens, free_pages, num_free, page_
     seqlens_k, new_lens = seqlens_k.contiguous(), new_lens.contiguous()
     dev = block_table.device
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    small = torch.empty(2 * b + 2, dtype=torch.int32, device=dev)  # one allocation for the three small outputs
-    cu, lens, left = small[:b + 1], small[b + 1:2 * b + 1], small[2 * b + 1:].view(num_free.shape)
+    cu, lens, left = torch.empty(b + 1, dtype=torch.int32, device=dev), torch.empty_like(seqlens_k), torch.empty_like(num_free)
     p = _pages_params(block_table, seqlens_k, free_pages, num_free, page_size, num_tokens)
     p.new_lens, p.slots, p.cu_seqlens = new_lens.data_ptr(), slots.data_ptr(), cu.data_ptr()
     p.seqlens_out, p.num_free_out = lens.data_ptr(), left.data_ptr()
@@ -1490,41 +1489,48 @@ def release_pages(block_table, seqlens_k, done, free_pages, num_free, page_size:
     lib = _pages_library()
     block_table, seqlens_k, done = _plain_table(block_table), seqlens_k.contiguous(), done.contiguous()
     keep_lens = None if keep_lens is None else keep_lens.contiguous()
-    b, dev = block_table.shape[0], block_table.device
-    small = torch.empty(b + 1, dtype=torch.int32, device=dev)
-    lens, left = small[:b], small[b:].view(num_free.shape)
+    lens, left = torch.empty_like(seqlens_k), torch.empty_like(num_free)
     p = _pages_params(block_table, seqlens_k, free_pages, num_free, page_size)
     p.done, p.keep_lens = done.data_ptr(), None if keep_lens is None else keep_lens.data_ptr()
     p.seqlens_out, p.num_free_out = lens.data_ptr(), left.data_ptr()
-    with _on_device(dev):
+    with _on_device(block_table.device):
         _check(lib.fa_release_pages(p, _stream(block_table)), "release_pages")
     return lens, left
 
 
+def _pool_writable(pool: torch.Tensor) -> bool:
+    """Whether a 16-bit pool can be written in place in 16-byte pieces."""
+    if pool.data_ptr() % 16:
+        return False
+    if pool.is_contiguous():
+        return True
+    z, st = pool.shape, pool.stride()
+    return st[3] == 1 and all(z[i] <= 1 or (st[i] > 0 and st[i] % 8 == 0) for i in range(3))
+
+
 def check_append_paged(k, v, k_cache, v_cache, slots) -> None:
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
-        raise RuntimeError(f"k and v must both be [T, Hkv, D] of one type, got {k.dtype} {tuple(k.shape)} and "
-                           f"{v.dtype} {tuple(v.shape)}")
-    if k.dtype not in (torch.float16, torch.bfloat16):
-        raise RuntimeError(f"k and v must be float16 or bfloat16, got {k.dtype}")
-    if k.shape[2] % 8:
-        raise RuntimeError(f"D must be a multiple of 8, got {k.shape[2]}")
+    ks, dtype, dev = k.shape, k.dtype, k.device
+    if len(ks) != 3 or ks != v.shape or dtype != v.dtype:
+        raise RuntimeError(f"k and v must both be [T, Hkv, D] of one type, got {dtype} {tuple(ks)} and {v.dtype} {tuple(v.shape)}")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"k and v must be float16 or bfloat16, got {dtype}")
+    if ks[2] % 8:
+        raise RuntimeError(f"D must be a multiple of 8, got {ks[2]}")
     for name, pool in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if pool.dim() != 4 or pool.dtype != k.dtype or (pool.shape[1], pool.shape[3]) != tuple(k.shape[1:]):
-            raise RuntimeError(f"{name} must be {k.dtype} [num_pages, {k.shape[1]}, page_size, {k.shape[2]}], got {pool.dtype} "
-                               f"{tuple(pool.shape)}")
+        z = pool.shape
+        if len(z) != 4 or pool.dtype != dtype or z[1] != ks[1] or z[3] != ks[2]:
+            raise RuntimeError(f"{name} must be {dtype} [num_pages, {ks[1]}, page_size, {ks[2]}], got {pool.dtype} {tuple(z)}")
         # written in place: it cannot be copied into another layout first
-        if pool.numel() and (pool.stride(3) != 1 or pool.data_ptr() % 16
-                             or any(pool.size(i) > 1 and (pool.stride(i) <= 0 or pool.stride(i) % 8) for i in range(3))):
+        if pool.numel() and not _pool_writable(pool):
             raise RuntimeError(f"{name} needs a unit D stride, a 16-byte aligned start and strides of whole 16 bytes")
     if k_cache.shape != v_cache.shape:
         raise RuntimeError(f"k_cache and v_cache must have the same shape, got {tuple(k_cache.shape)} and "
                            f"{tuple(v_cache.shape)}")
-    if slots.dtype != torch.int64 or tuple(slots.shape) != (k.shape[0],):
-        raise RuntimeError(f"slots must be int64 [{k.shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
+    if slots.dtype != torch.int64 or slots.shape != ks[:1]:
+        raise RuntimeError(f"slots must be int64 [{ks[0]}], got {slots.dtype} {tuple(slots.shape)}")
     for t in (v, k_cache, v_cache, slots):
-        if t.device != k.device:
-            raise RuntimeError(f"all tensors must be on {k.device}, got {t.device}")
+        if t.device != dev:
+            raise RuntimeError(f"all tensors must be on {dev}, got {t.device}")
 
 
 def append_kv_paged(k, v, k_cache, v_cache, slots) -> None:

@@ -52,10 +52,11 @@ def test_abi():
     p = _hip.FwdParams(16, 16, 16, 16, 4 * 128, 128, 128, 0, 64, 128, 0, 64, 128, 4 * 128, 128, 128, 5, 4, 2, 1, 0, 128, 0.1, 0,
                        _hip.BF16, _hip.BF16)
     kv = _hip.PagedKV(16, 4, 4, 64, 16, 9, 0, 8192, 8192)
-    s = _hip.SharedPrefix(16, 16, 2, 100, 50, 0)
+    s = _hip.SharedPrefix(16, 16, 2, 100, 50, 128)
     need = lib.fa_shared_prefix_workspace_bytes(p, kv, s)
     # one partition of the prefix and one of the own keys: partials, maxima and sums of 20 rows
     assert need == 20 * 2 * (128 + 2) * 4
+    assert lib.fa_shared_prefix_workspace_bytes(p, kv, _hip.SharedPrefix(16, 16, 2, 100, 50, 0)) >= need
 
     def status(ws=16, nbytes=need, **kw):
         ps = [type(x).from_buffer_copy(x) for x in (p, kv, s)]
