@@ -75,7 +75,7 @@ def _torch_commands() -> list[list[str]]:
                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", inc,
                 "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", rocm, "-isystem", python,
                 "-c", os.path.join(CSRC, TORCH_SOURCE), "-o", obj]
-    link = [HIPCC, "-shared", "-fPIC", obj, "-L", lib, "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-o",
+    link = [HIPCC, "-shared", "-fPIC", obj, "-L", lib, "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip", "-o",
             TORCH_OUT + ".tmp"]
     return [compile_, link]
 

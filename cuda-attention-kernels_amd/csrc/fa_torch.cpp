@@ -8,6 +8,9 @@
 //
 // The choice of kernel and partitions repeats ops._hip_kernel_for and ops.default_split_len
 // (fa_torch_route lets a test compare the two).
+//
+// fa_torch_shared_prefix, _allocate_pages, _release_pages and _append_kv_paged do the same for Python functions that are no
+// ops: they take the tensors as Python objects, and return None for what the Python code is to handle.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -15,12 +18,15 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
+#include <initializer_list>
+#include <vector>
 
 #include "../../include/fused_attn_hip.h"
 
@@ -36,6 +42,17 @@ struct Abi {
   const char* (*last_error)();
 };
 Abi g_abi{};
+struct SharedAbi {
+  size_t (*workspace_bytes)(const fa_fwd_params*, const fa_paged_kv*, const fa_shared_prefix*);
+  fa_status (*call)(const fa_fwd_params*, const fa_paged_kv*, const fa_shared_prefix*, void*, size_t, void*);
+};
+SharedAbi g_shared{};
+struct PagesAbi {
+  fa_status (*allocate)(const fa_pages_params*, void*);
+  fa_status (*release)(const fa_pages_params*, void*);
+  fa_status (*append)(const fa_append_paged_params*, void*);
+};
+PagesAbi g_pages{};
 std::atomic<uint64_t> g_devices{0};
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -176,6 +193,257 @@ at::Tensor attention_gpu(const at::Tensor& q, const at::Tensor& k, const at::Ten
   return o;
 }
 
+// Rows of whole 16-byte pieces, as `readable`, for elements of any size.
+bool readable_rows(const at::Tensor& t) {
+  const int64_t size = (int64_t)t.element_size();
+  if (t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0) return false;
+  for (int i = 0; i < 3; ++i) {
+    if (t.size(i) > INT32_MAX || (t.size(i) > 1 && t.stride(i) * size % 16 != 0)) return false;
+  }
+  return t.size(2) <= 1 || t.stride(2) * size < (int64_t{1} << 24);
+}
+
+// An int32 vector of n on dev that can be read as it is.
+bool int32s(const at::Tensor& t, int64_t n, const c10::Device& dev) {
+  return t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kInt && t.device() == dev && (n <= 1 || t.stride(0) == 1);
+}
+
+bool enabled(const c10::Device& dev) {
+  const int i = dev.is_cuda() ? dev.index() : -1;
+  return i >= 0 && i < 64 && ((g_devices.load(std::memory_order_acquire) >> i) & 1);
+}
+
+void* stream_of(const c10::Device& dev) { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream(); }
+
+// The parameters that allocate_pages and release_pages share; false for operands that need preparation.
+bool pages_params(const at::Tensor& table, const at::Tensor& seqlens, const at::Tensor& free_pages, const at::Tensor& num_free,
+                  int64_t page_size, int64_t num_tokens, fa_pages_params& p) {
+  const c10::Device dev = table.device();
+  if (!enabled(dev) || table.dim() != 2 || table.scalar_type() != at::kInt) return false;
+  const int64_t b = table.size(0), cols = table.size(1);
+  if (b == 0 || cols == 0 || b > INT32_MAX || cols > INT32_MAX || (cols > 1 && table.stride(1) != 1) || (b > 1 && table.stride(0) < cols))
+    return false;
+  if (!int32s(seqlens, b, dev) || free_pages.dim() != 1 || !int32s(free_pages, free_pages.size(0), dev)) return false;
+  if (num_free.numel() != 1 || num_free.scalar_type() != at::kInt || num_free.device() != dev) return false;
+  if (page_size <= 0 || page_size > FA_MAX_PAGE_SIZE || num_tokens < 0 || num_tokens >= INT32_MAX || free_pages.size(0) >= INT32_MAX)
+    return false;
+  p.block_table = (int32_t*)table.const_data_ptr();
+  p.block_table_stride = b > 1 ? table.stride(0) : 0;
+  p.batch = (int32_t)b;
+  p.block_table_cols = (int32_t)cols;
+  p.page_size = (int32_t)page_size;
+  p.free_capacity = (int32_t)free_pages.size(0);
+  p.num_tokens = (int32_t)num_tokens;
+  p.seqlens = (const int32_t*)seqlens.const_data_ptr();
+  p.free_pages = (int32_t*)free_pages.const_data_ptr();
+  p.num_free = (const int32_t*)num_free.const_data_ptr();
+  return !backend_forced();
+}
+
+// (slots, cu_seqlens, seqlens, num_free), or nothing.
+std::vector<at::Tensor> allocate_pages(const at::Tensor& table, const at::Tensor& seqlens, const at::Tensor& new_lens,
+                                       const at::Tensor& free_pages, const at::Tensor& num_free, int64_t page_size, int64_t num_tokens) {
+  fa_pages_params p{};
+  if (!pages_params(table, seqlens, free_pages, num_free, page_size, num_tokens, p) || !int32s(new_lens, p.batch, table.device()))
+    return {};
+  const c10::DeviceGuard guard(table.device());
+  std::vector<at::Tensor> out{at::empty({num_tokens}, table.options().dtype(at::kLong)), at::empty({p.batch + 1}, table.options()),
+                              at::empty({p.batch}, table.options()), at::empty(num_free.sizes(), table.options())};
+  p.new_lens = (const int32_t*)new_lens.const_data_ptr();
+  p.slots = (int64_t*)out[0].mutable_data_ptr();
+  p.cu_seqlens = (int32_t*)out[1].mutable_data_ptr();
+  p.seqlens_out = (int32_t*)out[2].mutable_data_ptr();
+  p.num_free_out = (int32_t*)out[3].mutable_data_ptr();
+  if (g_pages.allocate(&p, stream_of(table.device())) != FA_OK) return {};
+  return out;
+}
+
+// (seqlens, num_free), or nothing.
+std::vector<at::Tensor> release_pages(const at::Tensor& table, const at::Tensor& seqlens, const at::Tensor& done,
+                                      const at::Tensor& free_pages, const at::Tensor& num_free, const at::Tensor& keep_lens,
+                                      int64_t page_size) {
+  fa_pages_params p{};
+  if (!pages_params(table, seqlens, free_pages, num_free, page_size, 0, p)) return {};
+  if (done.dim() != 1 || done.size(0) != p.batch || done.device() != table.device() || (p.batch > 1 && done.stride(0) != 1) ||
+      (done.scalar_type() != at::kBool && done.scalar_type() != at::kByte))
+    return {};
+  if (keep_lens.defined() && !int32s(keep_lens, p.batch, table.device())) return {};
+  const c10::DeviceGuard guard(table.device());
+  std::vector<at::Tensor> out{at::empty({p.batch}, table.options()), at::empty(num_free.sizes(), table.options())};
+  p.done = (const uint8_t*)done.const_data_ptr();
+  p.keep_lens = keep_lens.defined() ? (const int32_t*)keep_lens.const_data_ptr() : nullptr;
+  p.seqlens_out = (int32_t*)out[0].mutable_data_ptr();
+  p.num_free_out = (int32_t*)out[1].mutable_data_ptr();
+  if (g_pages.release(&p, stream_of(table.device())) != FA_OK) return {};
+  return out;
+}
+
+bool append_kv_paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& slots) {
+  const c10::Device dev = k.device();
+  if (!enabled(dev) || k.dim() != 3 || kc.dim() != 4 || !k.sizes().equals(v.sizes()) || !kc.sizes().equals(vc.sizes())) return false;
+  if (k.scalar_type() != at::kHalf && k.scalar_type() != at::kBFloat16) return false;
+  for (const at::Tensor* t : {&v, &kc, &vc}) {
+    if (t->scalar_type() != k.scalar_type() || t->device() != dev) return false;
+  }
+  if (k.numel() == 0 || kc.numel() == 0 || k.size(2) % 8 || kc.size(1) != k.size(1) || kc.size(3) != k.size(2)) return false;
+  if (slots.dim() != 1 || slots.size(0) != k.size(0) || slots.scalar_type() != at::kLong || slots.device() != dev ||
+      (slots.size(0) > 1 && slots.stride(0) != 1))
+    return false;
+  auto in_pieces = [](const at::Tensor& t, bool written) {  // unit stride along D, whole 16 bytes
+    const int64_t last = t.dim() - 1;
+    if (t.stride(last) != 1 || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0) return false;
+    for (int64_t i = 0; i < last; ++i) {
+      if (t.size(i) > INT32_MAX || (t.size(i) > 1 && (t.stride(i) % 8 != 0 || (written && t.stride(i) <= 0)))) return false;
+    }
+    return true;
+  };
+  if (!in_pieces(k, false) || !in_pieces(v, false) || !in_pieces(kc, true) || !in_pieces(vc, true) || backend_forced()) return false;
+  auto step = [](const at::Tensor& x, int i) { return x.size(i) > 1 ? x.stride(i) : 0; };
+  fa_append_paged_params p{};
+  p.k = k.const_data_ptr();
+  p.v = v.const_data_ptr();
+  p.k_stride_t = step(k, 0), p.k_stride_h = step(k, 1);
+  p.v_stride_t = step(v, 0), p.v_stride_h = step(v, 1);
+  p.k_cache = kc.mutable_data_ptr();
+  p.v_cache = vc.mutable_data_ptr();
+  p.k_page_stride = step(kc, 0), p.k_cache_stride_h = step(kc, 1), p.k_cache_stride_n = step(kc, 2);
+  p.v_page_stride = step(vc, 0), p.v_cache_stride_h = step(vc, 1), p.v_cache_stride_n = step(vc, 2);
+  p.slots = (const int64_t*)slots.const_data_ptr();
+  p.num_tokens = (int32_t)k.size(0);
+  p.heads = (int32_t)k.size(1);
+  p.head_dim = (int32_t)k.size(2);
+  p.num_pages = (int32_t)kc.size(0);
+  p.page_size = (int32_t)kc.size(2);
+  const c10::DeviceGuard guard(dev);
+  return g_pages.append(&p, stream_of(dev)) == FA_OK;
+}
+
+struct SharedCall {
+  at::Tensor q, k, v, table, seqlens, prefix_lens, cu_groups, k_scale, v_scale;  // the last four may be undefined
+  int64_t max_prefix, max_suffix;
+  bool causal;
+  double scale;
+  int32_t split_len;
+};
+
+// The call's output; undefined where it needs preparation or is refused.
+at::Tensor shared_prefix(const SharedCall& c) {
+  const at::Tensor &q = c.q, &k = c.k, &v = c.v;
+  if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !q.is_cuda()) return {};
+  const c10::Device dev = q.device();
+  if (!enabled(dev)) return {};
+  if (k.device() != dev || v.device() != dev || c.table.device() != dev) return {};
+  const bool fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
+  if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) return {};
+  if ((!fp8 && k.scalar_type() != q.scalar_type()) || v.scalar_type() != k.scalar_type()) return {};
+  if (q.numel() == 0 || k.numel() == 0 || !k.sizes().equals(v.sizes()) || k.size(3) != q.size(3) || q.size(1) % k.size(1) != 0) return {};
+  const int64_t b = q.size(0), page = k.size(2);
+  const at::Tensor& t = c.table;
+  if (t.dim() != 2 || t.scalar_type() != at::kInt || t.size(0) != b || t.size(1) == 0 || t.size(1) > INT32_MAX ||
+      (t.size(1) > 1 && t.stride(1) != 1) || (b > 1 && t.stride(0) < t.size(1)))
+    return {};
+  if (!int32s(c.seqlens, b, dev)) return {};
+  int64_t groups = 1;
+  if (c.cu_groups.defined()) {
+    groups = c.cu_groups.numel() - 1;
+    if (groups < 1 || groups > b || !int32s(c.cu_groups, groups + 1, dev)) return {};
+  }
+  if (c.prefix_lens.defined() && !int32s(c.prefix_lens, groups, dev)) return {};
+  if (c.max_prefix < 0 || c.max_suffix < 0 || c.max_prefix > (1 << 29) || c.max_suffix > (1 << 29)) return {};
+  if (!readable_rows(q) || !readable_rows(k) || !readable_rows(v)) return {};
+  if (fp8) {
+    if (page % 64 != 0 || !c.k_scale.defined() || !c.v_scale.defined()) return {};
+    const int64_t want[3] = {k.size(0), k.size(1), page / 64};
+    for (const at::Tensor* s : {&c.k_scale, &c.v_scale}) {
+      if (s->scalar_type() != at::kFloat || s->device() != dev || !s->sizes().equals(at::IntArrayRef(want, 3)) || s->stride(2) != 1)
+        return {};
+    }
+    if (!c.k_scale.strides().equals(c.v_scale.strides())) return {};
+  }
+  if (backend_forced()) return {};
+
+  const c10::DeviceGuard guard(dev);
+  at::Tensor o = at::empty(q.sizes(), q.options());
+  auto step = [](const at::Tensor& x, int i) { return x.size(i) > 1 ? x.stride(i) : 0; };
+  fa_fwd_params p{};
+  p.q = q.const_data_ptr();
+  p.k = k.const_data_ptr();
+  p.v = v.const_data_ptr();
+  p.o = o.mutable_data_ptr();
+  p.q_stride_b = step(q, 0), p.q_stride_h = step(q, 1), p.q_stride_n = step(q, 2);
+  p.k_stride_h = step(k, 1), p.k_stride_n = step(k, 2);
+  p.v_stride_h = step(v, 1), p.v_stride_n = step(v, 2);
+  p.o_stride_b = step(o, 0), p.o_stride_h = step(o, 1), p.o_stride_n = step(o, 2);
+  p.batch = (int32_t)b;
+  p.heads_q = (int32_t)q.size(1);
+  p.heads_kv = (int32_t)k.size(1);
+  p.seqlen_q = (int32_t)q.size(2);
+  p.head_dim = (int32_t)q.size(3);
+  p.scale = (float)c.scale;
+  p.causal = c.causal ? 1 : 0;
+  p.dtype = dtype_code(q.scalar_type());
+  p.kv_dtype = fp8 ? FA_DTYPE_FP8_E4M3 : p.dtype;
+  if (fp8) {
+    p.k_scale = (const float*)c.k_scale.const_data_ptr();
+    p.v_scale = (const float*)c.v_scale.const_data_ptr();
+    p.scale_stride_b = c.k_scale.stride(0);
+    p.scale_stride_h = c.k_scale.stride(1);
+  }
+  fa_paged_kv kv{};
+  kv.block_table = (const int32_t*)t.const_data_ptr();
+  kv.block_table_stride = t.stride(0);
+  kv.block_table_cols = (int32_t)t.size(1);
+  kv.page_size = (int32_t)page;
+  kv.seqlens_k = (const int32_t*)c.seqlens.const_data_ptr();
+  kv.num_pages = (int32_t)k.size(0);
+  kv.k_page_stride = step(k, 0);
+  kv.v_page_stride = step(v, 0);
+  fa_shared_prefix s{};
+  s.prefix_lens = c.prefix_lens.defined() ? (const int32_t*)c.prefix_lens.const_data_ptr() : nullptr;
+  s.cu_groups = c.cu_groups.defined() ? (const int32_t*)c.cu_groups.const_data_ptr() : nullptr;
+  s.num_groups = (int32_t)groups;
+  s.max_prefix_len = (int32_t)c.max_prefix;
+  s.max_suffix_len = (int32_t)c.max_suffix;
+  s.split_len = c.split_len;
+  const size_t need = g_shared.workspace_bytes(&p, &kv, &s);
+  if (need == 0) return {};  // refused: the Python code reports it
+  const at::Tensor ws = at::empty({(int64_t)(need / 4)}, q.options().dtype(at::kFloat));
+  return g_shared.call(&p, &kv, &s, ws.mutable_data_ptr(), need, stream_of(dev)) == FA_OK ? o : at::Tensor();
+}
+
+// What f makes of tensors (those in `maybe` may be None), or None.  Nothing is thrown and no Python error is left: what
+// fails here (memory, say) fails again in the Python code, which reports it.
+template <class F>
+PyObject* with_tensors(std::initializer_list<PyObject*> always, std::initializer_list<PyObject*> maybe, F&& f) {
+  try {
+    for (PyObject* o : always) {
+      if (!THPVariable_CheckExact(o)) Py_RETURN_NONE;
+    }
+    for (PyObject* o : maybe) {
+      if (o != Py_None && !THPVariable_CheckExact(o)) Py_RETURN_NONE;
+    }
+    if (PyObject* out = f()) return out;
+  } catch (const std::exception&) {
+  }
+  PyErr_Clear();
+  Py_RETURN_NONE;
+}
+
+at::Tensor tensor_or_none(PyObject* o) { return o == Py_None ? at::Tensor() : THPVariable_Unpack(o); }
+
+PyObject* tuple_of(const std::vector<at::Tensor>& out) {
+  PyObject* t = out.empty() ? nullptr : PyTuple_New((Py_ssize_t)out.size());
+  for (size_t i = 0; t != nullptr && i < out.size(); ++i) {
+    PyObject* o = THPVariable_Wrap(out[i]);
+    if (o == nullptr) {
+      Py_DECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, (Py_ssize_t)i, o);
+  }
+  return t;
+}
+
 // Autograd: the op has no formula of its own, so a call that would record one goes to the Python kernel, which
 // records the node that the op's users registered, or one that raises.
 at::Tensor attention_autograd(c10::DispatchKeySet ks, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool causal,
@@ -216,6 +484,57 @@ void fa_torch_bind(void* fwd_workspace_bytes, void* fwd_ws, void* splitk_workspa
   g_abi.splitk_workspace_bytes = (decltype(g_abi.splitk_workspace_bytes))splitk_workspace_bytes;
   g_abi.splitk = (decltype(g_abi.splitk))splitk;
   g_abi.last_error = (decltype(g_abi.last_error))last_error;
+}
+
+void fa_torch_bind_shared(void* workspace_bytes, void* call) {
+  g_shared.workspace_bytes = (decltype(g_shared.workspace_bytes))workspace_bytes;
+  g_shared.call = (decltype(g_shared.call))call;
+}
+
+// attention_shared_prefix of tensors (the last four may be None) that need no preparation: its output, or None.  Called
+// with the GIL held; nothing is thrown and no Python error is set.
+PyObject* fa_torch_shared_prefix(PyObject* q, PyObject* k, PyObject* v, PyObject* table, PyObject* seqlens, PyObject* prefix_lens,
+                                 PyObject* cu_groups, PyObject* k_scale, PyObject* v_scale, int64_t max_prefix,
+                                 int64_t max_suffix, int32_t causal, double scale, int32_t split_len) {
+  return with_tensors({q, k, v, table, seqlens}, {prefix_lens, cu_groups, k_scale, v_scale}, [&]() -> PyObject* {
+    const at::Tensor out = shared_prefix({THPVariable_Unpack(q), THPVariable_Unpack(k), THPVariable_Unpack(v), THPVariable_Unpack(table),
+                                          THPVariable_Unpack(seqlens), tensor_or_none(prefix_lens), tensor_or_none(cu_groups),
+                                          tensor_or_none(k_scale), tensor_or_none(v_scale), max_prefix, max_suffix, causal != 0, scale,
+                                          split_len});
+    return out.defined() ? THPVariable_Wrap(out) : nullptr;
+  });
+}
+
+void fa_torch_bind_pages(void* allocate, void* release, void* append) {
+  g_pages.allocate = (decltype(g_pages.allocate))allocate;
+  g_pages.release = (decltype(g_pages.release))release;
+  g_pages.append = (decltype(g_pages.append))append;
+}
+
+// The same for allocate_pages (a tuple), release_pages (keep_lens may be None; a tuple) and append_kv_paged (True).
+PyObject* fa_torch_allocate_pages(PyObject* table, PyObject* seqlens, PyObject* new_lens, PyObject* free_pages, PyObject* num_free,
+                                  int64_t page_size, int64_t num_tokens) {
+  return with_tensors({table, seqlens, new_lens, free_pages, num_free}, {}, [&] {
+    return tuple_of(allocate_pages(THPVariable_Unpack(table), THPVariable_Unpack(seqlens), THPVariable_Unpack(new_lens),
+                                   THPVariable_Unpack(free_pages), THPVariable_Unpack(num_free), page_size, num_tokens));
+  });
+}
+
+PyObject* fa_torch_release_pages(PyObject* table, PyObject* seqlens, PyObject* done, PyObject* free_pages, PyObject* num_free,
+                                 PyObject* keep_lens, int64_t page_size) {
+  return with_tensors({table, seqlens, done, free_pages, num_free}, {keep_lens}, [&] {
+    return tuple_of(release_pages(THPVariable_Unpack(table), THPVariable_Unpack(seqlens), THPVariable_Unpack(done),
+                                  THPVariable_Unpack(free_pages), THPVariable_Unpack(num_free), tensor_or_none(keep_lens), page_size));
+  });
+}
+
+PyObject* fa_torch_append_kv_paged(PyObject* k, PyObject* v, PyObject* k_cache, PyObject* v_cache, PyObject* slots) {
+  return with_tensors({k, v, k_cache, v_cache, slots}, {}, [&]() -> PyObject* {
+    if (!append_kv_paged(THPVariable_Unpack(k), THPVariable_Unpack(v), THPVariable_Unpack(k_cache), THPVariable_Unpack(v_cache),
+                         THPVariable_Unpack(slots)))
+      return nullptr;
+    Py_RETURN_TRUE;
+  });
 }
 
 // Device `index` runs the library bound above (which happens before).

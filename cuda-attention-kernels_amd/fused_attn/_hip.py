@@ -427,6 +427,7 @@ def library_loaded() -> bool:
 TORCH_LIB_NAME = "libfused_attn_torch.so"
 _native: Optional[ctypes.CDLL] = None
 _native_devices: set[int] = set()
+native = None  # calls of Python functions that need no preparation (NativeFunctions), once a device is enabled
 
 
 def load_native() -> None:
@@ -457,11 +458,41 @@ def load_native() -> None:
     lib.fa_torch_enable.restype = None
     lib.fa_torch_route.argtypes = [ctypes.c_int32] + [ctypes.c_int64] * 6
     lib.fa_torch_route.restype = ctypes.c_int64
+    if _has_native_functions(lib):
+        lib.fa_torch_bind_shared.argtypes, lib.fa_torch_bind_shared.restype = [ctypes.c_void_p] * 2, None
+        lib.fa_torch_bind_pages.argtypes, lib.fa_torch_bind_pages.restype = [ctypes.c_void_p] * 3, None
     _native = lib
+
+
+def _has_native_functions(lib: ctypes.CDLL) -> bool:
+    return isinstance(getattr(lib, "fa_torch_allocate_pages", None), lib._FuncPtr)
+
+
+class NativeFunctions:
+    """fa_torch_*: each returns None for a call that Python has to prepare or refuse."""
+
+    def __init__(self, lib):
+        obj, i64 = ctypes.py_object, ctypes.c_int64
+        for name, args in (("shared_prefix", [obj] * 9 + [i64] * 2 + [ctypes.c_int32, ctypes.c_double, ctypes.c_int32]),
+                           ("allocate_pages", [obj] * 5 + [i64] * 2), ("release_pages", [obj] * 6 + [i64]),
+                           ("append_kv_paged", [obj] * 5)):
+            f = getattr(lib, "fa_torch_" + name)
+            f.argtypes, f.restype = args, obj
+            setattr(self, name, f)
+
+
+def _bind_native_functions(hip: ctypes.CDLL) -> NativeFunctions:
+    def pointers(*fs):
+        return (ctypes.cast(f, ctypes.c_void_p) for f in fs)
+
+    _native.fa_torch_bind_shared(*pointers(hip.fa_shared_prefix_workspace_bytes, hip.fa_attention_shared_prefix))
+    _native.fa_torch_bind_pages(*pointers(hip.fa_allocate_pages, hip.fa_release_pages, hip.fa_append_kv_paged))
+    return NativeFunctions(ctypes.PyDLL(_native._name))  # (PyDLL keeps the GIL: they take Python objects)
 
 
 def _enable_native(index: int) -> None:
     """Let the native kernels serve device ``index``, which ``device_supported`` has accepted."""
+    global native
     hip = load_library()
     with _lock:
         if _native is not None and _has_fwd_workspace(hip):
@@ -469,6 +500,8 @@ def _enable_native(index: int) -> None:
                 _native.fa_torch_bind(*(ctypes.cast(f, ctypes.c_void_p) for f in (
                     hip.fa_attention_fwd_workspace_bytes, hip.fa_attention_fwd_ws, hip.fa_splitk_workspace_bytes,
                     hip.fa_attention_splitk, hip.fa_last_error)))
+                if _has_pages(hip) and _has_native_functions(_native):
+                    native = _bind_native_functions(hip)
             _native.fa_torch_enable(index)
         _native_devices.add(index)
 

@@ -41,6 +41,9 @@ def allocate_pages(block_table: torch.Tensor, seqlens_k: torch.Tensor, new_lens:
     columns, whose tokens would pass num_tokens, or that needs pages when too few are left for it and those before it,
     keeps its length and its row, and its tokens have slot -1."""
     args = (block_table, seqlens_k, new_lens, free_pages, num_free, int(page_size), int(num_tokens))
+    out = None if _hip.native is None else _hip.native.allocate_pages(*args)
+    if out is not None:
+        return out
     if block_table.is_cuda and _pick_backend(block_table) == "hip":
         return _hip.allocate_pages(*args)
     _hip.check_pages(block_table, seqlens_k, free_pages, num_free, args[5], new_lens=new_lens, num_tokens=args[6])
@@ -81,6 +84,9 @@ def release_pages(block_table: torch.Tensor, seqlens_k: torch.Tensor, done: torc
     the list.  A request whose pages the list has no room for keeps them and its length.  ``block_table`` is not changed:
     a row's entries past its length mean nothing."""
     args = (block_table, seqlens_k, done, free_pages, num_free, int(page_size), keep_lens)
+    out = None if _hip.native is None else _hip.native.release_pages(*args[:5], keep_lens, args[5])
+    if out is not None:
+        return out
     if block_table.is_cuda and _pick_backend(block_table) == "hip":
         return _hip.release_pages(*args)
     _hip.check_pages(block_table, seqlens_k, free_pages, num_free, args[5], done=done, keep_lens=keep_lens)
@@ -103,6 +109,8 @@ def append_kv_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     multiple of 8.  A token with a slot outside [0, num_pages * page_size) is not written; no two may have the same one.
 
     (An FP8 pool shares a scale among 64 keys and cannot take single rows; 4-bit pools have ``append_kv_int4``.)"""
+    if _hip.native is not None and _hip.native.append_kv_paged(k, v, k_cache, v_cache, slots):
+        return
     if k.is_cuda and _pick_backend(k) == "hip":
         return _hip.append_kv_paged(k, v, k_cache, v_cache, slots)
     _hip.check_append_paged(k, v, k_cache, v_cache, slots)

@@ -42,6 +42,13 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     own are not read.  ``split_len``: keys per partition, a multiple of 64."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     number = not isinstance(prefix_lens, torch.Tensor)
+    if _hip.native is not None and max_suffix_len is not None and not return_lse and split_len is None \
+            and (number or max_prefix_len is not None):
+        bound = prefix_lens if max_prefix_len is None else min(max_prefix_len, prefix_lens) if number else max_prefix_len
+        o = _hip.native.shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, None if number else prefix_lens, cu_groups,
+                                      k_scale, v_scale, max(0, int(bound)), max(0, int(max_suffix_len)), bool(causal), float(scale), 0)
+        if o is not None:
+            return o
     _hip.check_shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups)
     if not q.is_cuda or _pick_backend(q) != "hip":
         return attention_paged(q, k_cache, v_cache, block_table, seqlens_k, causal=causal, scale=scale, return_lse=return_lse,
