@@ -171,7 +171,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   // tiles belong to it or to an earlier split.
   auto key0 = [&](int t) __attribute__((always_inline)) { return SHARED ? klo + t * BN : (tile0 + t) * BN; };
   auto local_tiles = [&](int n) __attribute__((always_inline)) { return SPLIT ? max(n - tile0, 0) : n; };
-  const int n_tiles = SHARED ? (khi - klo + BN - 1) / BN : local_tiles(khi > 0 ? (khi + BN - 1) / BN : 0);
+  int n_tiles = local_tiles(khi > 0 ? (khi + BN - 1) / BN : 0);
   // Tiles [0, n_fast) hold only keys that every query of the workgroup sees (SHARED: of the wave, below).
   const int wg_mask_from = !SHARED && a.causal ? min(khi, r0 + offset + 1) : khi;
   int n_fast = local_tiles(wg_mask_from > 0 ? wg_mask_from / BN : 0);
@@ -187,7 +187,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   // before the workgroup's last row, and its later tiles hold only -inf scores (P = 0), so the
   // wave skips their compute and only issues its share of the DMA (with 8 waves up to 3 tiles).
   const int wave_khi = a.causal ? min(khi, min(wr0 + 32, seq_q) - 1 + offset + 1) : khi;
-  const int wave_tiles = SHARED ? n_tiles : local_tiles(wave_khi > 0 ? (wave_khi + BN - 1) / BN : 0);
+  const int wave_tiles = local_tiles(wave_khi > 0 ? (wave_khi + BN - 1) / BN : 0);
   int qlim = qi + offset;  // last key this lane's row may see (causal)
   // SHARED: row qi's request, q-head and query, and its place in the output
   int bq = b, hrow = hq, nqi = 0, out_row = 0, row_len = 0;
@@ -258,13 +258,25 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     pslot -= first_slot;
   }
   // SHARED: the table row read above is the group's first request's, which holds the shared keys unless it is shorter (a
-  // padded batch): the entries are then loaded again from one that does.  (Both loads start together.)
+  // padded batch): the entries are then loaded again from one that does, or from the longest, whose keys are then all that
+  // any row sees.  (Both loads start together.)
   if constexpr (SHARED) {
-    const int holder = prefix_holder(a.seqlens_k, b0, b1, shared);
-    table_row = holder;
-    if (holder != b) {
+    int longest;
+    table_row = prefix_holder(a.seqlens_k, b0, b1, shared, longest);
+    khi = min(khi, longest);
+    if (khi <= klo) {  // uniform over the workgroup
+      if (row_ok) {
+        const int64_t place = (int64_t)out_row * a.shared.part_stride + sp;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) st16((float*)a.o + place * D + g * (D / 2) + 4 * i, u32x4{0, 0, 0, 0});
+        if (g == 0) st8(a.ml + place * 2, __builtin_bit_cast(u32x2, f32x2{NEG_INF, 0.f}));
+      }
+      return;
+    }
+    n_tiles = (khi - klo + BN - 1) / BN;
+    if (table_row != b) {
       const int slot_end = a.shared.by_page.of(khi - 1) + 1;
-      const int32_t* bt = a.block_table + (int64_t)holder * a.sbt;
+      const int32_t* bt = a.block_table + (int64_t)table_row * a.sbt;
 #pragma unroll
       for (int r = 0; r < PG_REGS; ++r) {
         const int sl = first_slot + 64 * r + lane;
@@ -350,9 +362,9 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   uint32_t k_put = (uint32_t)(row0 * D + (((col0 / 8) ^ Shape::swz_k(row0)) * 8)) * 2u;
   uint32_t v_put = (uint32_t)(row0 * D + (((col0 / 8) ^ VShape::swz_v(row0)) * 8)) * 2u;
   auto fetch = [&](const PageRows& src, int64_t row_bytes, bool keys, int i) __attribute__((always_inline)) {
-    // (the rows of a partition's tiles are all there, or none of them: its ends are whole 64 keys)
-    return __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(src.base, src.limit), keys ? k_at : v_at,
-                                                 i * (keys ? kperm(PR) : PR) * (int)row_bytes, 0);
+    int& at = keys ? k_at : v_at;
+    __asm__ volatile("" : "+v"(at));
+    return buffer_load16<false>(make_rsrc(src.base, src.limit), at + i * (keys ? kperm(PR) : PR) * (int)row_bytes);
   };
   // half h (8 values) of piece i to its place in a tile
   auto widen = [&](const u32x4& piece, uint16_t* dst, bool keys, int i, int h) __attribute__((always_inline)) {
@@ -777,6 +789,13 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     const int64_t rows = (int64_t)a.kv_groups * a.group * seq_q;
     const int64_t row0 = sp * rows + ((int64_t)b * a.hq + hq) * seq_q + wr0;
     const float inv = l_tot > 0.f ? (IS8 ? v_cur : 1.f) / l_tot : 0.f;
+    if constexpr (SHARED) {  // (a row without a key here: zeros, whatever V's other rows hold)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[d][r] = l_tot == 0.f ? 0.f : oacc[d][r];
+      }
+    }
     if (row_ok && g == 0) st8(a.ml + (SHARED ? (int64_t)out_row * part_stride + sp : row0 + j) * 2, __builtin_bit_cast(u32x2, f32x2{m_run, l_tot}));
     if constexpr (NW * 32 * D * 4 <= 4 * TILE * 2) {
       // through LDS, as the output below: whole rows per store instruction

@@ -120,21 +120,25 @@ __device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_eac
   return false;
 }
 
-// The request of [b0, b1) whose block-table row names the group's shared keys: the first that holds them all, or else
-// (no row sees more) the first of the longest (uniform; every lane calls it).
-__device__ __forceinline__ int prefix_holder(const int32_t* seqlens, int b0, int b1, int keys) {
+// The request of [b0, b1) whose block-table row names the group's shared keys: the first that holds them all, or else the
+// first of the longest; `longest`: how many of them it holds (uniform; every lane calls it).
+__device__ __forceinline__ int prefix_holder(const int32_t* seqlens, int b0, int b1, int keys, int& longest) {
   const int lane = (int)threadIdx.x & 63;
-  int best = b0, most = -1;
+  int best = b0;
+  longest = 0;
   for (int base = b0; base < b1; base += 64) {
-    const int n = base + lane < b1 ? min(seqlens[base + lane], keys) : -1;
+    const int n = base + lane < b1 ? min(seqlens[base + lane], keys) : 0;
     const uint64_t whole = __builtin_amdgcn_ballot_w64(n == keys);
-    if (whole != 0) return base + __builtin_ctzll(whole);
+    if (whole != 0) {
+      longest = keys;
+      return base + __builtin_ctzll(whole);
+    }
     int top = n;
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) top = max(top, __shfl_xor(top, d));
     top = __builtin_amdgcn_readfirstlane(top);
-    if (top > most) {
-      most = top;
+    if (top > longest) {
+      longest = top;
       best = base + __builtin_ctzll(__builtin_amdgcn_ballot_w64(n == top));
     }
   }

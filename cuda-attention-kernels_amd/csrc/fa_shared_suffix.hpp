@@ -315,8 +315,9 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
   for (int d = 0; d < DB; ++d) {
 #pragma unroll
     for (int rq = 0; rq < 4; ++rq) {
-      st16(op + d * 32 + 8 * rq, __builtin_bit_cast(u32x4, f32x4{oacc[d][4 * rq] * inv, oacc[d][4 * rq + 1] * inv,
-                                                                 oacc[d][4 * rq + 2] * inv, oacc[d][4 * rq + 3] * inv}));
+      // (a row without a key here: zeros, whatever V's other rows hold)
+      const f32x4 o = {oacc[d][4 * rq] * inv, oacc[d][4 * rq + 1] * inv, oacc[d][4 * rq + 2] * inv, oacc[d][4 * rq + 3] * inv};
+      st16(op + d * 32 + 8 * rq, l_tot == 0.f ? u32x4{0, 0, 0, 0} : __builtin_bit_cast(u32x4, o));
     }
   }
   if (g == 0) st8(a.ml + place * 2, __builtin_bit_cast(u32x2, f32x2{m_run, l_tot}));

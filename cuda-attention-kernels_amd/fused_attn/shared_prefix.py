@@ -33,8 +33,9 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     Group g is the requests ``cu_groups[g]`` to ``cu_groups[g + 1] - 1`` (int32 [G + 1] from 0 to B; None: one group, the
     whole batch), whose rows name the same keys in their first ``prefix_lens[g]`` positions (int32 [G], or one number for
-    every group).  A prefix may be 0, need not fill whole pages, and a request may be shorter than it (a padded batch's
-    empty ones among them).
+    every group); the pages may be the same or copies (of an FP8 page: with its scales).  A prefix may be 0, need not fill
+    whole pages, and a request may be shorter than it (a padded batch's empty ones among them).  The shared keys are read
+    through the row of a request that holds them all, and at most as far as the longest request of the group has them.
 
     ``max_prefix_len`` and ``max_suffix_len`` size the grid: the largest of prefix_lens, and of a request's keys behind
     its group's prefix.  When omitted they are read from the device, which waits for it; as numbers, they let the call be

@@ -25,8 +25,10 @@ class Case:
             0.5 * torch.randn(s[-1], device=device, generator=g))
         start = [p for p, c in zip(prefixes, groups) for _ in range(c)]
         group_of = [i for i, c in enumerate(groups) for _ in range(c)]
-        shared_pages = [min(p, max([lens[i] for i in range(b) if group_of[i] == gi], default=0)) // page
-                        for gi, p in enumerate(prefixes)]
+        # (nobody longer than the prefix: the last page that the longest request has is shared too, since an FP8 page's scales
+        # depend on all its rows, and copies with other rows behind would hold other keys)
+        most = [max([lens[i] for i in range(b) if group_of[i] == gi], default=0) for gi in range(len(groups))]
+        shared_pages = [p // page if m > p else -(-m // page) for p, m in zip(prefixes, most)]
         total = sum(shared_pages) + sum(max(0, -(-lens[i] // page) - shared_pages[group_of[i]]) for i in range(b)) + 3
         order = torch.randperm(total, generator=torch.Generator().manual_seed(seed)).tolist()
         shared = [[order.pop() for _ in range(c)] for c in shared_pages]
