@@ -139,6 +139,20 @@ __device__ __forceinline__ u32x2 fp8x4_to_e(uint32_t w) {
   return r;
 }
 
+// The same in one instruction a pair, scaled by 1.
+template <class E>
+__device__ __forceinline__ u32x2 fp8x4_widen(uint32_t w) {
+  u32x2 r;
+  if constexpr (std::is_same<E, BF16>::value) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, true));
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true));
+  }
+  return r;
+}
+
 // acc + lo + hi of a dword holding two 16-bit values, via v_dot2 with (1, 1):
 // the exact sum of the rounded values, one instruction per pair.
 template <class E>

@@ -80,8 +80,8 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   __shared__ __align__(16) uint16_t v_buf0[VTILE * ROOM];
   __shared__ __align__(16) uint16_t v_buf1[VTILE * ROOM];
   if constexpr (SHARED) {
-    const int own = (int)blockIdx.x - a.shared.prefix_wgs;
-    if (own >= 0) {  // the waves of a request's own keys
+    const int own = (int)blockIdx.x - a.shared.prefix_first;
+    if (own >= 0 && own < a.shared.suffix_wgs) {  // the waves of a request's own keys
       const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
       const int item = own * 4 + w, half = (w & 1) * 32 * D;
       if (item >= a.n_items) return;
@@ -113,7 +113,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   if constexpr (SHARED) {
     // kv-head innermost (8 of them: one to an XCD, whose L2 then holds its keys), then the row blocks, which read the
     // same keys at about the same time, then the key partitions
-    const int item = (int)blockIdx.x;
+    const int item = (int)blockIdx.x < a.shared.prefix_first ? (int)blockIdx.x : (int)blockIdx.x - a.shared.suffix_wgs;
     const int rest = a.shared.by_hkv.of(item);
     it.kvh = item - rest * a.hkv;
     part = a.shared.by_prefix_blocks.of(rest);
@@ -358,9 +358,12 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   // reload waits for the rows in flight.
   constexpr int PR = IS8 ? 1024 / D : 1;
   const int row0 = IS8 ? wave * (BN / NW) + lane * 16 / D : 0, col0 = IS8 ? lane * 16 % D : 0;
-  int k_at = (kperm(row0) & 15) * (int)krow_bytes + col0, v_at = (row0 & 15) * (int)vrow_bytes + col0;
+  // (V at D = 128: rows 0, 4, 1, 5, ... follow each other over the lanes, whose swizzles differ in their lowest bit, so that
+  // 16 lanes' writes of every second chunk of two rows meet all banks once)
+  const int vrow0 = IS8 && D == 128 ? (row0 & ~7) | ((row0 & 1) << 2) | ((row0 >> 1) & 3) : row0;
+  int k_at = (kperm(row0) & 15) * (int)krow_bytes + col0, v_at = (vrow0 & 15) * (int)vrow_bytes + col0;
   uint32_t k_put = (uint32_t)(row0 * D + (((col0 / 8) ^ Shape::swz_k(row0)) * 8)) * 2u;
-  uint32_t v_put = (uint32_t)(row0 * D + (((col0 / 8) ^ VShape::swz_v(row0)) * 8)) * 2u;
+  uint32_t v_put = (uint32_t)(vrow0 * D + (((col0 / 8) ^ VShape::swz_v(vrow0)) * 8)) * 2u;
   auto fetch = [&](const PageRows& src, int64_t row_bytes, bool keys, int i) __attribute__((always_inline)) {
     int& at = keys ? k_at : v_at;
     __asm__ volatile("" : "+v"(at));
@@ -368,7 +371,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   };
   // half h (8 values) of piece i to its place in a tile
   auto widen = [&](const u32x4& piece, uint16_t* dst, bool keys, int i, int h) __attribute__((always_inline)) {
-    const u32x2 lo = fp8x4_to_e<E>(piece[2 * h]), hi = fp8x4_to_e<E>(piece[2 * h + 1]);
+    const u32x2 lo = fp8x4_widen<E>(piece[2 * h]), hi = fp8x4_widen<E>(piece[2 * h + 1]);
     const uint32_t flip = (uint32_t)(h ^ (keys ? Shape::swz_k(i * PR) ^ Shape::swz_k(0) : VShape::swz_v(i * PR) ^ VShape::swz_v(0))) * 16u;
     uint32_t& put = keys ? k_put : v_put;
     __asm__ volatile("" : "+v"(put));

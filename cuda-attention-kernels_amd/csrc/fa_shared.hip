@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const MergeArgs a) {
 
 namespace {
 
+constexpr int kCus = 256;
 constexpr int prefix_tile_keys(int d) { return d == 256 ? 32 : 64; }
 
 template <int D, class E>
@@ -156,7 +157,7 @@ SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int pa
   // keys, 47 at 320), but no more than 576 keys each, for the last to start not to run on alone, and 320 where there are
   // many (256 requests of up to 1000 keys, 8 kv-heads, D = 64: 95 us whole, 91 at 576, 88 at 320; 32 of up to 2000: 66 at
   // 576, 72 at 320).
-  constexpr int64_t kWgs = 256, kLong = 1024, kWaves = 1024;
+  constexpr int64_t kWgs = kCus, kLong = 1024, kWaves = 1024;
   auto whole = [](int64_t keys, int64_t parts) { return ((keys + parts - 1) / parts + kPrefixUnit - 1) / kPrefixUnit * kPrefixUnit; };
   auto fits = [&](int64_t len, int64_t pages) {  // a partition spans a limited number of pages, and of FP8 scale blocks
     len = std::min(len, (pages - 2) * page_size / kPrefixUnit * kPrefixUnit);
@@ -222,7 +223,6 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   const int rows = a.group * p.seqlen_q;
   const int64_t prefix_wgs = plan.prefix_blocks * p.heads_kv * plan.prefix_parts;
   hipError_t e = hipSuccess;
-  a.shared.prefix_wgs = (int32_t)prefix_wgs;
   a.n_rowblk = (int32_t)plan.prefix_blocks;
   a.shared.suffix_blocks = (rows + 31) / 32;
   a.shared.by_page = FastDiv::by(kv.page_size);
@@ -233,7 +233,14 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   a.shared.by_prefix_blocks = FastDiv::by(a.n_rowblk);
   a.shared.by_suffix_blocks = FastDiv::by(a.shared.suffix_blocks);
   a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts * a.shared.suffix_blocks);
-  a.total = (int32_t)(a.shared.prefix_wgs + ((int64_t)a.n_items + 3) / 4);
+  // The shared keys' workgroups go first; where the requests' own keys take longer (an estimate: 0.65 us a tile and CU of the
+  // former, 4.5 TB/s for half of the longest of the latter), only one a CU, the rest behind the own keys' (256 requests of
+  // up to 1000 keys behind 4080, D = 64: 82 us, 79 so; FP8, 128 of up to 700 behind 32768: 174, 183 so).
+  const double prefix_us = 0.65 * plan.prefix_blocks * p.heads_kv * (plan.max_prefix / 64.0) / kCus;
+  const double suffix_us = (double)p.batch * p.heads_kv * plan.max_suffix * p.head_dim * (fp8 ? 1 : 2) / 4.5e6;
+  a.shared.prefix_first = (int32_t)(suffix_us > prefix_us ? std::min<int64_t>(prefix_wgs, kCus) : prefix_wgs);
+  a.shared.suffix_wgs = (int32_t)(((int64_t)a.n_items + 3) / 4);
+  a.total = (int32_t)(prefix_wgs + a.shared.suffix_wgs);
   e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) { return launch_tiles<decltype(d)::value, decltype(t)>(a, fp8, stream); });
   if (e != hipSuccess) return hip_status(e, err);
 

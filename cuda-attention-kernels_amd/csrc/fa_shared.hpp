@@ -38,7 +38,8 @@ struct SharedArgs {
   int32_t prefix_split, suffix_split;  // keys per partition
   int32_t suffix_blocks;               // blocks of 32 rows of a request
   FastDiv by_page, by_hkv, by_group, by_nq, by_batch, by_prefix_blocks, by_suffix_blocks;
-  int32_t prefix_wgs;                  // workgroups of the shared keys; the ones behind them read the requests' own
+  // the grid: prefix_first workgroups of the shared keys, suffix_wgs of the requests' own, the rest of the shared keys'
+  int32_t prefix_first, suffix_wgs;
 };
 
 struct SharedTileArgs : TileArgs {

@@ -188,7 +188,7 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
 
   const uint8_t *k8 = (const uint8_t*)kl, *v8 = (const uint8_t*)vl;
   auto wide = [&](const u32x2& raw) __attribute__((always_inline)) {
-    const u32x2 lo = fp8x4_to_e<E>(raw[0]), hi = fp8x4_to_e<E>(raw[1]);
+    const u32x2 lo = fp8x4_widen<E>(raw[0]), hi = fp8x4_widen<E>(raw[1]);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
   Rows next[UNITS];  // where the next tile's rows lie

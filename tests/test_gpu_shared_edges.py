@@ -40,6 +40,21 @@ def test_nan_and_infinity_in_keys_that_a_request_does_not_see():
     assert torch.isposinf(got[0]).all() and torch.equal(got[1:3], want[1:3])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shared", [True, False])
+def test_every_fp8_value_is_widened_exactly(dtype, shared):
+    """64 keys with the same scores and the same V row: the output is that row's value, all 254 finite codes, bit for bit
+    (sums of 64 equal numbers and the division by 64 are exact; the scale is a power of two)."""
+    codes = torch.tensor([c for c in range(256) if c & 127 != 127] + [0, 0], dtype=torch.uint8, device="cuda")
+    v = codes.expand(2, 1, 64, 256).contiguous().view(torch.float8_e4m3fn)
+    k = torch.zeros_like(v.view(torch.uint8)).view(torch.float8_e4m3fn)
+    scale = torch.full((2, 1, 1), 0.25, device="cuda")
+    table, lens = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.full((2,), 64, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 2, 1, 256, device="cuda").to(dtype)
+    o = fused_attn.attention_shared_prefix(q, k, v, table, lens, 64 if shared else 0, k_scale=scale, v_scale=scale)
+    assert torch.equal(o, (codes.view(torch.float8_e4m3fn).float() * 0.25).to(dtype).expand_as(o))
+
+
 @pytest.mark.parametrize("prefix", [0, 1, 63, 64, 65, 127])
 @pytest.mark.parametrize("fp8", [False, True])
 def test_short_prefixes(prefix, fp8):
