@@ -231,8 +231,6 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     return __builtin_amdgcn_readfirstlane(valid > 0 ? (uint32_t)(valid - 1) * (uint32_t)row_bytes + (uint32_t)(D * 2)
                                                     : 0u);
   };
-  // Tile descriptors (a tile past khi gets a zero-length one: its DMA writes zeros) and
-  // the wave's i-th 1-KiB DMA instruction of a K or V tile.
   // SHARED: the rows of a tile that a wave loads lie in one page (16 rows, or 8 of 16; page sizes are multiples of 16, and
   // kperm keeps a row among its 16).  Lane i of pg[r] holds block-table entry 64 r + i of the workgroup's keys.  The address
   // of tile t + 3's rows is formed during iteration t, a few scalar instructions a slot and without a branch: formed in one
@@ -357,12 +355,20 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   // places are formed anew from three registers each time: as registers of their own they would be spilled, and a spill's
   // reload waits for the rows in flight.
   constexpr int PR = IS8 ? 1024 / D : 1;
-  const int row0 = IS8 ? wave * (BN / NW) + lane * 16 / D : 0, col0 = IS8 ? lane * 16 % D : 0;
-  // (V at D = 128: rows 0, 4, 1, 5, ... follow each other over the lanes, whose swizzles differ in their lowest bit, so that
-  // 16 lanes' writes of every second chunk of two rows meet all banks once)
-  const int vrow0 = IS8 && D == 128 ? (row0 & ~7) | ((row0 & 1) << 2) | ((row0 >> 1) & 3) : row0;
-  int k_at = (kperm(row0) & 15) * (int)krow_bytes + col0, v_at = (vrow0 & 15) * (int)vrow_bytes + col0;
-  uint32_t k_put = (uint32_t)(row0 * D + (((col0 / 8) ^ Shape::swz_k(row0)) * 8)) * 2u;
+  int krow0 = 0, vrow0 = 0, col0 = 0;
+  if constexpr (IS8 && D == 128) {
+    // Eight lanes take half rows of two rows whose swizzles differ in their lowest bit: what they write then differs mod 8
+    // chunks (a write goes 128 bytes a cycle, and every second chunk of one row meets each bank twice; 1024 rows x 32768 keys
+    // of 8 heads: 162 us, one row after the other 163).
+    krow0 = wave * (BN / NW) + 2 * (lane >> 4) + ((lane >> 2) & 1);
+    vrow0 = wave * (BN / NW) + (lane >> 4) + 4 * ((lane >> 2) & 1);
+    col0 = ((lane & 3) + ((lane >> 1) & 4)) * 16;
+  } else if constexpr (IS8) {
+    krow0 = vrow0 = wave * (BN / NW) + lane * 16 / D;
+    col0 = lane * 16 % D;
+  }
+  int k_at = (kperm(krow0) & 15) * (int)krow_bytes + col0, v_at = (vrow0 & 15) * (int)vrow_bytes + col0;
+  uint32_t k_put = (uint32_t)(krow0 * D + (((col0 / 8) ^ Shape::swz_k(krow0)) * 8)) * 2u;
   uint32_t v_put = (uint32_t)(vrow0 * D + (((col0 / 8) ^ VShape::swz_v(vrow0)) * 8)) * 2u;
   auto fetch = [&](const PageRows& src, int64_t row_bytes, bool keys, int i) __attribute__((always_inline)) {
     int& at = keys ? k_at : v_at;
@@ -377,6 +383,8 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     __asm__ volatile("" : "+v"(put));
     st16((uint8_t*)dst + ((put ^ flip) + (uint32_t)(i * PR * D * 2)), u32x4{lo[0], lo[1], hi[0], hi[1]});
   };
+  // Tile descriptors (a tile past khi gets a zero-length one: its DMA writes zeros) and
+  // the wave's i-th 1-KiB DMA instruction of a K or V tile.
   auto k_rsrc = [&](int n0) __attribute__((always_inline)) {
     if constexpr (SHARED) {
       return ksrc;

@@ -3,7 +3,8 @@
 Same public surface as the reference package (fused_attn/__init__.py:2-23):
 the ``fused_attn::attention`` custom op, ``attention_varlen``, the unfused
 reference, split-K decode and the FP8 KV-cache path; beyond it, paged and 4-bit
-caches, and eviction by accumulated attention weight.  The ``*_triton`` names
+caches, pages allocated on the GPU, attention behind shared prefixes, and eviction by
+accumulated attention weight.  The ``*_triton`` names
 are kept as aliases of the HIP-backed functions.
 """
 from .evict import attention_scored, evict_kv

@@ -23,6 +23,9 @@ gathered keys.
 its (scale, zero) pairs, fp16 [num_pages, Hkv, page_size, 2], as ``k_scale`` / ``v_scale``; new tokens are
 written into them by ``append_kv_int4``.
 
+Block tables, slots and 16-bit page writes are made on the GPU by ``allocate_pages``, ``append_kv_paged`` and
+``release_pages`` (pages.py); sequences that share their first keys are served by ``attention_shared_prefix``.
+
 ``causal`` aligns each sequence's queries to the end of its own keys (bottom-right, as
 the dense op).  On the GPU this runs the split-K HIP kernel in its paged mode (4-bit pools: the 4-bit cache's kernel); page_size
 must be a multiple of 16 (64 for FP8 pools).  CPU tensors, or ``FUSED_ATTN_BACKEND=reference``, gather the
