@@ -39,8 +39,9 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     ``max_prefix_len`` and ``max_suffix_len`` size the grid: the largest of prefix_lens, and of a request's keys behind
     its group's prefix.  When omitted they are read from the device, which waits for it; as numbers, they let the call be
-    captured into a graph.  Longer prefixes than max_prefix_len are shared up to it; keys past max_suffix_len of their
-    own are not read.  ``split_len``: keys per partition, a multiple of 64."""
+    captured into a graph.  Longer prefixes than max_prefix_len are shared up to it, the rest of them counts as own
+    keys; keys past max_suffix_len of their own are not read.  ``split_len``: keys per partition, a multiple of 64 that spans
+    at most 128 pages (of FP8 pools: at most 4096 keys)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     number = not isinstance(prefix_lens, torch.Tensor)
     if _hip.native is not None and max_suffix_len is not None and not return_lse and split_len is None \
@@ -57,7 +58,7 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if max_prefix_len is None:
         max_prefix_len = prefix_lens if number else int(prefix_lens.max().item()) if prefix_lens.numel() else 0
     if max_suffix_len is None:
-        max_suffix_len = _longest_suffix(seqlens_k, prefix_lens, cu_groups)
+        max_suffix_len = _longest_suffix(seqlens_k, prefix_lens, cu_groups, max_prefix_len)
     if number:  # (the kernels hold every group's prefix to max_prefix_len)
         max_prefix_len, prefix_lens = min(int(max_prefix_len), int(prefix_lens)), None
     return _hip.shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups, max(0, int(max_prefix_len)),
@@ -65,14 +66,15 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                               return_lse=return_lse, k_scale=k_scale, v_scale=v_scale)
 
 
-def _longest_suffix(seqlens_k: torch.Tensor, prefix_lens, cu_groups: Optional[torch.Tensor]) -> int:
+def _longest_suffix(seqlens_k: torch.Tensor, prefix_lens, cu_groups: Optional[torch.Tensor], max_prefix_len: int) -> int:
+    """The most keys that a request has behind what its group shares (at most max_prefix_len)."""
     if seqlens_k.numel() == 0:
         return 0
     if isinstance(prefix_lens, torch.Tensor):
-        p = prefix_lens.long().clamp(min=0)
+        p = prefix_lens.long().clamp(min=0, max=max(0, int(max_prefix_len)))
         if cu_groups is not None:
             request = torch.arange(seqlens_k.numel(), device=seqlens_k.device)
             p = p[torch.searchsorted(cu_groups[1:].long().contiguous(), request, right=True).clamp(max=p.numel() - 1)]
     else:
-        p = max(0, int(prefix_lens))
+        p = max(0, min(int(prefix_lens), int(max_prefix_len)))
     return max(0, int((seqlens_k.long() - p).max().item()))

@@ -197,7 +197,8 @@ typedef struct fa_shared_prefix {
   const int32_t* cu_groups;   /* [num_groups + 1] on the device, from 0 to batch, ascending; NULL: one group, the batch */
   int32_t num_groups;
   int32_t max_prefix_len, max_suffix_len;
-  int32_t split_len; /* keys per partition, a positive multiple of 64, or 0 for the library's choice */
+  int32_t split_len; /* keys per partition, a positive multiple of 64 that spans at most 128 pages (FP8 pools: at most 4096
+                        keys), or 0 for the library's choice */
 } fa_shared_prefix;
 /* Bytes of workspace (16-byte aligned).  0 for parameters that the call would refuse, and without a batch or queries. */
 size_t fa_shared_prefix_workspace_bytes(const fa_fwd_params* p, const fa_paged_kv* kv, const fa_shared_prefix* s);

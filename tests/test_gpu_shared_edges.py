@@ -193,3 +193,13 @@ def test_pools_behind_4_gib(fp8):
     assert torch.equal(got, want)
     check_rows(got[:3], q[:3], *[x[:3] for x in small.kv], causal=True, lens=small.lens[:3])
     del big
+
+
+@pytest.mark.parametrize("number", [False, True])
+def test_a_bound_below_the_prefix_alone(number):
+    """max_prefix_len below the prefix, max_suffix_len left to be read: the rest of the prefix counts as own keys."""
+    case = Case([5], [500], [510, 600, 500, 507, 800], d=128, page=16)
+    q = case.q(8, 2)
+    kw = {"prefix_lens": 500} if number else {}
+    for bound in (0, 100, 192, 499):
+        case.check(case.call(q, causal=True, max_prefix_len=bound, **kw), q, True)

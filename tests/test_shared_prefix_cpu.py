@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import fused_attn
-from fused_attn import _hip
+from fused_attn import _hip, shared_prefix
 from shared_helpers import Case
 
 
@@ -81,3 +81,12 @@ def test_abi():
     assert status(ws=0) == _hip.FA_ERR_WORKSPACE
     assert status(ws=8) == _hip.FA_ERR_WORKSPACE
     assert status(batch=0) == _hip.FA_OK and status(seqlen_q=0) == _hip.FA_OK
+
+
+@pytest.mark.parametrize("bound,longest", [(1000, 60), (100, 60), (64, 96), (0, 160)])
+def test_own_keys_are_counted_from_the_shared_ones(bound, longest):
+    # a prefix longer than max_prefix_len is shared up to it, and the rest of it is each request's own
+    lens, cu = torch.tensor([160, 90, 0, 70], dtype=torch.int32), torch.tensor([0, 3, 4], dtype=torch.int32)
+    prefixes = torch.tensor([100, 50], dtype=torch.int32)
+    assert shared_prefix._longest_suffix(lens, prefixes, cu, bound) == longest
+    assert shared_prefix._longest_suffix(lens[:3], 100, None, bound) == longest
