@@ -1,4 +1,5 @@
 // Software-pipelined FlashAttention-2 prefill kernel for MI355X (gfx950).
+// (the kernel itself is in fa_prefill_kernel.hpp; shared prefixes use it too)
 //
 // Serves the reference's dense and varlen prefill, attn_fwd_mma_kernel
 // (csrc/flash_attn_mma.cu:63-242) and _attn_fwd_kernel
