@@ -9,8 +9,8 @@
 // The choice of kernel and partitions repeats ops._hip_kernel_for and ops.default_split_len
 // (fa_torch_route lets a test compare the two).
 //
-// fa_torch_shared_prefix, _allocate_pages, _release_pages and _append_kv_paged do the same for Python functions that are no
-// ops: they take the tensors as Python objects, and return None for what the Python code is to handle.
+// fa_torch_functions gives functions that do the same for attention_shared_prefix, allocate_pages, release_pages and
+// append_kv_paged, which are no ops: they take Python objects, and return None for what the Python code is to handle.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -444,6 +444,82 @@ PyObject* tuple_of(const std::vector<at::Tensor>& out) {
   return t;
 }
 
+// Numbers among the arguments: anything else, or past the range, ends the call (as above: None).
+struct NoNumber : std::exception {};
+int64_t whole(PyObject* o) {
+  const long long x = PyLong_AsLongLong(o);
+  if (x == -1 && PyErr_Occurred() != nullptr) throw NoNumber();
+  return x;
+}
+int32_t whole32(PyObject* o) {
+  const int64_t x = whole(o);
+  if (x < INT32_MIN || x > INT32_MAX) throw NoNumber();
+  return (int32_t)x;
+}
+double real(PyObject* o) {
+  const double x = PyFloat_AsDouble(o);
+  if (x == -1.0 && PyErr_Occurred() != nullptr) throw NoNumber();
+  return x;
+}
+
+bool takes(Py_ssize_t given, Py_ssize_t wanted) {
+  if (given != wanted) PyErr_Format(PyExc_TypeError, "%zd arguments in place of %zd", given, wanted);
+  return given == wanted;
+}
+
+// attention_shared_prefix of (q, k, v, block_table, seqlens_k, prefix_lens or None, cu_groups or None, k_scale or None, v_scale
+// or None, max_prefix, max_suffix, causal, scale, split_len or 0): its output.
+PyObject* py_shared_prefix(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (!takes(n, 14)) return nullptr;
+  return with_tensors({x[0], x[1], x[2], x[3], x[4]}, {x[5], x[6], x[7], x[8]}, [&]() -> PyObject* {
+    const at::Tensor out = shared_prefix({THPVariable_Unpack(x[0]), THPVariable_Unpack(x[1]), THPVariable_Unpack(x[2]),
+                                          THPVariable_Unpack(x[3]), THPVariable_Unpack(x[4]), tensor_or_none(x[5]),
+                                          tensor_or_none(x[6]), tensor_or_none(x[7]), tensor_or_none(x[8]), whole(x[9]), whole(x[10]),
+                                          whole(x[11]) != 0, real(x[12]), whole32(x[13])});
+    return out.defined() ? THPVariable_Wrap(out) : nullptr;
+  });
+}
+
+// allocate_pages of (block_table, seqlens_k, new_lens, free_pages, num_free, page_size, num_tokens): a tuple.
+PyObject* py_allocate_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (!takes(n, 7)) return nullptr;
+  return with_tensors({x[0], x[1], x[2], x[3], x[4]}, {}, [&] {
+    return tuple_of(allocate_pages(THPVariable_Unpack(x[0]), THPVariable_Unpack(x[1]), THPVariable_Unpack(x[2]),
+                                   THPVariable_Unpack(x[3]), THPVariable_Unpack(x[4]), whole(x[5]), whole(x[6])));
+  });
+}
+
+// release_pages of (block_table, seqlens_k, done, free_pages, num_free, keep_lens or None, page_size): a tuple.
+PyObject* py_release_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (!takes(n, 7)) return nullptr;
+  return with_tensors({x[0], x[1], x[2], x[3], x[4]}, {x[5]}, [&] {
+    return tuple_of(release_pages(THPVariable_Unpack(x[0]), THPVariable_Unpack(x[1]), THPVariable_Unpack(x[2]),
+                                  THPVariable_Unpack(x[3]), THPVariable_Unpack(x[4]), tensor_or_none(x[5]), whole(x[6])));
+  });
+}
+
+// append_kv_paged of (k, v, k_cache, v_cache, slots): True.
+PyObject* py_append_kv_paged(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (!takes(n, 5)) return nullptr;
+  return with_tensors({x[0], x[1], x[2], x[3], x[4]}, {}, [&]() -> PyObject* {
+    if (!append_kv_paged(THPVariable_Unpack(x[0]), THPVariable_Unpack(x[1]), THPVariable_Unpack(x[2]), THPVariable_Unpack(x[3]),
+                         THPVariable_Unpack(x[4])))
+      return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// (functions of Python's own calling convention: through ctypes a call took 0.2 to 0.6 us more)
+template <class F>
+PyCFunction function(F* f) {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
+}
+PyMethodDef kFunctions[] = {{"shared_prefix", function(py_shared_prefix), METH_FASTCALL, nullptr},
+                            {"allocate_pages", function(py_allocate_pages), METH_FASTCALL, nullptr},
+                            {"release_pages", function(py_release_pages), METH_FASTCALL, nullptr},
+                            {"append_kv_paged", function(py_append_kv_paged), METH_FASTCALL, nullptr},
+                            {nullptr, nullptr, 0, nullptr}};
+
 // Autograd: the op has no formula of its own, so a call that would record one goes to the Python kernel, which
 // records the node that the op's users registered, or one that raises.
 at::Tensor attention_autograd(c10::DispatchKeySet ks, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool causal,
@@ -491,50 +567,22 @@ void fa_torch_bind_shared(void* workspace_bytes, void* call) {
   g_shared.call = (decltype(g_shared.call))call;
 }
 
-// attention_shared_prefix of tensors (the last four may be None) that need no preparation: its output, or None.  Called
-// with the GIL held; nothing is thrown and no Python error is set.
-PyObject* fa_torch_shared_prefix(PyObject* q, PyObject* k, PyObject* v, PyObject* table, PyObject* seqlens, PyObject* prefix_lens,
-                                 PyObject* cu_groups, PyObject* k_scale, PyObject* v_scale, int64_t max_prefix,
-                                 int64_t max_suffix, int32_t causal, double scale, int32_t split_len) {
-  return with_tensors({q, k, v, table, seqlens}, {prefix_lens, cu_groups, k_scale, v_scale}, [&]() -> PyObject* {
-    const at::Tensor out = shared_prefix({THPVariable_Unpack(q), THPVariable_Unpack(k), THPVariable_Unpack(v), THPVariable_Unpack(table),
-                                          THPVariable_Unpack(seqlens), tensor_or_none(prefix_lens), tensor_or_none(cu_groups),
-                                          tensor_or_none(k_scale), tensor_or_none(v_scale), max_prefix, max_suffix, causal != 0, scale,
-                                          split_len});
-    return out.defined() ? THPVariable_Wrap(out) : nullptr;
-  });
-}
-
 void fa_torch_bind_pages(void* allocate, void* release, void* append) {
   g_pages.allocate = (decltype(g_pages.allocate))allocate;
   g_pages.release = (decltype(g_pages.release))release;
   g_pages.append = (decltype(g_pages.append))append;
 }
 
-// The same for allocate_pages (a tuple), release_pages (keep_lens may be None; a tuple) and append_kv_paged (True).
-PyObject* fa_torch_allocate_pages(PyObject* table, PyObject* seqlens, PyObject* new_lens, PyObject* free_pages, PyObject* num_free,
-                                  int64_t page_size, int64_t num_tokens) {
-  return with_tensors({table, seqlens, new_lens, free_pages, num_free}, {}, [&] {
-    return tuple_of(allocate_pages(THPVariable_Unpack(table), THPVariable_Unpack(seqlens), THPVariable_Unpack(new_lens),
-                                   THPVariable_Unpack(free_pages), THPVariable_Unpack(num_free), page_size, num_tokens));
-  });
-}
-
-PyObject* fa_torch_release_pages(PyObject* table, PyObject* seqlens, PyObject* done, PyObject* free_pages, PyObject* num_free,
-                                 PyObject* keep_lens, int64_t page_size) {
-  return with_tensors({table, seqlens, done, free_pages, num_free}, {keep_lens}, [&] {
-    return tuple_of(release_pages(THPVariable_Unpack(table), THPVariable_Unpack(seqlens), THPVariable_Unpack(done),
-                                  THPVariable_Unpack(free_pages), THPVariable_Unpack(num_free), tensor_or_none(keep_lens), page_size));
-  });
-}
-
-PyObject* fa_torch_append_kv_paged(PyObject* k, PyObject* v, PyObject* k_cache, PyObject* v_cache, PyObject* slots) {
-  return with_tensors({k, v, k_cache, v_cache, slots}, {}, [&]() -> PyObject* {
-    if (!append_kv_paged(THPVariable_Unpack(k), THPVariable_Unpack(v), THPVariable_Unpack(k_cache), THPVariable_Unpack(v_cache),
-                         THPVariable_Unpack(slots)))
-      return nullptr;
-    Py_RETURN_TRUE;
-  });
+// {name: function} of the Python functions above, called with the GIL held.
+PyObject* fa_torch_functions(void) {
+  PyObject* all = PyDict_New();
+  for (PyMethodDef* m = kFunctions; all != nullptr && m->ml_name != nullptr; ++m) {
+    PyObject* f = PyCFunction_New(m, nullptr);
+    const bool kept = f != nullptr && PyDict_SetItemString(all, m->ml_name, f) == 0;
+    Py_XDECREF(f);
+    if (!kept) Py_CLEAR(all);
+  }
+  return all;
 }
 
 // Device `index` runs the library bound above (which happens before).

@@ -465,20 +465,16 @@ def load_native() -> None:
 
 
 def _has_native_functions(lib: ctypes.CDLL) -> bool:
-    return isinstance(getattr(lib, "fa_torch_allocate_pages", None), lib._FuncPtr)
+    return isinstance(getattr(lib, "fa_torch_functions", None), lib._FuncPtr)
 
 
 class NativeFunctions:
-    """fa_torch_*: each returns None for a call that Python has to prepare or refuse."""
+    """shared_prefix, allocate_pages, release_pages and append_kv_paged of positional arguments: each returns None for a
+    call that Python has to prepare or refuse."""
 
-    def __init__(self, lib):
-        obj, i64 = ctypes.py_object, ctypes.c_int64
-        for name, args in (("shared_prefix", [obj] * 9 + [i64] * 2 + [ctypes.c_int32, ctypes.c_double, ctypes.c_int32]),
-                           ("allocate_pages", [obj] * 5 + [i64] * 2), ("release_pages", [obj] * 6 + [i64]),
-                           ("append_kv_paged", [obj] * 5)):
-            f = getattr(lib, "fa_torch_" + name)
-            f.argtypes, f.restype = args, obj
-            setattr(self, name, f)
+    def __init__(self, lib: ctypes.PyDLL):
+        lib.fa_torch_functions.argtypes, lib.fa_torch_functions.restype = [], ctypes.py_object
+        self.__dict__.update(lib.fa_torch_functions())
 
 
 def _bind_native_functions(hip: ctypes.CDLL) -> NativeFunctions:
@@ -487,7 +483,7 @@ def _bind_native_functions(hip: ctypes.CDLL) -> NativeFunctions:
 
     _native.fa_torch_bind_shared(*pointers(hip.fa_shared_prefix_workspace_bytes, hip.fa_attention_shared_prefix))
     _native.fa_torch_bind_pages(*pointers(hip.fa_allocate_pages, hip.fa_release_pages, hip.fa_append_kv_paged))
-    return NativeFunctions(ctypes.PyDLL(_native._name))  # (PyDLL keeps the GIL: they take Python objects)
+    return NativeFunctions(ctypes.PyDLL(_native._name))  # (PyDLL keeps the GIL)
 
 
 def _enable_native(index: int) -> None:

@@ -135,3 +135,24 @@ def test_abi():
         for name, value in kw.items():
             setattr(q, name, value)
         assert lib.fa_append_kv_paged(q, x) == _hip.FA_OK
+
+
+def test_native_functions_hand_on_what_they_do_not_serve():
+    import ctypes
+
+    from fused_attn import _hip
+
+    assert _hip._native is not None, "libfused_attn_torch.so is not built"
+    n = _hip.NativeFunctions(ctypes.PyDLL(_hip._native._name))
+    t = torch.zeros(2, 2, dtype=torch.int32)
+    for other in (t, 1, None, "x"):  # tensors of the CPU, and what is no tensor
+        assert n.append_kv_paged(other, t, t, t, t) is None
+        assert n.allocate_pages(t, other, t, t, t, 16, 1) is None
+        assert n.release_pages(t, t, t, t, other, None, 16) is None
+        assert n.shared_prefix(t, t, t, t, other, None, None, None, None, 64, 64, False, 0.1, 0) is None
+    for number in (1.5, 1 << 70, "x", None):  # no whole numbers, and one past 64 bits
+        assert n.allocate_pages(t, t, t, t, t, number, 1) is None
+        assert n.shared_prefix(t, t, t, t, t, None, None, None, None, 64, number, False, 0.1, 0) is None
+    for f in vars(n).values():
+        with pytest.raises(TypeError, match="arguments"):
+            f(t)
