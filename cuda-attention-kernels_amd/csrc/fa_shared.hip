@@ -8,7 +8,7 @@
 //
 // What bounds it: the shared keys' products (matrix cores and, with as many vector cycles, the exponentials) beside the
 // stream of the own keys, and about 8 us of start and end.  64 requests of 4 rows a kv-head (8 of them, D = 128) behind
-// 8192 keys, up to 512 of their own: 27 us and the merge's 4.4; 32 of 16 rows behind 16384, up to 2000: 56 and 6.6.  Whole
+// 8192 keys, up to 512 of their own: 27 us and the merge's 4.4; 32 of 16 rows behind 16384, up to 2000: 56 and 5.8.  Whole
 // calls 31 and 63 us; with the split-K kernels over both parts, one after the other, 70 and 114.
 #include <hip/hip_runtime.h>
 
@@ -27,28 +27,30 @@ struct MergeArgs {
   int64_t sob, soh, son, slb, slh;
   const int32_t* seqlens;
   int32_t hq, nq, chunks;  // chunks: workgroups a request
+  FastDiv by_chunks, by_prefix_split, by_suffix_split;
   SharedArgs shared;
 };
 
-// Bound by its launch, and by the partials' bytes where they are many (2048 rows x 10 partials of D = 128: 4.4 us; a
-// workgroup for every row, the partials dealt to its threads, took 8.4).
+// Bound by its launch, and by the partials' bytes where they are many (2048 rows x 10 partials of D = 128: 4.6 us; a
+// workgroup for every row, the partials dealt to its threads, took 8.4; 8192 rows 8.7).  Few instructions a row: with 8
+// partials a thread in place of 4, most of them none, and divisions by numbers that the host knows, the latter took 11.
 //
 // A thread merges 4 values of a row over every WAYS-th of its partials, CH of them in flight together; WAYS threads meet
 // in LDS.  A workgroup's rows are one request's, so that its group and its partitions are found once, uniformly.
 template <int D, class E, int WAYS>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const MergeArgs a) {
-  constexpr int TPR = D / 4, ROWS = 256 / (TPR * WAYS), CH = 8;
+  constexpr int TPR = D / 4, ROWS = 256 / (TPR * WAYS), CH = WAYS > 1 ? 4 : 8;
   static_assert(ROWS >= 1, "a row per workgroup at least");
   constexpr float NEG_INF = -__builtin_inff();
   __shared__ f32x4 s_acc[WAYS > 1 ? 256 : 1];
   __shared__ f32x2 s_ml[WAYS > 1 ? ROWS * WAYS : 1];
-  const int b = (int)(blockIdx.x / (uint32_t)a.chunks), chunk = (int)(blockIdx.x - (uint32_t)b * (uint32_t)a.chunks);
+  const int b = a.by_chunks.of((int)blockIdx.x), chunk = (int)blockIdx.x - b * a.chunks;
   const int tid = (int)threadIdx.x, dq = tid % TPR, way = tid / TPR % WAYS, sub = tid / (TPR * WAYS);
   const int rows = a.hq * a.nq, r = chunk * ROWS + sub;  // (q-head, query) of the request
   const int shared = shared_keys_of(a.shared, b);
   const int keys = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens[b]), shared);
-  const int first = (shared + a.shared.prefix_split - 1) / a.shared.prefix_split;
-  const int count = r < rows ? first + (keys > shared ? (keys - shared + a.shared.suffix_split - 1) / a.shared.suffix_split : 0) : 0;
+  const int first = a.by_prefix_split.of(shared + a.shared.prefix_split - 1);
+  const int count = r < rows ? first + (keys > shared ? a.by_suffix_split.of(keys - shared + a.shared.suffix_split - 1) : 0) : 0;
   const int skip = a.shared.part_base - first;  // places between the two runs of a row's partials
   const int64_t base = ((int64_t)b * rows + min(r, rows - 1)) * a.shared.part_stride;
   const float* ml = a.ml + base * 2;
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const MergeArgs a) {
   }
   if (r >= rows) return;
   const float l_safe = (l == 0.f) ? 1.f : l, inv = 1.f / l_safe;
-  const int h = r / a.nq, n = r - h * a.nq;
+  const int h = a.shared.by_nq.of(r), n = r - h * a.nq;
   if (a.lse != nullptr && dq == 0) a.lse[b * a.slb + (int64_t)h * a.slh + n] = (m + __log2f(l_safe)) * kLn2;
   uint16_t* o = (uint16_t*)a.o + b * a.sob + (int64_t)h * a.soh + (int64_t)n * a.son + 4 * dq;
   st8(o, u32x2{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv)});
@@ -132,13 +134,14 @@ template <int D, class E, int WAYS>
 hipError_t launch_merge_ways(MergeArgs a, int batch, hipStream_t stream) {
   constexpr int ROWS = 256 / (D / 4 * WAYS);
   a.chunks = (a.hq * a.nq + ROWS - 1) / ROWS;
+  a.by_chunks = FastDiv::by(a.chunks);
   hipLaunchKernelGGL((shared_merge_kernel<D, E, WAYS>), dim3((unsigned)a.chunks * (unsigned)batch), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
 template <int D, class E>
 hipError_t launch_merge(const MergeArgs& a, int batch, int parts, hipStream_t stream) {
-  // more than one round of CH partials a thread: four threads share them
+  // more than one round of CH partials: four threads share them, 4 each
   if (parts <= 8) return launch_merge_ways<D, E, 1>(a, batch, stream);
   return launch_merge_ways<D, E, 4>(a, batch, stream);
 }
@@ -266,6 +269,8 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   m.seqlens = kv.seqlens_k;
   m.hq = p.heads_q;
   m.nq = p.seqlen_q;
+  m.by_prefix_split = FastDiv::by(plan.prefix_split);
+  m.by_suffix_split = FastDiv::by(plan.suffix_split);
   m.shared = a.shared;
   e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) {
     return launch_merge<decltype(d)::value, decltype(t)>(m, p.batch, stride, stream);
