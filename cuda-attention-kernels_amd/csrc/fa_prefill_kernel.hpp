@@ -348,6 +348,11 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   auto scale_of = [&](float scales, int t) __attribute__((always_inline)) {
     return lane_value(scales, t * BN / 64);
   };
+  // V's rows of tile t, which read as zeros where its scale is no unit of O
+  auto valued_rows = [&](PageRows src, int t) __attribute__((always_inline)) {
+    src.limit = is_unit(scale_of(v_scales, t)) ? src.limit : 0u;
+    return src;
+  };
   // what tile t's products are multiplied with to be scores in log2 units
   auto score_scale = [&](int t) __attribute__((always_inline)) { return IS8 ? fmaxf(c * scale_of(k_scales, t), kMinScale) : c; };
   // Lane's row of piece 0, and where piece i lies from there: a uniform distance in memory (the pieces' rows are PR apart,
@@ -453,6 +458,9 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
       source(2);
 #pragma unroll
       for (int i = 0; i < NP; ++i) kreg[i] = fetch(ksrc, krow_bytes, true, i);
+      v_scales = v_units(v_scales);  // (behind the loads above)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) vreg[i] = is_unit(scale_of(v_scales, 0)) ? vreg[i] : u32x4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < 2 * NP; ++i) {
         widen(first[i / 2], k_buf0, true, i / 2, i % 2);
@@ -460,7 +468,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
         widen(second[i / 2], k_buf1, true, i / 2, i % 2);
       }
 #pragma unroll
-      for (int i = 0; i < NP; ++i) vreg[i] = fetch(vsrc[0], vrow_bytes, false, i);
+      for (int i = 0; i < NP; ++i) vreg[i] = fetch(valued_rows(vsrc[0], 1), vrow_bytes, false, i);
       source(3);  // (in iteration 0, K of tile 2 and V of tile 1 go to LDS, and K of tile 3 and V of tile 2 are fetched)
     } else {
       load_k(key0(0), k_buf0);
@@ -610,17 +618,19 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     float m_safe = (m_run == NEG_INF) ? 0.f : m_run;
     // FP8: O is held in units of v_cur, the V block scale of a recent tile.  A tile whose scale vb is within a factor 2 of
     // it takes vb / v_cur into its exponents, and out of its row sum again; any other first brings O to its own scale.
+    // (v_scales hold units, v_units above.)
     const float c_this = score_scale(t), c_next = score_scale(t + 1);
     float unfold = 1.f;
     if constexpr (IS8) {
       const float vb = scale_of(v_scales, t);
-      if (vb > 0.f && !(vb <= 2.f * v_cur && v_cur <= 2.f * vb)) {
+      const bool valued = is_unit(vb);  // (else V's rows are zeros)
+      if (valued && !(vb <= 2.f * v_cur && v_cur <= 2.f * vb)) {
         const float ratio = v_cur / vb;
 #pragma unroll
         for (int d = 0; d < DB; ++d) oacc[d] *= ratio;
         v_cur = vb;
       }
-      if (vb > 0.f) {
+      if (valued) {
         unfold = v_cur / vb;
         m_safe += __log2f(unfold);
       }
@@ -674,7 +684,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
             if constexpr (u % 2 == 1) kreg[i] = fetch(ksrc, krow_bytes, true, i);
           } else {
             widen(vreg[i], vd, false, i, u % 2);
-            if constexpr (u % 2 == 1) vreg[i] = fetch(vsrc[0], vrow_bytes, false, i);
+            if constexpr (u % 2 == 1) vreg[i] = fetch(valued_rows(vsrc[0], t + 2), vrow_bytes, false, i);
           }
         }
       } else if constexpr (m < NDMA) {
@@ -799,12 +809,16 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     // here) and (m, l), [S][B, Hq, Nq][D]
     const int64_t rows = (int64_t)a.kv_groups * a.group * seq_q;
     const int64_t row0 = sp * rows + ((int64_t)b * a.hq + hq) * seq_q + wr0;
-    const float inv = l_tot > 0.f ? (IS8 ? v_cur : 1.f) / l_tot : 0.f;
+    float inv = l_tot > 0.f ? (IS8 ? v_cur : 1.f) / l_tot : 0.f;
     if constexpr (SHARED) {  // (a row without a key here: zeros, whatever V's other rows hold)
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) oacc[d][r] = l_tot == 0.f ? 0.f : oacc[d][r];
+      }
+      if constexpr (IS8) {
+        const int none = first_without_value(v_scales);
+        if (none < 64 && klo + 64 * none <= qlim) inv = __builtin_nanf("");
       }
     }
     if (row_ok && g == 0) st8(a.ml + (SHARED ? (int64_t)out_row * part_stride + sp : row0 + j) * 2, __builtin_bit_cast(u32x2, f32x2{m_run, l_tot}));

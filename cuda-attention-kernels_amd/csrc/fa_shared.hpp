@@ -16,6 +16,27 @@ constexpr int kPrefixPages = 128;  // pages that a partition of the shared keys 
 constexpr int kSuffixPages = 256;  // and one of a request's own
 constexpr int kFp8Keys = 64 * 64;  // keys of an FP8 partition: a lane holds a 64-key block's scales
 
+// The V scales of an FP8 partition (lane i: block i) as units in which O can be held: 0 for a block whose values count as 0
+// (a scale of 0, or below 2^-90 of the partition's largest, in which O would overflow: O is at most 448 codes x 2^8 (P) x
+// 2^12 keys, 2^29), NaN for an infinite one or NaN, whose block makes NaN of every row that sees it.  Every lane calls it.
+__device__ __forceinline__ float v_units(float scale) {
+  const float size = fabsf(scale);
+  const bool finite = size < __builtin_inff();
+  float top = finite ? size : 0.f;
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  return !finite ? __builtin_nanf("") : size > top * 0x1p-90f ? scale : 0.f;
+}
+// Neither 0 nor NaN, of a uniform value.
+__device__ __forceinline__ bool is_unit(float unit) {
+  return (__builtin_bit_cast(uint32_t, unit) & 0x7fffffffu) - 1u < 0x7f7fffffu;
+}
+// The first block without a value among the units of a partition, at most 64 (uniform).
+__device__ __forceinline__ int first_without_value(float units) {
+  const uint64_t none = __builtin_amdgcn_ballot_w64(units != units);
+  return none != 0 ? __builtin_ctzll(none) : 64;
+}
+
 // Division of 0 <= n < 2^31 by a number that the host knows: (n * mul) >> shift.
 struct FastDiv {
   uint32_t mul;

@@ -200,6 +200,7 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
     load(next, vbase, a.spv, vrow, vl, false);
     find(klo + BN, next);
   }
+  if constexpr (IS8) v_scales = v_units(v_scales);
   for (int t = 0; t < n_tiles; ++t) {
     const int n0 = klo + t * BN;
     wait_loads<BLOCKS>();  // K_t landed; V_t may be in flight
@@ -248,15 +249,17 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
       m_run = m_new;
     }
     float m_safe = (m_run == NEG_INF) ? 0.f : m_run, unfold = 1.f;
+    bool valued = true;
     if constexpr (IS8) {  // V's scale: into the exponents, out of the row sum; far from O's unit, O takes it first
       const float vb = lane_value(v_scales, t);
-      if (vb > 0.f && !(vb <= 2.f * v_cur && v_cur <= 2.f * vb)) {
+      valued = is_unit(vb);
+      if (valued && !(vb <= 2.f * v_cur && v_cur <= 2.f * vb)) {
         const float ratio = v_cur / vb;
 #pragma unroll
         for (int d = 0; d < DB; ++d) oacc[d] *= ratio;
         v_cur = vb;
       }
-      if (vb > 0.f) {
+      if (valued) {
         unfold = v_cur / vb;
         m_safe += __log2f(unfold);
       }
@@ -277,6 +280,12 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
       }
     }
     l_run += IS8 ? rs * unfold : rs;
+    if constexpr (IS8) {
+      if (!valued) {  // the tile has weights, but its values are 0
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) pf[kb][0] = pf[kb][1] = u32x4{0, 0, 0, 0};
+      }
+    }
     if (more) {
       wait_loads<BLOCKS>();  // V_t landed; K_{t+1} stays in flight
     } else {
@@ -309,7 +318,11 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
 
   // the partial: O normalised by its own row sum (zeros without a key), and (m, l)
   const float l_tot = sum_xor32(l_run);
-  const float inv = l_tot > 0.f ? v_cur / l_tot : 0.f;
+  float inv = l_tot > 0.f ? v_cur / l_tot : 0.f;
+  if constexpr (IS8) {
+    const int none = first_without_value(v_scales);
+    if (none < 64 && klo + 64 * none <= qlim) inv = __builtin_nanf("");
+  }
   if (!row_ok) return;
   const int64_t place = ((int64_t)(b * a.hq + hq) * a.nq + qi) * a.shared.part_stride + a.shared.part_base + part;
   float* op = (float*)a.o + place * D + 4 * g;

@@ -36,6 +36,8 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     every group); the pages may be the same or copies (of an FP8 page: with its scales).  A prefix may be 0, need not fill
     whole pages, and a request may be shorter than it (a padded batch's empty ones among them).  The shared keys are read
     through the row of a request that holds them all, and at most as far as the longest request of the group has them.
+    (On the GPU a shared 64-key block of FP8 V whose scale is 0, or below 2^-90 of another's in its partition, counts as
+    zeros, and an infinite or NaN scale makes NaN of the rows that see the block.)
 
     ``max_prefix_len`` and ``max_suffix_len`` size the grid: the largest of prefix_lens, and of a request's keys behind
     its group's prefix.  When omitted they are read from the device, which waits for it; as numbers, they let the call be
