@@ -27,9 +27,111 @@ struct MergeArgs {
   int64_t sob, soh, son, slb, slh;
   const int32_t* seqlens;
   int32_t hq, nq, chunks;  // chunks: workgroups a request
+  int32_t causal;
   FastDiv by_chunks, by_prefix_split, by_suffix_split;
   SharedArgs shared;
+  TileArgs tile;  // for partials that are formed anew
+  int32_t fp8;
 };
+
+// One value of a row: 16-bit E, or an FP8 code.
+template <class E>
+__device__ __forceinline__ float value_at(const void* p, int64_t at, bool fp8) {
+  if (fp8) return __builtin_amdgcn_cvt_pk_f32_fp8((int)((const uint8_t*)p)[at], false)[0];
+  return lo_f32<E>(((const uint16_t*)p)[at]);
+}
+
+// A row that sees the first keys of a partition only (its request ends there, or its causal end lies there) shared the
+// partition's products with rows that see all of it.  Its weight of a key that it does not see is 0, and 0 times an infinity or
+// NaN in that key's V is NaN.  So a partial of such a row that is not finite is formed anew, over the keys that it sees: a dot
+// product a thread for 256 keys at a time, then a column of V a thread.  Slow, and only ever done where V holds such values;
+// other calls pay a comparison a request, and one load and barrier where a request ends among the shared keys.
+//
+// The workgroup's rows are r0 to r0 + ROWS - 1 of request b, which has `keys` keys; all threads call it.
+template <int D, class E, int ROWS>
+__device__ __forceinline__ void renew_partials(int b, int r0, int shared, int keys) {
+  // (the arguments through a pointer that the compiler does not know: it would load what is used here at the kernel's
+  // entry, and spill: 0.5 to 2 us a call)
+  uint64_t address = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+#if defined(__HIP_DEVICE_COMPILE__)
+  __asm__ volatile("" : "+s"(address));
+  const auto& a = *reinterpret_cast<const MergeArgs __attribute__((address_space(4)))*>(address);
+#else
+  const MergeArgs& a = *reinterpret_cast<const MergeArgs*>(address);
+#endif
+  __shared__ float s_p[256];
+  __shared__ int64_t s_at[256];  // V's row of a key, in elements; -1: no value
+  __shared__ float s_scale[256];
+  const auto& t = a.tile;
+  const int tid = (int)threadIdx.x, rows = min(ROWS, a.hq * a.nq - r0);
+  // the row's keys, and the partition that they end in, if that has more
+  auto ends_in = [&](int r, int& limit) {
+    limit = t.causal ? keys - a.nq + (r - a.shared.by_nq.of(r) * a.nq) + 1 : keys;
+    if (limit <= 0 || limit >= shared) return -1;
+    const int s = a.by_prefix_split.of(limit - 1);
+    return limit < min((s + 1) * a.shared.prefix_split, shared) ? s : -1;
+  };
+  auto part_of = [&](int r, int s) { return (float*)a.part + (((int64_t)b * a.hq * a.nq + r) * a.shared.part_stride + s) * D; };
+  bool spoiled = false;
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    int limit;
+    const int r = r0 + i / (D / 4), s = ends_in(r, limit);
+    if (s < 0) continue;
+    const f32x4 v = __builtin_bit_cast(f32x4, ld16(part_of(r, s) + i % (D / 4) * 4));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) spoiled |= !(fabsf(v[e]) < __builtin_inff());
+  }
+  if (!__syncthreads_or(spoiled)) return;
+
+  const int32_t* bt = t.block_table + (int64_t)b * t.sbt;
+  for (int r = r0; r < r0 + rows; ++r) {
+    int limit;
+    const int s = ends_in(r, limit);
+    if (s < 0) continue;
+    float* out = part_of(r, s);
+    if (!__syncthreads_or(tid < D && !(fabsf(out[tid % D]) < __builtin_inff()))) continue;
+    const int h = a.shared.by_nq.of(r), kvh = a.shared.by_group.of(h);
+    const uint16_t* q = (const uint16_t*)t.q + (int64_t)b * t.sqb + (int64_t)h * t.sqh + (int64_t)(r - h * a.nq) * t.sqn;
+    const float m = a.ml[(((int64_t)b * a.hq * a.nq + r) * a.shared.part_stride + s) * 2], m_safe = m == -__builtin_inff() ? 0.f : m;
+    float acc = 0.f, sum = 0.f;
+    for (int n0 = s * a.shared.prefix_split; n0 < limit; n0 += 256) {
+      const int n = n0 + tid;
+      float p = 0.f;
+      s_at[tid] = -1;
+      if (n < limit) {
+        const int slot = a.shared.by_page.of(n), page = bt[slot], off = n - slot * t.page_size;
+        float score = 0.f, c = fabsf(t.qk_scale);
+        if ((uint32_t)page < (uint32_t)t.num_pages) {  // (keys outside the pool are zeros)
+          const int64_t at = (int64_t)page * t.spk + (int64_t)kvh * t.skh + (int64_t)off * t.skn;
+#pragma unroll 4
+          for (int d = 0; d < D; ++d) score += lo_f32<E>(q[d]) * value_at<E>(t.k, at + d, a.fp8);
+          s_at[tid] = (int64_t)page * t.spv + (int64_t)kvh * t.svh + (int64_t)off * t.svn;
+          if (a.fp8) {
+            const int64_t block = (int64_t)page * t.ssb + (int64_t)kvh * t.ssh + off / 64;
+            const float vs = t.v_scale[block];
+            c *= t.k_scale[block];
+            s_scale[tid] = fabsf(vs) < __builtin_inff() ? vs : __builtin_nanf("");
+            if (vs == 0.f) s_at[tid] = -1;
+          }
+        } else {
+          c = 0.f;
+        }
+        p = fast_exp2((t.qk_scale < 0.f ? -score : score) * fmaxf(c, kMinScale) - m_safe);
+      }
+      s_p[tid] = p;
+      __syncthreads();
+      const int count = min(limit - n0, 256);
+      for (int i = 0; i < count; ++i) {
+        const float w = s_p[i];
+        sum += w;
+        if (tid < D && s_at[i] >= 0) acc += w * (value_at<E>(t.v, s_at[i] + tid, a.fp8) * (a.fp8 ? s_scale[i] : 1.f));
+      }
+      __syncthreads();
+    }
+    if (tid < D) out[tid] = sum == 0.f ? 0.f : acc / sum;
+  }
+  __syncthreads();
+}
 
 // Bound by its launch, and by the partials' bytes where they are many (2048 rows x 10 partials of D = 128: 4.6 us; a
 // workgroup for every row, the partials dealt to its threads, took 8.4; 8192 rows 8.7).  Few instructions a row: with 8
@@ -52,6 +154,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const MergeArgs a) {
   const int first = a.by_prefix_split.of(shared + a.shared.prefix_split - 1);
   const int count = r < rows ? first + (keys > shared ? a.by_suffix_split.of(keys - shared + a.shared.suffix_split - 1) : 0) : 0;
   const int skip = a.shared.part_base - first;  // places between the two runs of a row's partials
+  if ((a.causal ? keys - a.nq + 1 : keys) < shared) renew_partials<D, E, ROWS>(b, chunk * ROWS, shared, keys);  // uniform
   const int64_t base = ((int64_t)b * rows + min(r, rows - 1)) * a.shared.part_stride;
   const float* ml = a.ml + base * 2;
   const float* op = a.part + base * D + 4 * dq;
@@ -271,7 +374,10 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   m.nq = p.seqlen_q;
   m.by_prefix_split = FastDiv::by(plan.prefix_split);
   m.by_suffix_split = FastDiv::by(plan.suffix_split);
+  m.causal = p.causal;
   m.shared = a.shared;
+  m.tile = a;
+  m.fp8 = fp8;
   e = by_dim_and_type(p.head_dim, bf, [&](auto d, auto t) {
     return launch_merge<decltype(d)::value, decltype(t)>(m, p.batch, stride, stream);
   });

@@ -80,3 +80,57 @@ def test_fp8_scales_without_a_value(d, bad, block):
     assert torch.isnan(got[sees]).all()
     err, tol = row_errors(got.masked_fill(sees[..., None], 0), q, *case.kv, causal=True, lens=LENS)
     assert (err <= tol)[~sees].all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("split", [None, 192])
+def test_rows_of_v_that_a_shorter_request_does_not_hold(fp8, dtype, d, split):
+    """V rows of shared keys are NaN or infinite: the rows that see one are no numbers, all others are what they are without
+    them, also where the bad row lies in their own last tile, page or partition."""
+    announce(f"shared bad rows of V fp8={fp8} {dtype} d={d} split={split}")
+    lens = [650, 100, 0, 700, 391, 399, 400, 401, 402, 640, 384, 130, 131]
+    case = Case([len(lens)], [640], lens, d=d, page=64, fp8=fp8, dtype=dtype)
+    for bad, key in ((math.nan, 400), (math.inf, 400), (-math.inf, 129), (math.nan, 639)):
+        if fp8 and bad != math.nan:
+            bad = math.nan
+        page = int(case.table[0, key // 64])
+        row = case.v[page, :, key % 64]
+        keep = row.view(torch.uint8).clone()
+        if fp8:
+            row.view(torch.uint8).fill_(0x7f)
+        else:
+            row.fill_(bad)
+        for nq, causal in ((1, False), (3, True), (40, True)):
+            q = case.q(8, nq, dtype)
+            got = case.call(q, causal=causal, split_len=split)
+            sees = torch.tensor([[key < (n - nq + 1 + i if causal else n) for i in range(nq)] for n in lens], device="cuda")
+            sees = sees[:, None].expand(-1, 8, -1)
+            assert sees.any() and not sees.all()
+            if math.isnan(bad):
+                assert torch.isnan(got[sees]).all()
+            else:
+                assert (got[sees] == bad).all()
+            err, tol = row_errors(got.masked_fill(sees[..., None], 0), q, *case.kv, causal=causal, lens=lens)
+            assert (err <= tol)[~sees].all(), (bad, key, nq)
+        row.view(torch.uint8).copy_(keep)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_bad_rows_of_v_in_groups_of_their_own(page):
+    """Several groups, long partitions, a negative scale, pools in another layout: the short requests' rows are those of the same
+    pools without the bad rows."""
+    lens = [3300, 40, 700, 3001, 900, 20, 1000]
+    case = Case([4, 3], [3000, 900], lens, hkv=2, d=128, page=page)
+    pools = [p.transpose(1, 2).contiguous().transpose(1, 2) for p in (case.k, case.v)]
+    case.k, case.v = pools
+    q = case.q(8, 2)
+    want = case.call(q, causal=True, scale=-0.1)
+    for i, key in ((0, 1500), (4, 60)):
+        case.v[int(case.table[i, key // page]), :, key % page] = math.inf
+    got = case.call(q, causal=True, scale=-0.1)
+    for i in (1, 2, 5):  # 40, 700, 20 keys
+        assert ((got[i].double() - want[i].double()).norm(dim=-1) <= 2.0 ** -6 * (1 + want[i].double().norm(dim=-1))).all()
+    for i in (0, 3, 4, 6):
+        assert torch.isposinf(got[i]).all()
