@@ -109,7 +109,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   }
   PrefillItem it;
   int b0 = 0, b1 = 0;     // SHARED: the group's requests,
-  int shared = 0, part = 0;  // its shared keys, and the workgroup's partition of them
+  int prefix = 0, shared = 0, part = 0;  // its prefix, the shared keys of it, and the workgroup's partition of them
   if constexpr (SHARED) {
     // kv-head innermost (8 of them: one to an XCD, whose L2 then holds its keys), then the row blocks, which read the
     // same keys at about the same time, then the key partitions
@@ -118,7 +118,8 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     it.kvh = item - rest * a.hkv;
     part = a.shared.by_prefix_blocks.of(rest);
     it.rb = rest - part * a.n_rowblk;
-    if (!group_of_block(a.shared, a.group * a.nq, NW * 32, it.rb, b0, b1, shared)) return;  // uniform over the workgroup
+    if (!group_of_block(a.shared, a.group * a.nq, NW * 32, it.rb, b0, b1, prefix)) return;  // uniform over the workgroup
+    shared = shared_keys(a.shared, prefix);
     if (part * a.shared.prefix_split >= shared) return;
     it.b = b0;  // (the request whose table row is read: below)
     it.hq = it.kvh * a.group;
@@ -488,7 +489,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (SHARED) {
     // a row sees the shared keys that its request has, up to its own causal end
-    const int n = keys_of(a.shared, row_len, seq_k);
+    const int n = keys_of(a.shared, row_len, prefix);
     qlim = (a.causal ? n - a.nq + nqi : n - 1);
     int least = row_ok ? max(qlim + 1, 0) : khi;
 #pragma unroll

@@ -149,8 +149,8 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const MergeArgs a) {
   const int b = a.by_chunks.of((int)blockIdx.x), chunk = (int)blockIdx.x - b * a.chunks;
   const int tid = (int)threadIdx.x, dq = tid % TPR, way = tid / TPR % WAYS, sub = tid / (TPR * WAYS);
   const int rows = a.hq * a.nq, r = chunk * ROWS + sub;  // (q-head, query) of the request
-  const int shared = shared_keys_of(a.shared, b);
-  const int keys = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens[b]), shared);
+  const int prefix = prefix_of_request(a.shared, b), shared = shared_keys(a.shared, prefix);
+  const int keys = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens[b]), prefix);
   const int first = a.by_prefix_split.of(shared + a.shared.prefix_split - 1);
   const int count = r < rows ? first + (keys > shared ? a.by_suffix_split.of(keys - shared + a.shared.suffix_split - 1) : 0) : 0;
   const int skip = a.shared.part_base - first;  // places between the two runs of a row's partials
@@ -328,8 +328,8 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   a.shared.cu_groups = s.cu_groups;
   a.shared.groups = s.cu_groups != nullptr ? s.num_groups : 1;
   a.shared.batch = p.batch;
-  a.shared.max_prefix = plan.max_prefix;
-  a.shared.max_suffix = plan.max_suffix;
+  a.shared.max_prefix = s.max_prefix_len;
+  a.shared.max_suffix = s.max_suffix_len;
   a.shared.table_keys = (int32_t)std::min<int64_t>((int64_t)kv.block_table_cols * kv.page_size, INT32_MAX);
   a.shared.part_stride = stride;
   a.shared.part_base = plan.prefix_parts;

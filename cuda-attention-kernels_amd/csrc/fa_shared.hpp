@@ -53,7 +53,7 @@ struct SharedArgs {
   const int32_t* prefix_lens;  // [groups], or NULL: max_prefix for every group
   const int32_t* cu_groups;    // [groups + 1], or NULL: one group of the whole batch
   int32_t groups, batch;
-  int32_t max_prefix, max_suffix;  // bounds of the shared keys, and of a request's keys behind them
+  int32_t max_prefix, max_suffix;  // bounds of the prefixes, and of a request's keys behind its own
   int32_t table_keys;              // keys that a block-table row can name
   int32_t part_base, part_stride;  // a row's partials: part_stride of them, those of its own keys from part_base on
   int32_t prefix_split, suffix_split;  // keys per partition
@@ -67,15 +67,17 @@ struct SharedTileArgs : TileArgs {
   SharedArgs shared;
 };
 
-// Shared keys of group g (in range).
-__device__ __forceinline__ int shared_keys(const SharedArgs& s, int g) {
-  const int p = s.prefix_lens != nullptr ? min(max(s.prefix_lens[g], 0), s.max_prefix) : s.max_prefix;
-  return min(p, s.table_keys) / kPrefixUnit * kPrefixUnit;
+// The prefix of group g (in range), and how many of its keys are shared.
+__device__ __forceinline__ int prefix_of(const SharedArgs& s, int g) {
+  return s.prefix_lens != nullptr ? min(max(s.prefix_lens[g], 0), s.max_prefix) : s.max_prefix;
+}
+__device__ __forceinline__ int shared_keys(const SharedArgs& s, int prefix) {
+  return min(prefix, s.table_keys) / kPrefixUnit * kPrefixUnit;
 }
 
-// Keys that request b is read to have, behind `shared` shared ones.
-__device__ __forceinline__ int keys_of(const SharedArgs& s, int seqlen, int shared) {
-  return min(max(seqlen, 0), min(shared + s.max_suffix, s.table_keys));
+// Keys that a request is read to have, behind a prefix of `prefix`.
+__device__ __forceinline__ int keys_of(const SharedArgs& s, int seqlen, int prefix) {
+  return min(max(seqlen, 0), min(prefix + s.max_suffix, s.table_keys));
 }
 
 // Requests [b0, b1) of group g (in range), within the batch whatever cu_groups holds.
@@ -88,16 +90,16 @@ __device__ __forceinline__ void group_range(const SharedArgs& s, int g, int& b0,
   }
 }
 
-// Shared keys of request b (uniform over the wave; every lane calls it).  A request of no group has none.
-__device__ __forceinline__ int shared_keys_of(const SharedArgs& s, int b) {
-  if (s.cu_groups == nullptr) return __builtin_amdgcn_readfirstlane(shared_keys(s, 0));
+// The prefix of request b (uniform over the wave; every lane calls it).  A request of no group has none.
+__device__ __forceinline__ int prefix_of_request(const SharedArgs& s, int b) {
+  if (s.cu_groups == nullptr) return __builtin_amdgcn_readfirstlane(prefix_of(s, 0));
   const int lane = (int)threadIdx.x & 63;
   for (int base = 0; base < s.groups; base += 64) {
     const int g = base + lane;
     int b0 = 0, b1 = 0, keys = 0;
     if (g < s.groups) {
       group_range(s, g, b0, b1);
-      keys = shared_keys(s, g);  // (every lane its group's: the loads are in flight together)
+      keys = prefix_of(s, g);  // (every lane its group's: the loads are in flight together)
     }
     const uint64_t in = __builtin_amdgcn_ballot_w64(b0 <= b && b < b1);
     if (in != 0) return __builtin_amdgcn_readlane(keys, __builtin_ctzll(in));
@@ -105,21 +107,21 @@ __device__ __forceinline__ int shared_keys_of(const SharedArgs& s, int b) {
   return 0;
 }
 
-// The requests [b0, b1) and shared keys of the group that row block `rb` belongs to, and the block within it, when a group
+// The requests [b0, b1) and the prefix of the group that row block `rb` belongs to, and the block within it, when a group
 // of n requests has ceil(n * rows_each / rows) blocks (uniform; every lane calls it).  False past the last block.
-__device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_each, int rows, int& rb, int& b0, int& b1, int& keys) {
+__device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_each, int rows, int& rb, int& b0, int& b1, int& prefix) {
   const int lane = (int)threadIdx.x & 63;
   if (s.cu_groups == nullptr) {
     b0 = 0;
     b1 = s.batch;
-    keys = __builtin_amdgcn_readfirstlane(shared_keys(s, 0));
+    prefix = __builtin_amdgcn_readfirstlane(prefix_of(s, 0));
     return rb < (s.batch * rows_each + rows - 1) / rows;
   }
   for (int base = 0; base < s.groups; base += 64) {
     int lo = 0, hi = 0, k = 0;
     if (base + lane < s.groups) {
       group_range(s, base + lane, lo, hi);
-      k = shared_keys(s, base + lane);
+      k = prefix_of(s, base + lane);
     }
     const int blocks = ((hi - lo) * rows_each + rows - 1) / rows;
     int end = blocks;
@@ -131,7 +133,7 @@ __device__ __forceinline__ bool group_of_block(const SharedArgs& s, int rows_eac
     const uint64_t in = __builtin_amdgcn_ballot_w64(end > rb);
     if (in != 0) {
       const int at = __builtin_ctzll(in);
-      keys = __builtin_amdgcn_readlane(k, at);
+      prefix = __builtin_amdgcn_readlane(k, at);
       b0 = __builtin_amdgcn_readlane(lo, at);
       b1 = __builtin_amdgcn_readlane(hi, at);
       rb -= __builtin_amdgcn_readlane(end - blocks, at);

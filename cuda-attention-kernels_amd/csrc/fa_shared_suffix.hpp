@@ -58,8 +58,8 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
   const SharedArgs& sh = a.shared;
   const int i1 = sh.by_suffix_blocks.of(item), i2 = sh.by_hkv.of(i1), part = sh.by_batch.of(i2);
   const int rb = item - i1 * sh.suffix_blocks, kvh = i1 - i2 * a.hkv, b = i2 - part * a.batch;
-  const int start = shared_keys_of(a.shared, b);
-  const int limit = min(start + a.shared.max_suffix, a.shared.table_keys);
+  const int prefix = prefix_of_request(a.shared, b), start = shared_keys(a.shared, prefix);
+  const int limit = min(prefix + a.shared.max_suffix, a.shared.table_keys);
   const int klo = start + part * a.shared.suffix_split;
 
   const int lane = (int)threadIdx.x & 63, g = lane >> 5, j = lane & 31;
@@ -91,7 +91,7 @@ __device__ __forceinline__ void suffix_rows(const SharedTileArgs& a, int item, u
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = (ld16(qp + 16 * s) ^ qsign) & keep;
   }
-  const int seq_k = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens_k[b]), start);
+  const int seq_k = keys_of(a.shared, __builtin_amdgcn_readfirstlane(a.seqlens_k[b]), prefix);
   if (klo >= seq_k) return;  // (the merge does not read this partial)
   __builtin_amdgcn_sched_barrier(0);  // Q's loads stay ahead of the first tile's
 

@@ -42,8 +42,8 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     ``max_prefix_len`` and ``max_suffix_len`` size the grid: the largest of prefix_lens, and of a request's keys behind
     its group's prefix.  When omitted they are read from the device, which waits for it; as numbers, they let the call be
     captured into a graph.  Longer prefixes than max_prefix_len are shared up to it, the rest of them counts as own
-    keys; keys past max_suffix_len of their own are not read.  ``split_len``: keys per partition, a multiple of 64 that spans
-    at most 128 pages (of FP8 pools: at most 4096 keys)."""
+    keys; a request with more than max_suffix_len keys of its own counts as one that ends there (its causal queries too).
+    ``split_len``: keys per partition, a multiple of 64 that spans at most 128 pages (of FP8 pools: at most 4096 keys)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     number = not isinstance(prefix_lens, torch.Tensor)
     if _hip.native is not None and max_suffix_len is not None and not return_lse and split_len is None \
@@ -55,6 +55,9 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             return o
     _hip.check_shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups)
     if not q.is_cuda or _pick_backend(q) != "hip":
+        if max_suffix_len is not None:
+            longest = _prefixes(seqlens_k, prefix_lens, cu_groups, max_prefix_len) + max(0, int(max_suffix_len))
+            seqlens_k = torch.minimum(seqlens_k.long(), longest).to(torch.int32)
         return attention_paged(q, k_cache, v_cache, block_table, seqlens_k, causal=causal, scale=scale, return_lse=return_lse,
                                k_scale=k_scale, v_scale=v_scale)
     if max_prefix_len is None:
@@ -68,15 +71,22 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                               return_lse=return_lse, k_scale=k_scale, v_scale=v_scale)
 
 
+def _prefixes(seqlens_k: torch.Tensor, prefix_lens, cu_groups: Optional[torch.Tensor],
+              max_prefix_len: Optional[int]) -> torch.Tensor:
+    """The prefix of every request (int64 [B]), at most max_prefix_len; 0 for one of no group."""
+    b, dev = seqlens_k.numel(), seqlens_k.device
+    groups = 1 if cu_groups is None else cu_groups.numel() - 1
+    p = prefix_lens.long() if isinstance(prefix_lens, torch.Tensor) else torch.full((groups,), int(prefix_lens), device=dev)
+    p = p.clamp(min=0, max=None if max_prefix_len is None else max(0, int(max_prefix_len)))
+    if cu_groups is None:
+        return p.expand(b)
+    request = torch.arange(b, device=dev)
+    group = torch.searchsorted(cu_groups[1:].long().contiguous(), request, right=True)
+    return torch.where((request >= cu_groups[0]) & (group < groups), p[group.clamp(max=groups - 1)], 0)
+
+
 def _longest_suffix(seqlens_k: torch.Tensor, prefix_lens, cu_groups: Optional[torch.Tensor], max_prefix_len: int) -> int:
     """The most keys that a request has behind what its group shares (at most max_prefix_len)."""
     if seqlens_k.numel() == 0:
         return 0
-    if isinstance(prefix_lens, torch.Tensor):
-        p = prefix_lens.long().clamp(min=0, max=max(0, int(max_prefix_len)))
-        if cu_groups is not None:
-            request = torch.arange(seqlens_k.numel(), device=seqlens_k.device)
-            p = p[torch.searchsorted(cu_groups[1:].long().contiguous(), request, right=True).clamp(max=p.numel() - 1)]
-    else:
-        p = max(0, min(int(prefix_lens), int(max_prefix_len)))
-    return max(0, int((seqlens_k.long() - p).max().item()))
+    return max(0, int((seqlens_k.long() - _prefixes(seqlens_k, prefix_lens, cu_groups, max_prefix_len)).max().item()))

@@ -190,7 +190,8 @@ fa_status fa_attention_paged_decode(const fa_fwd_params* p, const fa_paged_kv* k
    a group's shared keys read once for all its rows.  Group g is requests cu_groups[g] to cu_groups[g + 1] - 1, and their
    block-table rows name the same keys in the first prefix_lens[g] positions.  p->seqlen_k is unused: the grid is laid out
    for max_prefix_len shared keys and max_suffix_len keys behind them, which bound prefix_lens[g] and
-   seqlens_k[b] - prefix_lens[g] (larger values are read as these bounds allow).  A request may be shorter than its group's
+   seqlens_k[b] - prefix_lens[g]: a longer prefix is shared up to max_prefix_len, and a request with more keys behind that
+   than max_suffix_len counts as one that ends there.  A request may be shorter than its group's
    prefix, and then sees the keys that it has. */
 typedef struct fa_shared_prefix {
   const int32_t* prefix_lens; /* [num_groups] on the device, or NULL: max_prefix_len for every group */
