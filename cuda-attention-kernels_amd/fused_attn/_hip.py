@@ -981,6 +981,16 @@ def check_shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens
             raise RuntimeError(f"all tensors must be on {q.device}, got {t.device}")
 
 
+MAX_SHARED_LEN = 1 << 29  # what fa_attention_shared_prefix takes of max_prefix_len, max_suffix_len and split_len
+
+
+def check_shared_bounds(**bounds) -> None:
+    """Numbers that go into 32-bit fields, or None."""
+    for name, value in bounds.items():
+        if value is not None and int(value) > MAX_SHARED_LEN:
+            raise RuntimeError(f"{name} must be at most 2^29, got {value}")
+
+
 def shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups, max_prefix_len: int,
                   max_suffix_len: int, causal: bool = False, scale: Optional[float] = None, split_len: Optional[int] = None,
                   return_lse: bool = False, k_scale=None, v_scale=None):

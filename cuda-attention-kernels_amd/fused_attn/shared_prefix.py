@@ -43,7 +43,8 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     its group's prefix.  When omitted they are read from the device, which waits for it; as numbers, they let the call be
     captured into a graph.  Longer prefixes than max_prefix_len are shared up to it, the rest of them counts as own
     keys; a request with more than max_suffix_len keys of its own counts as one that ends there (its causal queries too).
-    ``split_len``: keys per partition, a multiple of 64 that spans at most 128 pages (of FP8 pools: at most 4096 keys)."""
+    ``split_len``: keys per partition, a multiple of 64 that spans at most 128 pages (of FP8 pools: at most 4096 keys).  All
+    three are at most 2^29."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     number = not isinstance(prefix_lens, torch.Tensor)
     if _hip.native is not None and max_suffix_len is not None and not return_lse and split_len is None \
@@ -54,10 +55,12 @@ def attention_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         if o is not None:
             return o
     _hip.check_shared_prefix(q, k_cache, v_cache, block_table, seqlens_k, prefix_lens, cu_groups)
+    longest = [int(n) for n in (max_prefix_len, prefix_lens if number else None) if n is not None]
+    _hip.check_shared_bounds(max_prefix_len=min(longest) if longest else None, max_suffix_len=max_suffix_len, split_len=split_len)
     if not q.is_cuda or _pick_backend(q) != "hip":
         if max_suffix_len is not None:
-            longest = _prefixes(seqlens_k, prefix_lens, cu_groups, max_prefix_len) + max(0, int(max_suffix_len))
-            seqlens_k = torch.minimum(seqlens_k.long(), longest).to(torch.int32)
+            end = _prefixes(seqlens_k, prefix_lens, cu_groups, max_prefix_len) + max(0, int(max_suffix_len))
+            seqlens_k = torch.minimum(seqlens_k.long(), end).to(torch.int32)
         return attention_paged(q, k_cache, v_cache, block_table, seqlens_k, causal=causal, scale=scale, return_lse=return_lse,
                                k_scale=k_scale, v_scale=v_scale)
     if max_prefix_len is None:

@@ -4,6 +4,7 @@ import torch
 
 from helpers import announce
 from shared_helpers import Case
+from test_shared_bounds_cpu import check_refused
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +39,9 @@ def test_the_bound_is_counted_from_the_prefix_as_it_is_shared():
         for bound in (0, 50, 64):
             case.lens = [min(n, min(p, most) + bound) for n, p in zip(full, start)]
             case.check(case.call(q, causal=True, max_prefix_len=most, max_suffix_len=bound), q, True)
+
+
+def test_bounds_that_do_not_fit_are_refused():
+    case = Case([3, 2], [70, 20], [75, 70, 130, 21, 90], page=16)
+    case.call(case.q(4, 2))
+    check_refused(case, case.q(4, 2))

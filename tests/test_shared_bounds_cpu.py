@@ -29,3 +29,22 @@ def test_prefixes_of_requests():
     p = torch.tensor([5, 6, -7], dtype=torch.int32)
     assert shared_prefix._prefixes(lens, p, cu, 4).tolist() == [0, 4, 4, 0, 0, 0]
     assert shared_prefix._prefixes(lens, p[:1], None, None).tolist() == [5] * 6
+
+
+BEYOND = [2 ** 29 + 1, 2 ** 31, 2 ** 32, 2 ** 32 + 64]  # the last two are 0 and 64 in 32 bits
+
+
+def check_refused(case, q):
+    for n in BEYOND:
+        for kw in ({"max_prefix_len": n}, {"max_suffix_len": n}, {"max_suffix_len": n, "max_prefix_len": 70}, {"split_len": n},
+                   {"prefix_lens": n}, {"prefix_lens": n, "max_suffix_len": 60}, {"prefix_lens": 70, "max_suffix_len": n}):
+            with pytest.raises(RuntimeError, match="2\\^29"):
+                case.call(q, **kw)
+    # the lesser of two bounds of the prefix counts
+    assert torch.equal(case.call(q, prefix_lens=2 ** 32, max_prefix_len=64, max_suffix_len=600),
+                       case.call(q, prefix_lens=64, max_suffix_len=600))
+
+
+def test_bounds_that_do_not_fit_are_refused():
+    case = Case([3, 2], [70, 20], [75, 70, 130, 21, 90], page=16, device="cpu")
+    check_refused(case, case.q(4, 2, torch.bfloat16))
