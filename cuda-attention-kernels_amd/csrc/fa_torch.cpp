@@ -208,6 +208,14 @@ bool int32s(const at::Tensor& t, int64_t n, const c10::Device& dev) {
   return t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kInt && t.device() == dev && (n <= 1 || t.stride(0) == 1);
 }
 
+// Without the GIL from here on: an allocation or a launch may wait, and other threads of Python go on meanwhile.
+struct NoGil {
+  PyThreadState* state = PyEval_SaveThread();
+  NoGil() = default;
+  NoGil(const NoGil&) = delete;
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
 bool enabled(const c10::Device& dev) {
   const int i = dev.is_cuda() ? dev.index() : -1;
   return i >= 0 && i < 64 && ((g_devices.load(std::memory_order_acquire) >> i) & 1);
@@ -246,6 +254,7 @@ std::vector<at::Tensor> allocate_pages(const at::Tensor& table, const at::Tensor
   fa_pages_params p{};
   if (!pages_params(table, seqlens, free_pages, num_free, page_size, num_tokens, p) || !int32s(new_lens, p.batch, table.device()))
     return {};
+  const NoGil released;
   const c10::DeviceGuard guard(table.device());
   std::vector<at::Tensor> out{at::empty({num_tokens}, table.options().dtype(at::kLong)), at::empty({p.batch + 1}, table.options()),
                               at::empty({p.batch}, table.options()), at::empty(num_free.sizes(), table.options())};
@@ -268,6 +277,7 @@ std::vector<at::Tensor> release_pages(const at::Tensor& table, const at::Tensor&
       (done.scalar_type() != at::kBool && done.scalar_type() != at::kByte))
     return {};
   if (keep_lens.defined() && !int32s(keep_lens, p.batch, table.device())) return {};
+  const NoGil released;
   const c10::DeviceGuard guard(table.device());
   std::vector<at::Tensor> out{at::empty({p.batch}, table.options()), at::empty(num_free.sizes(), table.options())};
   p.done = (const uint8_t*)done.const_data_ptr();
@@ -314,6 +324,7 @@ bool append_kv_paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor&
   p.head_dim = (int32_t)k.size(2);
   p.num_pages = (int32_t)kc.size(0);
   p.page_size = (int32_t)kc.size(2);
+  const NoGil released;
   const c10::DeviceGuard guard(dev);
   return g_pages.append(&p, stream_of(dev)) == FA_OK;
 }
@@ -362,6 +373,7 @@ at::Tensor shared_prefix(const SharedCall& c) {
   }
   if (backend_forced()) return {};
 
+  const NoGil released;
   const c10::DeviceGuard guard(dev);
   at::Tensor o = at::empty(q.sizes(), q.options());
   auto step = [](const at::Tensor& x, int i) { return x.size(i) > 1 ? x.stride(i) : 0; };
