@@ -322,14 +322,16 @@ def _cache_library() -> ctypes.CDLL:
 
 
 def _has_pages(lib: ctypes.CDLL) -> bool:
-    return isinstance(getattr(lib, "fa_allocate_pages", None), lib._FuncPtr)
+    return all(isinstance(getattr(lib, name, None), lib._FuncPtr) for name in (
+        "fa_allocate_pages", "fa_release_pages", "fa_append_kv_paged", "fa_shared_prefix_workspace_bytes",
+        "fa_attention_shared_prefix"))
 
 
 def _pages_library() -> ctypes.CDLL:
     """The library, if it has the functions of pages (added within this ABI version)."""
     lib = load_library()
     if not _has_pages(lib):
-        raise RuntimeError(f"fused_attn HIP backend: {library_path()} is older than allocate_pages: build it again")
+        raise RuntimeError(f"fused_attn HIP backend: {library_path()} is older than pages and shared prefixes: build it again")
     return lib
 
 
