@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(kBlock) release_pages_kernel(const PagesArgs a
 
 // K/V rows of packed tokens to their slots, K and V in one launch: one read and one write of every row.  A thread
 // moves kCopy 16-byte pieces of K and of V, whose loads are in flight together with those of the slots.  40001 tokens of 8
-// heads x 128: 58-59 us for 328 MB, the rate of a large copy (5.1 TB/s) and the launch; 64 tokens 4.2 us.
+// heads x 128, 328 MB: 63.9 us a call on buffers in turn, 5.1 TB/s (two torch copies of the same: 65); 58-59 under the profiler on
+// the same buffers, parts of which stay in the caches; 64 tokens 4.2 us.
 constexpr int kCopy = 4;
 
 __global__ void __launch_bounds__(kBlock) append_kv_paged_kernel(const AppendPagedArgs a) {

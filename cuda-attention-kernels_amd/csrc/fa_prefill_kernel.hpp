@@ -619,7 +619,7 @@ attn_fwd_kernel(const typename FwdArgs<SHARED>::type a) {
     float m_safe = (m_run == NEG_INF) ? 0.f : m_run;
     // FP8: O is held in units of v_cur, the V block scale of a recent tile.  A tile whose scale vb is within a factor 2 of
     // it takes vb / v_cur into its exponents, and out of its row sum again; any other first brings O to its own scale.
-    // (v_scales hold units, v_units above.)
+    // (v_scales hold v_units of the scales.)
     const float c_this = score_scale(t), c_next = score_scale(t + 1);
     float unfold = 1.f;
     if constexpr (IS8) {

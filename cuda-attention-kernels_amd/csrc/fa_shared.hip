@@ -8,8 +8,8 @@
 //
 // What bounds it: the shared keys' products (matrix cores and, with as many vector cycles, the exponentials) beside the
 // stream of the own keys, and about 8 us of start and end.  64 requests of 4 rows a kv-head (8 of them, D = 128) behind
-// 8192 keys, up to 512 of their own: 27 us and the merge's 4.4; 32 of 16 rows behind 16384, up to 2000: 56 and 5.8.  Whole
-// calls 31 and 63 us; with the split-K kernels over both parts, one after the other, 70 and 114.
+// 8192 keys, up to 512 of their own: 27 us and the merge's 4.8; 32 of 16 rows behind 16384, up to 2000: 56 and 5.9.  Whole
+// calls 30 and 61 us; with the split-K kernels over both parts, one after the other, 70 and 114.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -20,7 +20,7 @@
 namespace fa {
 
 struct MergeArgs {
-  const float* part;  // [batch, hq, nq, part_stride] partials, then their (m, l) in ml
+  float* part;  // [batch, hq, nq, part_stride] partials, then their (m, l) in ml
   const float* ml;
   void* o;
   float* lse;  // optional natural-log LSE
@@ -71,7 +71,7 @@ __device__ __forceinline__ void renew_partials(int b, int r0, int shared, int ke
     const int s = a.by_prefix_split.of(limit - 1);
     return limit < min((s + 1) * a.shared.prefix_split, shared) ? s : -1;
   };
-  auto part_of = [&](int r, int s) { return (float*)a.part + (((int64_t)b * a.hq * a.nq + r) * a.shared.part_stride + s) * D; };
+  auto part_of = [&](int r, int s) { return a.part + (((int64_t)b * a.hq * a.nq + r) * a.shared.part_stride + s) * D; };
   bool spoiled = false;
   for (int i = tid; i < rows * (D / 4); i += 256) {
     int limit;
@@ -133,8 +133,8 @@ __device__ __forceinline__ void renew_partials(int b, int r0, int shared, int ke
   __syncthreads();
 }
 
-// Bound by its launch, and by the partials' bytes where they are many (2048 rows x 10 partials of D = 128: 4.6 us; a
-// workgroup for every row, the partials dealt to its threads, took 8.4; 8192 rows 8.7).  Few instructions a row: with 8
+// Bound by its launch, and by the partials' bytes where they are many (2048 rows x 10 partials of D = 128: 4.8 us; a
+// workgroup for every row, the partials dealt to its threads, took 8.4; 8192 rows 8.9).  Few instructions a row: with 8
 // partials a thread in place of 4, most of them none, and divisions by numbers that the host knows, the latter took 11.
 //
 // A thread merges 4 values of a row over every WAYS-th of its partials, CH of them in flight together; WAYS threads meet
@@ -267,14 +267,17 @@ SharedPlan plan_shared(const fa_fwd_params& p, const fa_shared_prefix& s, int pa
   // D = 128, alone on its CU or one of two) and leaves 128 rows of partials; one a CU leaves the CU's other place to the
   // requests' own keys.  So: as many as there are CUs, half as many where those would have fewer than 1024 keys each (64
   // requests of 4 rows, 8 kv-heads, 8192 keys: the call takes 42 us at 512 keys, 37 at 1024; 32 of 16 rows, 16384 keys, 66
-  // at 2048 and 86 at 4096).  A group has a block at least; which ones have more, and how long their prefixes are, is not
-  // known here.  Own keys: 1024 waves, four a CU (512 at D = 256: 49 requests of up to 700 keys, 4 kv-heads, 55 us at 192
+  // at 2048 and 86 at 4096; measured at D = 128 with one group only.  At D = 256 and with groups of 16, 24, 8 and 1 request it leaves
+  // CUs empty: 162 working workgroups on 256).  A group has a block at least; which ones have more, and how long their
+  // prefixes are, is not known here.  Own keys: 1024 waves, four a CU (512 at D = 256: 49 requests of up to 700 keys, 4 kv-heads, 55 us at 192
   // keys, 47 at 320), but no more than 576 keys each, for the last to start not to run on alone, and 320 where there are
   // many (256 requests of up to 1000 keys, 8 kv-heads, D = 64: 95 us whole, 91 at 576, 88 at 320; 32 of up to 2000: 66 at
   // 576, 72 at 320).
   constexpr int64_t kWgs = kCus, kLong = 1024, kWaves = 1024;
   auto whole = [](int64_t keys, int64_t parts) { return ((keys + parts - 1) / parts + kPrefixUnit - 1) / kPrefixUnit * kPrefixUnit; };
-  auto fits = [&](int64_t len, int64_t pages) {  // a partition spans a limited number of pages, and of FP8 scale blocks
+  // a partition spans a limited number of pages, and of FP8 scale blocks (not evened out afterwards: 4032 keys in pages of 16
+  // are cut into 1984, 1984 and 64)
+  auto fits = [&](int64_t len, int64_t pages) {
     len = std::min(len, (pages - 2) * page_size / kPrefixUnit * kPrefixUnit);
     return (int32_t)std::max<int64_t>(kPrefixUnit, fp8 ? std::min<int64_t>(len, kFp8Keys) : len);
   };
@@ -349,7 +352,7 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   a.shared.by_suffix_blocks = FastDiv::by(a.shared.suffix_blocks);
   a.n_items = (int32_t)((int64_t)p.batch * p.heads_kv * plan.suffix_parts * a.shared.suffix_blocks);
   // The shared keys' workgroups go first; where the requests' own keys take longer (an estimate: 0.65 us a tile and CU of the
-  // former, 4.5 TB/s for half of the longest of the latter), only one a CU, the rest behind the own keys' (256 requests of
+  // former, D = 128's, 4.5 TB/s for half of the longest of the latter), only one a CU, the rest behind the own keys' (256 requests of
   // up to 1000 keys behind 4080, D = 64: 82 us, 79 so; FP8, 128 of up to 700 behind 32768: 174, 183 so).
   const double prefix_us = 0.65 * plan.prefix_blocks * p.heads_kv * (plan.max_prefix / 64.0) / kCus;
   const double suffix_us = (double)p.batch * p.heads_kv * plan.max_suffix * p.head_dim * (fp8 ? 1 : 2) / 4.5e6;
@@ -360,7 +363,7 @@ fa_status run_shared(const fa_fwd_params& p, const fa_paged_kv& kv, const fa_sha
   if (e != hipSuccess) return hip_status(e, err);
 
   MergeArgs m{};
-  m.part = (const float*)a.o;
+  m.part = (float*)a.o;
   m.ml = a.ml;
   m.o = p.o;
   m.lse = p.lse;

@@ -82,7 +82,8 @@ def release_pages(block_table: torch.Tensor, seqlens_k: torch.Tensor, done: torc
 
     ``keep_lens`` (int32 [B]): keys at the start of a request that others share; the whole pages they fill stay out of
     the list.  A request whose pages the list has no room for keeps them and its length.  ``block_table`` is not changed:
-    a row's entries past its length mean nothing."""
+    a row's entries past its length mean nothing.  What a row holds is put back as it is: a negative entry too (tokens that
+    get it later have slot -1), and a page that two finished requests share twice, unless keep_lens leaves it out."""
     args = (block_table, seqlens_k, done, free_pages, num_free, int(page_size), keep_lens)
     out = None if _hip.native is None else _hip.native.release_pages(*args[:5], keep_lens, args[5])
     if out is not None:
