@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from cache_norms import check_rows, row_errors
+from cache_norms import row_errors
 from helpers import announce
 from shared_helpers import Case
 
